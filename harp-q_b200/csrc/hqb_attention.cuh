@@ -1,0 +1,204 @@
+// Work division of the tree attention, shared by its kernels.
+//
+// An item is (request, key head, row tile): the row tile's query rows (row = node * group + head
+// in group, so every row of the tile reads the same keys) against the request's keys, which are
+// cut into blocks of 64: first the cached context, then the drafted nodes (the last block of
+// either may be partly filled).  Items lie in order request, key head, row tile; the blocks of
+// all items in that order are dealt to the CTAs in equal contiguous ranges, so ragged lengths
+// balance whatever their order.  An item that spans CTAs leaves one partial result per CTA
+// (unnormalised FP32 sums, running maximum and sum of weights) in the workspace, which
+// attention_join_kernel joins in CTA order: the result depends on the grid, never on timing.
+#pragma once
+
+#include "hqb_serve.cuh"
+
+namespace hqb {
+
+constexpr uint32_t kKeyBlock = 64;
+
+struct AttnParams {
+  hqb_attention_args a;
+  hqb_paged_cache c;
+  int* error;
+  float* parts;         // [cta][2][row tile][dim_pad + 2]
+  uint32_t group;       // query heads per key head
+  uint32_t rows;        // rows of a row tile
+  uint32_t max_tiles;   // row tiles of max_new nodes
+  uint32_t dim_pad;     // padded head dimension (columns of a partial row)
+  uint32_t min_blocks;  // fewest blocks worth a CTA of its own
+  uint32_t whole;       // 1: items are not cut (a unit is an item, no partials)
+  uint32_t grid;        // CTAs of the attention kernel
+  float scale_log2;     // scale * log2(e)
+};
+
+struct Request {
+  uint32_t start, nodes, ctx;
+  uint32_t cached_blocks, blocks;  // blocks: 0 for a request without nodes
+  uint32_t tiles;
+};
+
+__device__ __forceinline__ Request load_request(const AttnParams& p, uint32_t r, uint32_t& bad) {
+  Request q;
+  const int32_t s0 = __ldg(p.a.starts + r), s1 = __ldg(p.a.starts + r + 1);
+  const int32_t c = __ldg(p.a.context_lens + r);
+  const uint32_t cap = p.a.tokens;
+  q.start = s0 < 0 ? 0u : min(static_cast<uint32_t>(s0), cap);
+  const uint32_t end = s1 < 0 ? 0u : min(static_cast<uint32_t>(s1), cap);
+  q.nodes = end > q.start ? end - q.start : 0u;
+  if (s0 < 0 || s1 < s0 || static_cast<uint32_t>(s1) > cap || q.nodes > p.a.max_new || c < 0) bad |= HQB_DEVERR_INDEX;
+  q.nodes = min(q.nodes, p.a.max_new);
+  q.ctx = static_cast<uint32_t>(max(c, 0));
+  const uint64_t room = static_cast<uint64_t>(p.a.table_stride) * p.c.page_size;
+  if (q.ctx > room) {
+    bad |= HQB_DEVERR_PAGES;
+    q.ctx = static_cast<uint32_t>(room);
+  }
+  q.cached_blocks = (q.ctx + kKeyBlock - 1) / kKeyBlock;
+  q.blocks = q.nodes == 0 ? 0u : q.cached_blocks + (q.nodes + kKeyBlock - 1) / kKeyBlock;
+  q.tiles = (q.nodes * p.group + p.rows - 1) / p.rows;
+  return q;
+}
+
+__device__ __forceinline__ uint64_t request_units(const AttnParams& p, const Request& q) {
+  return static_cast<uint64_t>(q.tiles) * p.c.kv_heads * (p.whole ? 1u : q.blocks);
+}
+
+// Sum of the units of all requests, and of those before `until`; a whole warp calls it.
+__device__ __forceinline__ uint64_t total_units(const AttnParams& p, uint32_t until, uint64_t* before, uint32_t& bad) {
+  uint64_t all = 0, early = 0;
+  for (uint32_t r = threadIdx.x & 31; r < p.a.requests; r += 32) {
+    const uint64_t u = request_units(p, load_request(p, r, bad));
+    all += u;
+    if (r < until) early += u;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    early += __shfl_xor_sync(0xffffffffu, early, o);
+  }
+  *before = early;
+  return all;
+}
+
+// CTAs that get units: at least min_blocks each, so that short work is not cut into pieces
+// smaller than the cost of joining them.
+__device__ __forceinline__ uint32_t busy_ctas(const AttnParams& p, uint64_t units) {
+  const uint64_t most = p.whole ? units : (units + p.min_blocks - 1) / p.min_blocks;
+  return static_cast<uint32_t>(most < p.grid ? most : p.grid);
+}
+
+__device__ __forceinline__ uint64_t first_unit(uint32_t cta, uint64_t units, uint32_t ctas) {
+  return units * cta / ctas;
+}
+// The CTA whose range [first_unit(i), first_unit(i + 1)) holds unit u.
+__device__ __forceinline__ uint32_t cta_of_unit(uint64_t u, uint64_t units, uint32_t ctas) {
+  return static_cast<uint32_t>(((u + 1) * ctas - 1) / units);
+}
+
+// A CTA's walk over its units, one segment (a range of one item's blocks) at a time.  Every
+// thread keeps its own copy; begin() is called by whole warps.
+struct Walk {
+  uint64_t left;   // units not yet handed out
+  uint32_t r, head, tile, unit;
+  Request q;
+  // the current segment
+  uint32_t b0, b1;
+
+  __device__ __forceinline__ bool begin(const AttnParams& p, uint32_t cta, uint32_t& bad) {
+    uint64_t before;
+    const uint64_t units = total_units(p, 0, &before, bad);
+    const uint32_t ctas = busy_ctas(p, units);
+    left = 0;
+    if (cta >= ctas) return false;
+    const uint64_t u0 = first_unit(cta, units, ctas);
+    left = first_unit(cta + 1, units, ctas) - u0;
+    // the request that holds unit u0
+    uint64_t carry = 0;
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t r0 = 0; r0 < p.a.requests; r0 += 32) {
+      uint64_t mine = 0;
+      if (r0 + lane < p.a.requests) mine = request_units(p, load_request(p, r0 + lane, bad));
+      uint64_t inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= static_cast<uint32_t>(o)) inc += up;
+      }
+      const uint32_t past = ballot(carry + inc > u0);
+      if (past != 0) {
+        const uint32_t at = __ffs(past) - 1;
+        const uint64_t skip = u0 - (carry + __shfl_sync(0xffffffffu, inc - mine, at));
+        r = r0 + at;
+        q = load_request(p, r, bad);
+        const uint32_t per_item = p.whole ? 1u : q.blocks;
+        const uint64_t item = skip / per_item;
+        unit = static_cast<uint32_t>(skip - item * per_item);
+        head = static_cast<uint32_t>(item / q.tiles);
+        tile = static_cast<uint32_t>(item - static_cast<uint64_t>(head) * q.tiles);
+        return true;
+      }
+      carry += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
+  }
+
+  // Sets b0, b1 to the next segment's blocks; r, head, tile and q name its item.
+  __device__ __forceinline__ void open(const AttnParams& p) {
+    if (p.whole) {
+      b0 = 0;
+      b1 = q.blocks;
+      left -= 1;
+    } else {
+      b0 = unit;
+      const uint64_t n = q.blocks - unit;
+      b1 = unit + static_cast<uint32_t>(n < left ? n : left);
+      left -= b1 - b0;
+    }
+  }
+  // After a segment: the next item, unless the range ended inside this one.
+  __device__ __forceinline__ void advance(const AttnParams& p, uint32_t& bad) {
+    unit = 0;
+    if (left == 0) return;
+    if (++tile < q.tiles) return;
+    tile = 0;
+    if (++head < p.c.kv_heads) return;
+    head = 0;
+    do {  // a later request has the units that are left
+      ++r;
+      q = load_request(p, r, bad);
+    } while (q.tiles == 0 && r + 1 < p.a.requests);
+  }
+  __device__ __forceinline__ bool complete() const { return b0 == 0 && b1 == q.blocks; }
+};
+
+// Slot (of a CTA's two) of a partial segment: 1 where the item begins in this CTA, else 0.
+__device__ __forceinline__ float* part_row(const AttnParams& p, uint32_t cta, uint32_t slot, uint32_t row) {
+  return p.parts + ((static_cast<uint64_t>(cta) * 2 + slot) * p.rows + row) * (p.dim_pad + 2);
+}
+
+// Address of one cached key's row in k or v (elements from the base), its page checked.
+__device__ __forceinline__ uint64_t key_offset(const AttnParams& p, const int32_t* table, uint32_t key, uint32_t head,
+                                               uint32_t& bad) {
+  const uint32_t column = key / p.c.page_size, inside = key - column * p.c.page_size;
+  uint32_t page = static_cast<uint32_t>(__ldg(table + column));
+  if (page >= p.c.num_pages) {
+    bad |= HQB_DEVERR_PAGES;
+    page = 0;
+  }
+  return page * p.c.page_stride + inside * p.c.token_stride + head * p.c.head_stride;
+}
+
+// 32 bits of the nodes that node `node` of request q sees among nodes 32*word ..
+__device__ __forceinline__ uint32_t node_mask(const AttnParams& p, const Request& q, uint32_t node, uint32_t word) {
+  uint32_t bits;
+  if (p.a.mask != nullptr) {
+    bits = __ldg(p.a.mask + static_cast<uint64_t>(q.start + node) * p.a.mask_words + word);
+  } else {
+    const int32_t n = static_cast<int32_t>(node) + 1 - static_cast<int32_t>(word * 32);  // nodes 0 .. node
+    bits = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+  }
+  const int32_t live = static_cast<int32_t>(q.nodes) - static_cast<int32_t>(word * 32);
+  return live >= 32 ? bits : live <= 0 ? 0u : bits & ((1u << live) - 1u);
+}
+
+}  // namespace hqb

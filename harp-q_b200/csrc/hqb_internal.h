@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "harpq_b200.h"
 
 namespace hqb {
@@ -24,6 +26,21 @@ inline cudaError_t take_prior_error() { return cudaGetLastError(); }
 
 int device_sm_count(int device);
 
+// Devices (bits) on which a kernel's dynamic shared memory limit has been raised.
+using DeviceOnce = std::atomic<uint64_t>;
+
+// Raises a kernel's dynamic shared memory limit on the current device, once per device.
+inline cudaError_t allow_dynamic_smem(DeviceOnce& done, const void* kernel, uint32_t bytes) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 // The int8-limb GEMV on the reference's raw layout (hqb_raw_i8.cu): 128x128 tiles,
 // group 128, prefix 1..4, batch one, FP32 x / y.  HQB_ERR_UNSUPPORTED (nothing
 // enqueued) when the geometry, alignment or shared-memory size rules it out.
@@ -38,5 +55,8 @@ struct RawI8Launch {
 };
 int launch_raw_i8(const RawI8Launch& a, void* stream);
 uint32_t raw_i8_smem_bytes(uint64_t padded_cols);
+
+// Whether a paged cache's description (its pointers aside) can be used at all (hqb_page.cu).
+bool paged_cache_ok(const hqb_paged_cache* c);
 
 }  // namespace hqb

@@ -21,7 +21,7 @@ import torch
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "lib" / "libharpq_b200.so"
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2  # BF16: serving operators only
 FLAG_PDL, FLAG_SIMT, FLAG_RING, FLAG_TCGEN05, FLAG_STREAMK, FLAG_ROWBLOCK = 1, 2, 4, 8, 16, 32
 FLAG_F16MMA = 64  # keep the GEMV kernels on FP16-fragment MMAs (no int8 activation limbs)
 FLAG_BULK = 128  # bulk-copy kernel (batch <= 2, raw x): default for large layers, forced by this flag
@@ -31,7 +31,8 @@ TILE = 128
 RECORD_BYTES = 4352
 MAX_STAGES = 4
 MAX_BATCH = 16
-DEVERR_SCALE, DEVERR_DEPTH, DEVERR_TIMEOUT, DEVERR_LAUNCH = 1, 2, 4, 8
+DEVERR_SCALE, DEVERR_DEPTH, DEVERR_TIMEOUT, DEVERR_LAUNCH, DEVERR_PAGES, DEVERR_INDEX = 1, 2, 4, 8, 16, 32
+MAX_NODES, MAX_HEAD_DIM, MAX_RANK = 256, 256, 128
 HQB_OK, HQB_ERR_INVALID, HQB_ERR_UNSUPPORTED = 0, 1, 801
 NOALLOC_SCRATCH_BYTES = 4 << 20
 ERR_SCRATCH_LIMIT = 20001
@@ -80,6 +81,33 @@ class GatherC(ctypes.Structure):
                 ("peer_flags", vp * MAX_PEERS)]
 
 
+class PagedCacheC(ctypes.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("page_stride", u64), ("token_stride", u64), ("head_stride", u64),
+                ("dtype", i32), ("kv_heads", u32), ("head_dim", u32), ("page_size", u32), ("num_pages", u32),
+                ("reserved", u32)]
+
+
+class PagePlanC(ctypes.Structure):
+    _fields_ = [*[(n, u32) for n in ("requests", "page_size", "num_pages", "table_stride", "token_capacity",
+                                     "free_count", "mask_words", "reserved")],
+                *[(n, vp) for n in ("context_lens", "new_lens", "held", "free_pages", "free_head", "parents", "tables",
+                                    "starts", "token_request", "positions", "slots", "held_out", "free_head_out",
+                                    "mask", "flags")]]
+
+
+class AttentionC(ctypes.Structure):
+    _fields_ = [*[(n, u32) for n in ("requests", "tokens", "max_new", "max_context", "q_heads", "table_stride",
+                                     "mask_words")], ("scale", ctypes.c_float),
+                *[(n, vp) for n in ("starts", "context_lens", "tables", "mask", "q", "k", "v", "out", "lse")],
+                *[(n, u64) for n in ("q_token_stride", "q_head_stride", "kv_token_stride", "kv_head_stride",
+                                     "out_token_stride", "out_head_stride")]]
+
+
+class LoraSetC(ctypes.Structure):
+    _fields_ = [("a", vp), ("b", vp), ("ranks", vp), ("scales", vp), ("rows", u64), ("cols", u64), ("adapters", u32),
+                ("max_rank", u32), ("dtype", i32), ("reserved", u32)]
+
+
 EXPORTS = {
     "hqb_version": (i32, []),
     "hqb_status_string": (ctypes.c_char_p, [i32]),
@@ -120,6 +148,12 @@ EXPORTS = {
     "hqb_decode_planes": (i32, [ctypes.POINTER(PlaneMatrixC), u32, vp, vp, u64, vp]),
     "hqb_prefill_workspace_bytes": (u64, [ctypes.POINTER(PlaneMatrixC)]),
     "hqb_prefill_gemm": (i32, [ctypes.POINTER(PlaneMatrixC), u32, vp, i32, u32, vp, i32, vp, i32, vp, u64, vp]),
+    "hqb_page_plan": (i32, [vp, vp]),
+    "hqb_cache_append": (i32, [vp, vp, vp, i32, u64, u64, u32, vp, vp, u32, vp, vp]),
+    "hqb_tree_attention_workspace_bytes": (u64, [vp, vp, i32]),
+    "hqb_tree_attention": (i32, [vp, vp, vp, u64, vp]),
+    "hqb_lora_workspace_bytes": (u64, [vp, u32, i32]),
+    "hqb_lora": (i32, [vp, vp, u64, vp, u32, vp, u64, vp, i32, u64, vp, u64, vp]),
     "hqb_raw_gemv": (i32, [ctypes.POINTER(Geometry), ctypes.POINTER(RawStage), u32, u32, vp, u64, vp, u64, vp, u64,
                            vp]),
     "hqb_raw_gemv_ex": (i32, [ctypes.POINTER(Geometry), ctypes.POINTER(RawStage), u32, u32, vp, u64, vp, u64, vp,
@@ -543,6 +577,256 @@ class RawMatrix:
                                            _ptr(x), x.shape[0], _ptr(bias), _ptr(y), _stream(stream)),
               "hqb_raw_linear_ordered")
         return y
+
+
+# ---- serving operators: paged cache, drafted trees, adapters ------------------------------
+
+_SERVING_DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
+_ROW_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _ints(name: str, t: torch.Tensor | None, shape: tuple, device) -> None:
+    """Checks an int32 index tensor of a serving call."""
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()
+                          or t.device != device):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on {device}")
+
+
+class PagePlan:
+    """One decode step's lengths as addresses (hqb_page_plan), in buffers that are kept between
+    steps: starts [requests + 1], requests, positions and slots [tokens] (entries past the
+    step's last token are -1), held [requests], free_head [1], mask [tokens, words] (with
+    max_new > 0: trees of up to that many nodes) and flags [1] (HQB_DEVERR_* bits, OR-ed)."""
+
+    def __init__(self, requests: int, tokens: int, page_size: int, num_pages: int, max_new: int = 0, device=None):
+        if requests < 1 or tokens < 1 or page_size < 1 or num_pages < 1:
+            raise ValueError("requests, tokens, page_size and num_pages must be positive")
+        if not 0 <= max_new <= MAX_NODES:
+            raise ValueError(f"max_new must be 0..{MAX_NODES}")
+        self.device = torch.empty(0, device=device or "cuda").device
+        self.page_size, self.num_pages, self.words = page_size, num_pages, -(-max_new // 32)
+
+        def ints(n):
+            return torch.zeros(n, dtype=torch.int32, device=self.device)
+
+        self.starts, self.requests, self.positions, self.slots = ints(requests + 1), ints(tokens), ints(tokens), ints(tokens)
+        self.held, self.free_head, self.flags = ints(requests), ints(1), ints(1)
+        self.mask = torch.zeros(tokens, self.words, dtype=torch.int32, device=self.device) if self.words else None
+
+    def build(self, context_lens: torch.Tensor, new_lens: torch.Tensor, held: torch.Tensor | None = None,
+              tables: torch.Tensor | None = None, free_pages: torch.Tensor | None = None,
+              free_head: torch.Tensor | None = None, parents: torch.Tensor | None = None, stream=None) -> "PagePlan":
+        """Fills the buffers.  tables [requests, columns] (with free_pages and free_head) also gives the
+        new tokens pages and slots, writing new columns into it; parents [tokens or more] gives
+        tree positions and masks.  held and free_head are the counts before the step (pass the
+        previous plan's, not this one's)."""
+        n = self.held.numel()
+        _ints("context_lens", context_lens, (n,), self.device)
+        _ints("new_lens", new_lens, (n,), self.device)
+        _ints("held", held, (n,), self.device)
+        stride = free = 0
+        if tables is not None:
+            if free_pages is None or free_head is None:
+                raise ValueError("tables need free_pages and free_head")
+            stride, free = tables.shape[-1], free_pages.numel()
+            _ints("tables", tables, (n, stride), self.device)
+            _ints("free_pages", free_pages, (free,), self.device)
+            _ints("free_head", free_head, (1,), self.device)
+        if parents is not None:
+            _ints("parents", parents, (parents.numel(),), self.device)
+            if self.mask is None:
+                raise ValueError("parents need a plan with max_new > 0")
+        paged = tables is not None
+        args = PagePlanC(n, self.page_size, self.num_pages, stride, self.slots.numel(), free,
+                         self.words if parents is not None else 0, 0, _ptr(context_lens), _ptr(new_lens), _ptr(held),
+                         _ptr(free_pages) if paged else None, _ptr(free_head) if paged else None, _ptr(parents),
+                         _ptr(tables), _ptr(self.starts), _ptr(self.requests), _ptr(self.positions),
+                         _ptr(self.slots) if paged else None, _ptr(self.held) if paged else None,
+                         _ptr(self.free_head) if paged else None, _ptr(self.mask) if parents is not None else None,
+                         _ptr(self.flags))
+        check(lib().hqb_page_plan(ctypes.addressof(args), _stream(stream)), "hqb_page_plan")
+        return self
+
+
+class PagedCache:
+    """A paged cache over two device tensors k, v [pages, page_size, heads, dim] (FP16 or BF16;
+    any strides with adjacent elements within a head, the same for both: a cache that stores
+    heads before tokens is passed as its transpose(1, 2))."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must be [pages, page_size, heads, dim] tensors of one shape, layout, type and device")
+        if k.dtype not in _SERVING_DTYPES:
+            raise TypeError(f"unsupported dtype {k.dtype}; use float16 or bfloat16")
+        if k.stride(3) != 1:
+            raise ValueError("a head's elements must be adjacent")
+        self.k, self.v = k, v
+        self.num_pages, self.page_size, self.heads, self.dim = k.shape
+        self.device = k.device
+        self.flags = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self.c = PagedCacheC(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), _SERVING_DTYPES[k.dtype],
+                             self.heads, self.dim, self.page_size, self.num_pages, 0)
+        self._at = ctypes.addressof(self.c)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor | None = None,
+               stream=None) -> None:
+        """Writes rows of k and v [tokens, heads, dim] (FP16, BF16 or FP32) into the cache's slots
+        [count]: row rows[i], or i, goes to slots[i]; negative ones are skipped.  flags collects
+        HQB_DEVERR_* bits."""
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != self.heads or k.shape[2] != self.dim:
+            raise ValueError(f"k and v must be [tokens, {self.heads}, {self.dim}]")
+        if k.dtype != v.dtype or k.dtype not in _ROW_DTYPES:
+            raise TypeError("k and v must share a type: float16, bfloat16 or float32")
+        if k.stride() != v.stride() or (self.dim > 1 and k.stride(2) != 1) or k.device != self.device or v.device != self.device:
+            raise ValueError("k and v must share strides (adjacent elements within a head) and the cache's device")
+        n = slots.numel()
+        _ints("slots", slots, (n,), self.device)
+        _ints("rows", rows, (n,), self.device)
+        if rows is None and n > k.shape[0]:
+            raise ValueError("more slots than rows")
+        check(lib().hqb_cache_append(self._at, _ptr(k), _ptr(v), _ROW_DTYPES[k.dtype], k.stride(0), k.stride(1),
+                                     k.shape[0], _ptr(rows), _ptr(slots), n, _ptr(self.flags), _stream(stream)),
+              "hqb_cache_append")
+
+
+class TreeAttention:
+    """Attention of drafted trees over a paged cache (hqb_tree_attention) for steps of up to
+    `requests` requests, `tokens` tokens in all, max_new nodes and about max_context cached
+    tokens a request; holds the call's workspace, so calls that overlap need one each."""
+
+    def __init__(self, cache: PagedCache, q_heads: int, requests: int, tokens: int, max_new: int, max_context: int):
+        if q_heads < 1 or q_heads % cache.heads != 0:
+            raise ValueError("q_heads must be a multiple of the cache's heads")
+        if not 1 <= max_new <= MAX_NODES:
+            raise ValueError(f"max_new must be 1..{MAX_NODES}")
+        if not 1 <= cache.dim <= MAX_HEAD_DIM:
+            raise ValueError(f"the head dimension must be 1..{MAX_HEAD_DIM}")
+        if requests < 1 or tokens < 1 or max_context < 0:
+            raise ValueError("requests and tokens must be positive")
+        self.cache, self.q_heads, self.requests, self.tokens = cache, q_heads, requests, tokens
+        self.max_new, self.max_context = max_new, max_context
+        args = AttentionC(requests=requests, tokens=tokens, max_new=max_new, max_context=max_context, q_heads=q_heads)
+        index = cache.device.index
+        need = lib().hqb_tree_attention_workspace_bytes(cache._at, ctypes.addressof(args),
+                                                        torch.cuda.current_device() if index is None else index)
+        if need == 0:
+            raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
+        self.ws = Workspace(need, cache.device)
+
+    def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tables: torch.Tensor,
+                 context_lens: torch.Tensor, starts: torch.Tensor, mask: torch.Tensor | None = None,
+                 scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                 stream=None) -> torch.Tensor:
+        """out [tokens, q_heads, dim] for q [tokens, q_heads, dim] and the step's own k, v
+        [tokens, heads, dim]; request r owns tokens starts[r] .. starts[r + 1] and reads the
+        first context_lens[r] cached tokens of its row of tables [requests, columns].  mask
+        [tokens, words]: bit j of a node's row shows it node j of its request (None: the nodes
+        up to itself).  scale None: dim ** -0.5.  lse [tokens, q_heads] FP32 gets the logarithm of
+        the sum of weights."""
+        c = self.cache
+        tokens, requests = q.shape[0], context_lens.numel()
+        if out is None:
+            out = torch.empty(tokens, self.q_heads, c.dim, dtype=q.dtype, device=q.device)
+        for name, t, heads in (("q", q, self.q_heads), ("k", k, c.heads), ("v", v, c.heads), ("out", out, self.q_heads)):
+            if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != heads or t.shape[2] != c.dim:
+                raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}]")
+            if t.dtype != c.k.dtype or t.device != c.device:
+                raise TypeError(f"{name} must have the cache's type and device")
+            if c.dim > 1 and t.stride(2) != 1:
+                raise ValueError(f"{name}: a head's elements must be adjacent")
+        if k.stride() != v.stride():
+            raise ValueError("k and v must share strides")
+        if requests > self.requests or tokens > self.tokens:
+            raise ValueError(f"built for {self.requests} requests and {self.tokens} tokens, got {requests} and {tokens}")
+        columns = tables.shape[-1]
+        _ints("tables", tables, (requests, columns), c.device)
+        _ints("context_lens", context_lens, (requests,), c.device)
+        _ints("starts", starts, (requests + 1,), c.device)
+        words = 0
+        if mask is not None:
+            words = mask.shape[-1]
+            _ints("mask", mask, (mask.shape[0], words), c.device)
+            if mask.shape[0] < tokens or words * 32 < self.max_new:
+                raise ValueError(f"mask must be [{tokens}, {-(-self.max_new // 32)}] or larger")
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, self.q_heads)
+                                or not lse.is_contiguous() or lse.device != c.device):
+            raise ValueError(f"lse must be a contiguous float32 [{tokens}, {self.q_heads}] tensor")
+        args = AttentionC(requests, tokens, self.max_new, self.max_context, self.q_heads, columns, words,
+                          c.dim ** -0.5 if scale is None else scale, _ptr(starts), _ptr(context_lens), _ptr(tables),
+                          _ptr(mask), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), q.stride(0), q.stride(1),
+                          k.stride(0), k.stride(1), out.stride(0), out.stride(1))
+        check(lib().hqb_tree_attention(c._at, ctypes.addressof(args), self.ws.ptr(), self.ws.nbytes, _stream(stream)),
+              "hqb_tree_attention")
+        return out
+
+
+class LoraSet:
+    """Low-rank adapters stacked in two device tensors: a [adapters, max_rank, cols] and b
+    [adapters, rows, max_rank] (FP16 or BF16), with ranks [adapters] int32 (None: max_rank each)
+    and scales [adapters] FP32 (None: 1).  Workspaces are kept per stream."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, ranks: torch.Tensor | None = None,
+                 scales: torch.Tensor | None = None):
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError("a must be [adapters, max_rank, cols] and b [adapters, rows, max_rank]")
+        if a.dtype != b.dtype or a.dtype not in _SERVING_DTYPES:
+            raise TypeError("a and b must share a type: float16 or bfloat16")
+        if not a.is_contiguous() or not b.is_contiguous() or a.device != b.device:
+            raise ValueError("a and b must be contiguous and on one device")
+        self.adapters, self.max_rank, self.cols = a.shape
+        self.rows = b.shape[1]
+        if not 1 <= self.max_rank <= MAX_RANK:
+            raise ValueError(f"max_rank must be 1..{MAX_RANK}")
+        _ints("ranks", ranks, (self.adapters,), a.device)
+        if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (self.adapters,)
+                                   or not scales.is_contiguous() or scales.device != a.device):
+            raise ValueError(f"scales must be a contiguous float32 [{self.adapters}] tensor")
+        self.a, self.b, self.ranks, self.scales, self.device = a, b, ranks, scales, a.device
+        self.c = LoraSetC(a.data_ptr(), b.data_ptr(), _ptr(ranks), _ptr(scales), self.rows, self.cols, self.adapters,
+                          self.max_rank, _SERVING_DTYPES[a.dtype], 0)
+        self._at = ctypes.addressof(self.c)
+        self._ws: dict = {}
+
+    def workspace(self, tokens: int, stream: int) -> Workspace:
+        """The stream's workspace, grown to what `tokens` tokens need."""
+        ws = self._ws.get(stream)
+        if ws is None or tokens > ws.tokens:
+            # allocated on the stream that uses it: the allocator then reuses it in that order
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
+                ws = Workspace(lib().hqb_lora_workspace_bytes(self._at, tokens, 0), self.device)
+            ws.tokens = tokens
+            self._ws[stream] = ws
+        return ws
+
+    def apply(self, x: torch.Tensor, ids: torch.Tensor, base: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, y_dtype: torch.dtype | None = None, workspace: Workspace | None = None,
+              stream=None) -> torch.Tensor:
+        """base + scale_i * b_i (a_i x) per token, i = ids[token] (negative: base alone) (hqb_lora).
+        x [tokens, cols]; base [tokens, rows] (None: zeros) and the result share a type, the
+        set's or FP32.  out=base adds in place, e.g. to the output of a projection's gemv()."""
+        if x.dim() != 2 or x.shape[1] != self.cols or x.dtype != self.a.dtype or x.device != self.device:
+            raise ValueError(f"x must be [tokens, {self.cols}] of the set's type, on its device")
+        tokens = x.shape[0]
+        _ints("ids", ids, (tokens,), self.device)
+        if out is None:
+            kind = y_dtype or (base.dtype if base is not None else x.dtype)
+            out = torch.empty(tokens, self.rows, dtype=kind, device=self.device)
+        for name, t in (("out", out), ("base", base)):
+            if t is not None and (tuple(t.shape) != (tokens, self.rows) or t.dtype != out.dtype or t.device != self.device
+                                  or (self.rows > 1 and t.stride(1) != 1)):
+                raise ValueError(f"{name} must be [tokens, {self.rows}] with adjacent elements, of one type with the result")
+        if out.dtype != torch.float32 and out.dtype != self.a.dtype:
+            raise TypeError("the result must have the set's type or float32")
+        if tokens > 1 and min(x.stride(0) - self.cols, out.stride(0) - self.rows) < 0 or self.cols > 1 and x.stride(1) != 1:
+            raise ValueError("rows must not overlap, and a row's elements must be adjacent")
+        s = _stream(stream)
+        ws = workspace or self.workspace(tokens, s or 0)
+        # the stride of a single row is whatever torch left there: one row has its own length
+        strides = [max(t.stride(0), t.shape[1]) if t is not None and tokens > 1 else n
+                   for t, n in ((x, self.cols), (base, self.rows), (out, self.rows))]
+        check(lib().hqb_lora(self._at, _ptr(x), strides[0], _ptr(ids), tokens, _ptr(base), strides[1], _ptr(out),
+                             _ROW_DTYPES[out.dtype], strides[2], ws.ptr(), ws.nbytes, s), "hqb_lora")
+        return out
 
 
 # ---- output-row sharding across ranks --------------------------------------------------

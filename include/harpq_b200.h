@@ -40,6 +40,7 @@ extern "C" {
 /* element types of activations, bias and outputs */
 #define HQB_F32 0
 #define HQB_F16 1
+#define HQB_BF16 2 /* serving operators only (paged cache, attention, adapters) */
 
 /* hqb_gemv_ex flags */
 #define HQB_FLAG_PDL 1u  /* launch with programmatic dependent launch (see hqb_gemv_ex) */
@@ -80,6 +81,8 @@ extern "C" {
 #define HQB_DEVERR_DEPTH 2        /* a depth-map entry outside [1, stage_count]          */
 #define HQB_DEVERR_TIMEOUT 4      /* a pipeline wait exceeded its bound (kernel returned) */
 #define HQB_DEVERR_LAUNCH 8       /* shared memory sized below a CTA's work (kernel returned) */
+#define HQB_DEVERR_PAGES 16       /* no free page, a table row too short, a page or slot out of range */
+#define HQB_DEVERR_INDEX 32       /* a length, start, parent, row or adapter id out of range */
 
 /* Matrix geometry, same fields and order as ProgressiveGemvGeometry
  * (reference native/include/harpq/progressive_gemv.hpp:15-23). */
@@ -407,6 +410,176 @@ HQB_API uint64_t hqb_prefill_workspace_bytes(const hqb_plane_matrix* m);
 HQB_API int hqb_prefill_gemm(const hqb_plane_matrix* m, uint32_t prefix, const void* x, int x_dtype,
                              uint32_t batch, const void* bias, int bias_dtype, void* y, int y_dtype,
                              void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---- serving operators: paged cache, drafted trees, adapters --------------------------- */
+
+/* What a decode step needs beside its quantized projections.  The reference has none of it
+ * (its runtime stops at the projection, native/include/harpq/progressive_gemv.hpp:49-62); a
+ * progressive matrix drafts for itself (prefix 1 drafts, prefix 2-4 verifies), and these
+ * operators are the step around it: hqb_page_plan once per step, then per layer the
+ * projections (hqb_lora beside them), hqb_tree_attention, and hqb_cache_append of the tokens
+ * that were kept.  Lengths, tables and ids live on the device; nothing is read back.  Index
+ * arrays are int32.  A bad device value never faults: it is clamped or skipped as each
+ * declaration says, and its HQB_DEVERR_* bit is OR-ed into the call's error word. */
+
+/* Largest number of drafted nodes of one request. */
+#define HQB_MAX_NODES 256
+/* Largest head dimension of the attention. */
+#define HQB_MAX_HEAD_DIM 256
+/* Largest rank of an adapter. */
+#define HQB_MAX_RANK 128
+
+/* A paged cache of keys and values: element (page, token in page, head, d) of k and of v lies
+ * at page*page_stride + token*token_stride + head*head_stride + d (strides in elements), so
+ * tokens may be stored before heads or heads before tokens.  Slot s is token s % page_size of
+ * page s / page_size.  dtype: HQB_F16 or HQB_BF16. */
+typedef struct hqb_paged_cache {
+  void* k;
+  void* v;
+  uint64_t page_stride;
+  uint64_t token_stride;
+  uint64_t head_stride;
+  int dtype;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t page_size;
+  uint32_t num_pages;
+  uint32_t reserved;
+} hqb_paged_cache;
+
+/* One step's lengths turned into addresses, in one launch.  Request r holds context_lens[r]
+ * cached tokens in held[r] pages (held NULL: ceil(context / page_size)) and brings
+ * new_lens[r] new ones.
+ *   starts[r]            first of the request's tokens in the step's packed token order
+ *                        (starts[requests]: all of them)
+ *   token_request[t]     request of token t          (each optional: NULL leaves it out)
+ *   positions[t]         context + index in the request; with parents, context + depth
+ *   mask[t][w]           with parents (an earlier node of the same request, or -1): bit j of
+ *                        word j/32 set for j = t's node and its ancestors
+ * With tables (not NULL), the pages that the new tokens need beyond the held ones are taken
+ * from free_pages[*free_head ..) in request order and written into the table rows:
+ *   tables[r][c]         page of column c (in place: only new columns are written)
+ *   slots[t]             cache slot of token t; -1 without a page
+ *   held_out, free_head_out  the counts after the step (not the buffers of held, free_head)
+ * Entries of tokens past the last one, up to token_capacity, are -1 (mask: 0).
+ * HQB_DEVERR_PAGES: the free pages or a table row ran out, or a held page is out of range;
+ * the tokens without a page get slot -1 and the counts stop there.  HQB_DEVERR_INDEX: a
+ * negative length or head (taken as 0), more pages held than a table row has (taken as the
+ * row), fewer held than the context fills (the missing ones are taken as new pages), more
+ * tokens than token_capacity (left out), a parent that is not earlier (taken as -1) or a node
+ * past the mask (its bit is left out). */
+typedef struct hqb_page_plan_args {
+  uint32_t requests;
+  uint32_t page_size;
+  uint32_t num_pages;
+  uint32_t table_stride; /* entries of a table row */
+  uint32_t token_capacity;
+  uint32_t free_count; /* entries of free_pages */
+  uint32_t mask_words; /* words of a mask row; 0 without a mask */
+  uint32_t reserved;
+  const int32_t* context_lens;
+  const int32_t* new_lens;
+  const int32_t* held;
+  const int32_t* free_pages;
+  const int32_t* free_head;
+  const int32_t* parents;
+  int32_t* tables;
+  int32_t* starts;
+  int32_t* token_request;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* held_out;
+  int32_t* free_head_out;
+  uint32_t* mask;
+  int* flags; /* device error word (OR-ed), or NULL */
+} hqb_page_plan_args;
+HQB_API int hqb_page_plan(const hqb_page_plan_args* args, void* stream);
+
+/* Writes rows of new keys and values into the cache: slot slots[i] gets row rows[i] (rows
+ * NULL: row i) of k and v, for i < count.  Row r, head h, element d of both lies at
+ * r*token_stride + h*head_stride + d.  dtype: the rows' type, HQB_F16, HQB_BF16 or HQB_F32,
+ * rounded once to the cache's type where it differs.  A negative slot or row skips the entry;
+ * a slot past the cache or a row >= source_rows is skipped too (HQB_DEVERR_PAGES /
+ * HQB_DEVERR_INDEX in *flags).  Of two entries with one slot,
+ * which one stays is not determined. */
+HQB_API int hqb_cache_append(const hqb_paged_cache* cache, const void* k, const void* v, int dtype,
+                             uint64_t token_stride, uint64_t head_stride, uint32_t source_rows, const int32_t* rows,
+                             const int32_t* slots, uint32_t count, int* flags, void* stream);
+
+/* Attention of each request's drafted nodes over its cached context and over those drafted
+ * nodes that its mask row shows.  Request r owns tokens starts[r] .. starts[r+1) of q, k, v
+ * and out; its context is the first context_lens[r] tokens of its table row.  Node i sees the
+ * whole context, and node j where bit j of its mask row is set (mask NULL: j <= i, so that one
+ * node is plain decoding).  q_heads is a multiple of the cache's kv_heads; query head h reads
+ * key head h / (q_heads / kv_heads).  For each (token, query head)
+ *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q.k_j),  lse = log(sum_j w_j)
+ * over the keys it sees; where that sum is zero (no key seen, or every score -inf) out is zeros
+ * and lse = -inf.  Keys and values that a
+ * node does not see change nothing for it, NaN and infinities among them.  q, k, v and out have
+ * the cache's type; products are summed in FP32, softmax statistics kept in FP32, and the
+ * weights w_j rounded to the cache's type for the product with v.
+ * max_new and max_context bound the requests' lengths on the host: they size the launch.  A
+ * longer context is still computed in full; nodes past max_new are left out
+ * (HQB_DEVERR_INDEX).  A context longer than its table row is cut (HQB_DEVERR_PAGES), and a
+ * page out of range reads page 0 (HQB_DEVERR_PAGES). */
+typedef struct hqb_attention_args {
+  uint32_t requests;
+  uint32_t tokens; /* rows of q, k, v and out */
+  uint32_t max_new; /* 1 .. HQB_MAX_NODES */
+  uint32_t max_context;
+  uint32_t q_heads;
+  uint32_t table_stride;
+  uint32_t mask_words; /* words of a mask row: at least ceil(max_new / 32) with a mask */
+  float scale;
+  const int32_t* starts;       /* [requests + 1] */
+  const int32_t* context_lens; /* [requests] */
+  const int32_t* tables;       /* [requests][table_stride] */
+  const uint32_t* mask;        /* [tokens][mask_words] or NULL */
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse; /* [tokens][q_heads] or NULL */
+  uint64_t q_token_stride, q_head_stride;     /* elements; heads' elements are adjacent */
+  uint64_t kv_token_stride, kv_head_stride;   /* of k and of v */
+  uint64_t out_token_stride, out_head_stride;
+} hqb_attention_args;
+/* Scratch bytes of a call (its pointers are not looked at); 0 for arguments that are refused.
+ * It starts with the error word (hqb_workspace_error); hqb_workspace_init clears it once. */
+HQB_API uint64_t hqb_tree_attention_workspace_bytes(const hqb_paged_cache* cache, const hqb_attention_args* args,
+                                                    int device);
+HQB_API int hqb_tree_attention(const hqb_paged_cache* cache, const hqb_attention_args* args, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
+
+/* Low-rank adapters stacked in one set: adapter i has a[i] = [max_rank][cols] and
+ * b[i] = [rows][max_rank] (row-major; rows / columns past its rank are never used, whatever
+ * they hold), rank ranks[i] (NULL: max_rank) and factor scales[i] (NULL: 1).  dtype: HQB_F16
+ * or HQB_BF16.  max_rank 1 .. HQB_MAX_RANK. */
+typedef struct hqb_lora_set {
+  const void* a;
+  const void* b;
+  const int32_t* ranks;
+  const float* scales;
+  uint64_t rows;
+  uint64_t cols;
+  uint32_t adapters;
+  uint32_t max_rank;
+  int dtype;
+  uint32_t reserved;
+} hqb_lora_set;
+
+/* y[t] = base[t] + scale_a * b_a (a_a x[t]) with a = ids[t], for t < tokens: the adapters of
+ * many requests beside a projection that they share.  ids[t] < 0: no adapter, y[t] = base[t];
+ * an id >= adapters counts as none (HQB_DEVERR_INDEX), and so does a rank of 0; a rank past
+ * max_rank is taken as max_rank (HQB_DEVERR_INDEX).  base NULL: zeros; base may be y (with the
+ * same stride), otherwise they must not overlap.  x has the set's type; y and base have y_dtype (the set's type or
+ * HQB_F32).  Strides are elements between tokens.  Both products are summed in FP32.  The
+ * inner vector a_a x[t] is kept in FP32 and enters the second product as terms of the set's
+ * type: one term (HQB_F16, HQB_BF16 y) or enough of them for 22 bits (HQB_F32 y). */
+HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* set, uint32_t tokens, int device);
+HQB_API int hqb_lora(const hqb_lora_set* set, const void* x, uint64_t x_stride, const int32_t* ids, uint32_t tokens,
+                     const void* base, uint64_t base_stride, void* y, int y_dtype, uint64_t y_stride, void* workspace,
+                     uint64_t workspace_bytes, void* stream);
 
 /* Dense FP32 weights [rows][cols] decoded from planes, Σ_{s<d} code·scale summed in
  * stage order from 0.0f — bit-identical to DequantizePrefix
