@@ -13,6 +13,7 @@ this module without the built library, or calling it without a CUDA device, rais
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 from typing import Sequence
 
@@ -583,13 +584,37 @@ class RawMatrix:
 
 _SERVING_DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
 _ROW_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+# A step's host time is mostly this module's own, so the calls below read each attribute once,
+# pack their argument structures in one go and ask for the raw stream.
+_PAGE_PLAN = struct.Struct("@8I15P")
+_ATTENTION = struct.Struct("@7If9P6Q")
+assert _PAGE_PLAN.size == ctypes.sizeof(PagePlanC) and _ATTENTION.size == ctypes.sizeof(AttentionC)
 
 
-def _ints(name: str, t: torch.Tensor | None, shape: tuple, device) -> None:
-    """Checks an int32 index tensor of a serving call."""
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()
-                          or t.device != device):
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on {device}")
+def _device_index(device: torch.device) -> int:
+    return torch.cuda.current_device() if device.index is None else device.index
+
+
+def _raw_stream(stream, index: int) -> int:
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(index)
+    return _stream(stream) or 0
+
+
+def _ints(name: str, t: torch.Tensor, n: int, device) -> int:
+    """Checks an int32 index tensor of n elements and gives its address."""
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on {device}, "
+                         f"got {list(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _table(name: str, t: torch.Tensor, rows: int, device) -> int:
+    """Checks an int32 matrix of `rows` rows and gives its columns."""
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows, got {list(t.shape)}")
+    _ints(name, t, t.numel(), device)
+    return t.shape[1]
 
 
 class PagePlan:
@@ -603,48 +628,53 @@ class PagePlan:
             raise ValueError("requests, tokens, page_size and num_pages must be positive")
         if not 0 <= max_new <= MAX_NODES:
             raise ValueError(f"max_new must be 0..{MAX_NODES}")
-        self.device = torch.empty(0, device=device or "cuda").device
         self.page_size, self.num_pages, self.words = page_size, num_pages, -(-max_new // 32)
-
-        def ints(n):
-            return torch.zeros(n, dtype=torch.int32, device=self.device)
-
-        self.starts, self.requests, self.positions, self.slots = ints(requests + 1), ints(tokens), ints(tokens), ints(tokens)
-        self.held, self.free_head, self.flags = ints(requests), ints(1), ints(1)
-        self.mask = torch.zeros(tokens, self.words, dtype=torch.int32, device=self.device) if self.words else None
+        self.batch, self.tokens = requests, tokens
+        # one buffer, so that a step's metadata is one copy where it is wanted on the host
+        sizes = [requests + 1, tokens, tokens, tokens, requests, 1, 1, tokens * self.words]
+        parts = torch.zeros(sum(sizes), dtype=torch.int32, device=device or "cuda").split(sizes)
+        self.starts, self.requests, self.positions, self.slots, self.held, self.free_head, self.flags, mask = parts
+        self.mask = mask.view(tokens, self.words) if self.words else None
+        self.device = self.starts.device
+        self._index = _device_index(self.device)
+        self._out = [t.data_ptr() for t in parts]
+        self._args = ctypes.create_string_buffer(_PAGE_PLAN.size)
+        self._at = ctypes.addressof(self._args)
+        self._call = lib().hqb_page_plan
 
     def build(self, context_lens: torch.Tensor, new_lens: torch.Tensor, held: torch.Tensor | None = None,
               tables: torch.Tensor | None = None, free_pages: torch.Tensor | None = None,
               free_head: torch.Tensor | None = None, parents: torch.Tensor | None = None, stream=None) -> "PagePlan":
         """Fills the buffers.  tables [requests, columns] (with free_pages and free_head) also gives the
-        new tokens pages and slots, writing new columns into it; parents [tokens or more] gives
-        tree positions and masks.  held and free_head are the counts before the step (pass the
-        previous plan's, not this one's)."""
-        n = self.held.numel()
-        _ints("context_lens", context_lens, (n,), self.device)
-        _ints("new_lens", new_lens, (n,), self.device)
-        _ints("held", held, (n,), self.device)
-        stride = free = 0
+        new tokens pages and slots, writing new columns into it; parents [at least the step's
+        tokens] gives tree positions and masks.  held and free_head are the counts before the
+        step (a previous plan's, not this one's buffers)."""
+        n, device = self.batch, self.device
+        starts, requests, positions, slots, held_out, head_out, flags, mask = self._out
+        ctx = _ints("context_lens", context_lens, n, device)
+        new = _ints("new_lens", new_lens, n, device)
+        have = 0 if held is None else _ints("held", held, n, device)
+        stride = free = rows = pool = head = tree = words = 0
         if tables is not None:
             if free_pages is None or free_head is None:
                 raise ValueError("tables need free_pages and free_head")
-            stride, free = tables.shape[-1], free_pages.numel()
-            _ints("tables", tables, (n, stride), self.device)
-            _ints("free_pages", free_pages, (free,), self.device)
-            _ints("free_head", free_head, (1,), self.device)
+            stride, rows, free = _table("tables", tables, n, device), tables.data_ptr(), free_pages.numel()
+            pool = _ints("free_pages", free_pages, free, device)
+            head = _ints("free_head", free_head, 1, device)
+        else:
+            slots = held_out = head_out = 0
         if parents is not None:
-            _ints("parents", parents, (parents.numel(),), self.device)
-            if self.mask is None:
+            if not self.words:
                 raise ValueError("parents need a plan with max_new > 0")
-        paged = tables is not None
-        args = PagePlanC(n, self.page_size, self.num_pages, stride, self.slots.numel(), free,
-                         self.words if parents is not None else 0, 0, _ptr(context_lens), _ptr(new_lens), _ptr(held),
-                         _ptr(free_pages) if paged else None, _ptr(free_head) if paged else None, _ptr(parents),
-                         _ptr(tables), _ptr(self.starts), _ptr(self.requests), _ptr(self.positions),
-                         _ptr(self.slots) if paged else None, _ptr(self.held) if paged else None,
-                         _ptr(self.free_head) if paged else None, _ptr(self.mask) if parents is not None else None,
-                         _ptr(self.flags))
-        check(lib().hqb_page_plan(ctypes.addressof(args), _stream(stream)), "hqb_page_plan")
+            tree, words = _ints("parents", parents, parents.numel(), device), self.words
+        else:
+            mask = 0
+        _PAGE_PLAN.pack_into(self._args, 0, n, self.page_size, self.num_pages, stride, self.tokens, free, words, 0, ctx,
+                             new, have, pool, head, tree, rows, starts, requests, positions, slots, held_out, head_out,
+                             mask, flags)
+        status = self._call(self._at, _raw_stream(stream, self._index))
+        if status:
+            check(status, "hqb_page_plan")
         return self
 
 
@@ -658,35 +688,43 @@ class PagedCache:
             raise ValueError("k and v must be [pages, page_size, heads, dim] tensors of one shape, layout, type and device")
         if k.dtype not in _SERVING_DTYPES:
             raise TypeError(f"unsupported dtype {k.dtype}; use float16 or bfloat16")
-        if k.stride(3) != 1:
+        if k.stride(3) != 1 and k.shape[3] > 1:
             raise ValueError("a head's elements must be adjacent")
         self.k, self.v = k, v
         self.num_pages, self.page_size, self.heads, self.dim = k.shape
-        self.device = k.device
+        self.dtype, self.device = k.dtype, k.device
         self.flags = torch.zeros(1, dtype=torch.int32, device=k.device)
         self.c = PagedCacheC(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), _SERVING_DTYPES[k.dtype],
                              self.heads, self.dim, self.page_size, self.num_pages, 0)
-        self._at = ctypes.addressof(self.c)
+        self._at, self._flags = ctypes.addressof(self.c), self.flags.data_ptr()
+        self._index = _device_index(self.device)
+        self._call = lib().hqb_cache_append
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor | None = None,
                stream=None) -> None:
         """Writes rows of k and v [tokens, heads, dim] (FP16, BF16 or FP32) into the cache's slots
         [count]: row rows[i], or i, goes to slots[i]; negative ones are skipped.  flags collects
         HQB_DEVERR_* bits."""
-        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != self.heads or k.shape[2] != self.dim:
+        shape, strides, device = k.shape, k.stride(), self.device
+        if len(shape) != 3 or shape[1] != self.heads or shape[2] != self.dim or v.shape != shape:
             raise ValueError(f"k and v must be [tokens, {self.heads}, {self.dim}]")
-        if k.dtype != v.dtype or k.dtype not in _ROW_DTYPES:
+        kind = _ROW_DTYPES.get(k.dtype)
+        if kind is None or v.dtype is not k.dtype:
             raise TypeError("k and v must share a type: float16, bfloat16 or float32")
-        if k.stride() != v.stride() or (self.dim > 1 and k.stride(2) != 1) or k.device != self.device or v.device != self.device:
+        if v.stride() != strides or (strides[2] != 1 and self.dim > 1) or k.device != device or v.device != device:
             raise ValueError("k and v must share strides (adjacent elements within a head) and the cache's device")
         n = slots.numel()
-        _ints("slots", slots, (n,), self.device)
-        _ints("rows", rows, (n,), self.device)
-        if rows is None and n > k.shape[0]:
-            raise ValueError("more slots than rows")
-        check(lib().hqb_cache_append(self._at, _ptr(k), _ptr(v), _ROW_DTYPES[k.dtype], k.stride(0), k.stride(1),
-                                     k.shape[0], _ptr(rows), _ptr(slots), n, _ptr(self.flags), _stream(stream)),
-              "hqb_cache_append")
+        to = _ints("slots", slots, n, device)
+        if rows is not None:
+            pick = _ints("rows", rows, n, device)
+        else:
+            pick = 0
+            if n > shape[0]:
+                raise ValueError("more slots than rows")
+        status = self._call(self._at, k.data_ptr(), v.data_ptr(), kind, strides[0], strides[1], shape[0], pick, to, n,
+                            self._flags, _raw_stream(stream, self._index))
+        if status:
+            check(status, "hqb_cache_append")
 
 
 class TreeAttention:
@@ -706,12 +744,24 @@ class TreeAttention:
         self.cache, self.q_heads, self.requests, self.tokens = cache, q_heads, requests, tokens
         self.max_new, self.max_context = max_new, max_context
         args = AttentionC(requests=requests, tokens=tokens, max_new=max_new, max_context=max_context, q_heads=q_heads)
-        index = cache.device.index
-        need = lib().hqb_tree_attention_workspace_bytes(cache._at, ctypes.addressof(args),
-                                                        torch.cuda.current_device() if index is None else index)
+        need = lib().hqb_tree_attention_workspace_bytes(cache._at, ctypes.addressof(args), cache._index)
         if need == 0:
             raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
         self.ws = Workspace(need, cache.device)
+        self._ws = self.ws.ptr()
+        self._args = ctypes.create_string_buffer(_ATTENTION.size)
+        self._at = ctypes.addressof(self._args)
+        self._call = lib().hqb_tree_attention
+
+    def _rows(self, name: str, t: torch.Tensor, tokens: int, heads: int) -> tuple:
+        c, shape, strides = self.cache, t.shape, t.stride()
+        if len(shape) != 3 or shape[0] != tokens or shape[1] != heads or shape[2] != c.dim:
+            raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}], got {list(shape)}")
+        if t.dtype is not c.dtype or t.device != c.device:
+            raise TypeError(f"{name} must have the cache's type and device")
+        if strides[2] != 1 and c.dim > 1:
+            raise ValueError(f"{name}: a head's elements must be adjacent")
+        return strides
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tables: torch.Tensor,
                  context_lens: torch.Tensor, starts: torch.Tensor, mask: torch.Tensor | None = None,
@@ -723,50 +773,49 @@ class TreeAttention:
         [tokens, words]: bit j of a node's row shows it node j of its request (None: the nodes
         up to itself).  scale None: dim ** -0.5.  lse [tokens, q_heads] FP32 gets the logarithm of
         the sum of weights."""
-        c = self.cache
+        c, device = self.cache, self.cache.device
         tokens, requests = q.shape[0], context_lens.numel()
         if out is None:
-            out = torch.empty(tokens, self.q_heads, c.dim, dtype=q.dtype, device=q.device)
-        for name, t, heads in (("q", q, self.q_heads), ("k", k, c.heads), ("v", v, c.heads), ("out", out, self.q_heads)):
-            if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != heads or t.shape[2] != c.dim:
-                raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}]")
-            if t.dtype != c.k.dtype or t.device != c.device:
-                raise TypeError(f"{name} must have the cache's type and device")
-            if c.dim > 1 and t.stride(2) != 1:
-                raise ValueError(f"{name}: a head's elements must be adjacent")
-        if k.stride() != v.stride():
+            out = torch.empty(tokens, self.q_heads, c.dim, dtype=c.dtype, device=device)
+        qs = self._rows("q", q, tokens, self.q_heads)
+        ks = self._rows("k", k, tokens, c.heads)
+        if self._rows("v", v, tokens, c.heads) != ks:
             raise ValueError("k and v must share strides")
+        os = self._rows("out", out, tokens, self.q_heads)
         if requests > self.requests or tokens > self.tokens:
             raise ValueError(f"built for {self.requests} requests and {self.tokens} tokens, got {requests} and {tokens}")
-        columns = tables.shape[-1]
-        _ints("tables", tables, (requests, columns), c.device)
-        _ints("context_lens", context_lens, (requests,), c.device)
-        _ints("starts", starts, (requests + 1,), c.device)
-        words = 0
+        columns = _table("tables", tables, requests, device)
+        ctx = _ints("context_lens", context_lens, requests, device)
+        first = _ints("starts", starts, requests + 1, device)
+        bits = words = 0
         if mask is not None:
-            words = mask.shape[-1]
-            _ints("mask", mask, (mask.shape[0], words), c.device)
+            words = _table("mask", mask, mask.shape[0], device)
             if mask.shape[0] < tokens or words * 32 < self.max_new:
                 raise ValueError(f"mask must be [{tokens}, {-(-self.max_new // 32)}] or larger")
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, self.q_heads)
-                                or not lse.is_contiguous() or lse.device != c.device):
-            raise ValueError(f"lse must be a contiguous float32 [{tokens}, {self.q_heads}] tensor")
-        args = AttentionC(requests, tokens, self.max_new, self.max_context, self.q_heads, columns, words,
-                          c.dim ** -0.5 if scale is None else scale, _ptr(starts), _ptr(context_lens), _ptr(tables),
-                          _ptr(mask), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), q.stride(0), q.stride(1),
-                          k.stride(0), k.stride(1), out.stride(0), out.stride(1))
-        check(lib().hqb_tree_attention(c._at, ctypes.addressof(args), self.ws.ptr(), self.ws.nbytes, _stream(stream)),
-              "hqb_tree_attention")
+            bits = mask.data_ptr()
+        sums = 0
+        if lse is not None:
+            if (lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape[0] != tokens or lse.shape[1] != self.q_heads
+                    or not lse.is_contiguous() or lse.device != device):
+                raise ValueError(f"lse must be a contiguous float32 [{tokens}, {self.q_heads}] tensor")
+            sums = lse.data_ptr()
+        _ATTENTION.pack_into(self._args, 0, requests, tokens, self.max_new, self.max_context, self.q_heads, columns, words,
+                             c.dim ** -0.5 if scale is None else scale, first, ctx, tables.data_ptr(), bits, q.data_ptr(),
+                             k.data_ptr(), v.data_ptr(), out.data_ptr(), sums, qs[0], qs[1], ks[0], ks[1], os[0], os[1])
+        status = self._call(c._at, self._at, self._ws, self.ws.nbytes, _raw_stream(stream, c._index))
+        if status:
+            check(status, "hqb_tree_attention")
         return out
 
 
 class LoraSet:
     """Low-rank adapters stacked in two device tensors: a [adapters, max_rank, cols] and b
     [adapters, rows, max_rank] (FP16 or BF16), with ranks [adapters] int32 (None: max_rank each)
-    and scales [adapters] FP32 (None: 1).  Workspaces are kept per stream."""
+    and scales [adapters] FP32 (None: 1).  Workspaces are kept per stream; the constructing
+    stream's is made at once, for up to max_tokens tokens."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, ranks: torch.Tensor | None = None,
-                 scales: torch.Tensor | None = None):
+                 scales: torch.Tensor | None = None, max_tokens: int = 8192):
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
             raise ValueError("a must be [adapters, max_rank, cols] and b [adapters, rows, max_rank]")
         if a.dtype != b.dtype or a.dtype not in _SERVING_DTYPES:
@@ -775,28 +824,45 @@ class LoraSet:
             raise ValueError("a and b must be contiguous and on one device")
         self.adapters, self.max_rank, self.cols = a.shape
         self.rows = b.shape[1]
+        if self.adapters < 1 or self.rows < 1 or self.cols < 1:
+            raise ValueError("a set has at least one adapter, row and column")
         if not 1 <= self.max_rank <= MAX_RANK:
             raise ValueError(f"max_rank must be 1..{MAX_RANK}")
-        _ints("ranks", ranks, (self.adapters,), a.device)
+        if ranks is not None:
+            _ints("ranks", ranks, self.adapters, a.device)
         if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (self.adapters,)
                                    or not scales.is_contiguous() or scales.device != a.device):
             raise ValueError(f"scales must be a contiguous float32 [{self.adapters}] tensor")
-        self.a, self.b, self.ranks, self.scales, self.device = a, b, ranks, scales, a.device
+        self.a, self.b, self.ranks, self.scales = a, b, ranks, scales
+        self.dtype, self.device = a.dtype, a.device
         self.c = LoraSetC(a.data_ptr(), b.data_ptr(), _ptr(ranks), _ptr(scales), self.rows, self.cols, self.adapters,
                           self.max_rank, _SERVING_DTYPES[a.dtype], 0)
-        self._at = ctypes.addressof(self.c)
+        self._at, self._index = ctypes.addressof(self.c), _device_index(a.device)
+        self._call = lib().hqb_lora
         self._ws: dict = {}
+        self.workspace(max_tokens, _raw_stream(None, self._index))
 
     def workspace(self, tokens: int, stream: int) -> Workspace:
         """The stream's workspace, grown to what `tokens` tokens need."""
         ws = self._ws.get(stream)
         if ws is None or tokens > ws.tokens:
-            # allocated on the stream that uses it: the allocator then reuses it in that order
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
-                ws = Workspace(lib().hqb_lora_workspace_bytes(self._at, tokens, 0), self.device)
+            need = lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
+            if stream == _raw_stream(None, self._index):
+                ws = Workspace(need, self.device)
+            else:  # allocated on the stream that uses it: the allocator then reuses it in that order
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
+                    ws = Workspace(need, self.device)
             ws.tokens = tokens
             self._ws[stream] = ws
         return ws
+
+    def _out(self, name: str, t: torch.Tensor, tokens: int, kind) -> int:
+        shape, strides = t.shape, t.stride()
+        if len(shape) != 2 or shape[0] != tokens or shape[1] != self.rows or t.dtype is not kind or t.device != self.device:
+            raise ValueError(f"{name} must be [{tokens}, {self.rows}] {kind} on {self.device}")
+        if (strides[1] != 1 and self.rows > 1) or (strides[0] < self.rows and tokens > 1):
+            raise ValueError(f"{name}: a row's elements must be adjacent, and rows must not overlap")
+        return strides[0] if tokens > 1 else self.rows  # torch leaves any stride on a single row
 
     def apply(self, x: torch.Tensor, ids: torch.Tensor, base: torch.Tensor | None = None,
               out: torch.Tensor | None = None, y_dtype: torch.dtype | None = None, workspace: Workspace | None = None,
@@ -804,28 +870,28 @@ class LoraSet:
         """base + scale_i * b_i (a_i x) per token, i = ids[token] (negative: base alone) (hqb_lora).
         x [tokens, cols]; base [tokens, rows] (None: zeros) and the result share a type, the
         set's or FP32.  out=base adds in place, e.g. to the output of a projection's gemv()."""
-        if x.dim() != 2 or x.shape[1] != self.cols or x.dtype != self.a.dtype or x.device != self.device:
-            raise ValueError(f"x must be [tokens, {self.cols}] of the set's type, on its device")
-        tokens = x.shape[0]
-        _ints("ids", ids, (tokens,), self.device)
+        shape, strides = x.shape, x.stride()
+        if len(shape) != 2 or shape[1] != self.cols or x.dtype is not self.dtype or x.device != self.device:
+            raise ValueError(f"x must be [tokens, {self.cols}] {self.dtype} on {self.device}")
+        tokens = shape[0]
+        if (strides[1] != 1 and self.cols > 1) or (strides[0] < self.cols and tokens > 1):
+            raise ValueError("x: a row's elements must be adjacent, and rows must not overlap")
         if out is None:
             kind = y_dtype or (base.dtype if base is not None else x.dtype)
             out = torch.empty(tokens, self.rows, dtype=kind, device=self.device)
-        for name, t in (("out", out), ("base", base)):
-            if t is not None and (tuple(t.shape) != (tokens, self.rows) or t.dtype != out.dtype or t.device != self.device
-                                  or (self.rows > 1 and t.stride(1) != 1)):
-                raise ValueError(f"{name} must be [tokens, {self.rows}] with adjacent elements, of one type with the result")
-        if out.dtype != torch.float32 and out.dtype != self.a.dtype:
+        kind = out.dtype
+        if kind is not self.dtype and kind is not torch.float32:
             raise TypeError("the result must have the set's type or float32")
-        if tokens > 1 and min(x.stride(0) - self.cols, out.stride(0) - self.rows) < 0 or self.cols > 1 and x.stride(1) != 1:
-            raise ValueError("rows must not overlap, and a row's elements must be adjacent")
-        s = _stream(stream)
-        ws = workspace or self.workspace(tokens, s or 0)
-        # the stride of a single row is whatever torch left there: one row has its own length
-        strides = [max(t.stride(0), t.shape[1]) if t is not None and tokens > 1 else n
-                   for t, n in ((x, self.cols), (base, self.rows), (out, self.rows))]
-        check(lib().hqb_lora(self._at, _ptr(x), strides[0], _ptr(ids), tokens, _ptr(base), strides[1], _ptr(out),
-                             _ROW_DTYPES[out.dtype], strides[2], ws.ptr(), ws.nbytes, s), "hqb_lora")
+        which = _ints("ids", ids, tokens, self.device)
+        y_stride, base_stride, base_at = self._out("out", out, tokens, kind), 0, 0
+        if base is not None:
+            base_stride, base_at = self._out("base", base, tokens, kind), base.data_ptr()
+        s = _raw_stream(stream, self._index)
+        ws = workspace or self.workspace(tokens, s)
+        status = self._call(self._at, x.data_ptr(), strides[0] if tokens > 1 else self.cols, which, tokens, base_at,
+                            base_stride, out.data_ptr(), _ROW_DTYPES[kind], y_stride, ws.ptr(), ws.nbytes, s)
+        if status:
+            check(status, "hqb_lora")
         return out
 
 
