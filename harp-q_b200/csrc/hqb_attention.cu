@@ -1,6 +1,7 @@
 // Attention of drafted trees over a paged cache (hqb_tree_attention).
 //   attention_rows_kernel  16 query rows a tile on mma.sync: single tokens, small trees, and every
 //                          shape that the tensor-memory kernel does not take
+//   attention_tmem_kernel  256 query rows a tile on tcgen05 (hqb_attention_tmem.cu)
 //   attention_join_kernel  joins the partial results of items that span CTAs
 #include <cuda_runtime.h>
 
@@ -12,6 +13,7 @@ namespace {
 
 constexpr uint32_t kRowsThreads = 128;
 constexpr uint32_t kRowsWarps = kRowsThreads / 32;
+constexpr uint32_t kKeyBlock = 64;
 constexpr uint32_t kChunk = 16;  // keys a warp takes at once
 constexpr uint32_t kStages = 3;  // chunks of a warp's ring
 
@@ -274,7 +276,10 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t d = n * 8 + qd * 2 + (e & 1);
-            if (d < dim && (sees[e >> 1] >> j & 1u)) acc[n][e] += weight[e >> 1] * Elem<T>::to_float(row[d]);
+            if (d < dim && (sees[e >> 1] >> j & 1u)) {
+              const float v = Elem<T>::to_float(row[d]);
+              acc[n][e] += fabsf(v) < INFINITY ? weight[e >> 1] * v : v;  // weights are positive
+            }
           }
       }
     }
@@ -401,7 +406,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
 }
 
 struct Shape {
-  uint32_t rows, max_tiles, dim_pad, grid, whole;
+  uint32_t rows, block, max_tiles, dim_pad, grid, whole, tmem;
   uint64_t parts_bytes;
 };
 
@@ -414,13 +419,32 @@ bool shape_ok(const hqb_paged_cache* c, const hqb_attention_args* a) {
   return true;
 }
 
-Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, int sms) {
+// 16-byte copies need 16-byte rows everywhere; anything else goes element by element.
+bool aligned_rows(const hqb_paged_cache* c, const hqb_attention_args* a) {
+  const uintptr_t addresses = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) |
+                              reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
+                              reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->out);
+  const uint64_t strides = c->page_stride | c->token_stride | c->head_stride | a->q_token_stride | a->q_head_stride |
+                           a->kv_token_stride | a->kv_head_stride | a->out_token_stride | a->out_head_stride |
+                           c->head_dim;
+  return (addresses & 15u) == 0 && (strides & 7u) == 0;
+}
+
+// Whether the tensor-memory kernel takes the call: heads of up to 128, aligned rows, more rows
+// than one tile of the rows kernel, a positive scale (its masked scores are -inf * scale).
+bool takes_tmem(const hqb_paged_cache* c, const hqb_attention_args* a, bool aligned) {
+  return aligned && c->head_dim <= 128 && a->scale > 0.0f && a->max_new * (a->q_heads / c->kv_heads) > 16;
+}
+
+Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem, int sms) {
   Shape s{};
   const uint32_t group = a->q_heads / c->kv_heads;
   s.dim_pad = c->head_dim <= 64 ? 64u : c->head_dim <= 128 ? 128u : 256u;
-  s.rows = 16;
+  s.tmem = tmem ? 1u : 0u;
+  s.rows = tmem ? 256u : 16u;
+  s.block = tmem ? 128u : kKeyBlock;
   s.max_tiles = (a->max_new * group + s.rows - 1) / s.rows;
-  s.grid = static_cast<uint32_t>(sms) * (s.dim_pad == 256 ? 1u : 2u);
+  s.grid = static_cast<uint32_t>(sms) * (tmem || s.dim_pad == 256 ? 1u : 2u);
   const uint64_t items = static_cast<uint64_t>(a->requests) * c->kv_heads * s.max_tiles;
   // up to 8 blocks a request: an item is one CTA's work of a few microseconds, and cutting it
   // would add a second launch
@@ -448,8 +472,8 @@ cudaError_t launch_dim(const AttnParams& p, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t launch_attention(const AttnParams& p, bool vec, cudaStream_t st) {
-  cudaError_t e = vec ? launch_dim<T, true>(p, st) : launch_dim<T, false>(p, st);
+cudaError_t launch_attention(const AttnParams& p, bool vec, bool tmem, cudaStream_t st) {
+  cudaError_t e = tmem ? launch_attention_tmem<T>(p, st) : vec ? launch_dim<T, true>(p, st) : launch_dim<T, false>(p, st);
   if (e != cudaSuccess || p.whole) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.a.requests * p.c.kv_heads * p.max_tiles, (p.rows + 15) / 16);
@@ -474,7 +498,10 @@ HQB_API uint64_t hqb_tree_attention_workspace_bytes(const hqb_paged_cache* c, co
   if (!shape_ok(c, a)) return 0;
   const int sms = device_sm_count(device);
   if (sms <= 0) return 0;
-  return 256 + round_up(shape_of(c, a, sms).parts_bytes, 256);
+  // the call chooses its kernel by alignment and scale too: room for either
+  const uint64_t rows = shape_of(c, a, false, sms).parts_bytes, tmem = shape_of(c, a, true, sms).parts_bytes;
+  const bool may = c->head_dim <= 128 && a->max_new * (a->q_heads / c->kv_heads) > 16;
+  return 256 + round_up(may && tmem > rows ? tmem : rows, 256);
 }
 
 HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_args* a, void* workspace,
@@ -495,7 +522,8 @@ HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_arg
   if (e != cudaSuccess) return e;
   const int sms = device_sm_count(device);
   if (sms <= 0) return HQB_ERR_INVALID;
-  const Shape s = shape_of(c, a, sms);
+  const bool vec = aligned_rows(c, a), tmem = takes_tmem(c, a, vec);
+  const Shape s = shape_of(c, a, tmem, sms);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 ||
       workspace_bytes < 256 + s.parts_bytes)
     return HQB_ERR_INVALID;
@@ -507,22 +535,16 @@ HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_arg
   p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
   p.group = a->q_heads / c->kv_heads;
   p.rows = s.rows;
+  p.block = s.block;
   p.max_tiles = s.max_tiles;
   p.dim_pad = s.dim_pad;
   p.min_blocks = 4;
   p.whole = s.whole;
   p.grid = s.grid;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  // 16-byte copies need 16-byte rows everywhere; anything else goes element by element
-  const uintptr_t addresses = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) |
-                              reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
-                              reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->out);
-  const uint64_t strides = c->page_stride | c->token_stride | c->head_stride | a->q_token_stride | a->q_head_stride |
-                           a->kv_token_stride | a->kv_head_stride | a->out_token_stride | a->out_head_stride |
-                           c->head_dim;
-  const bool vec = (addresses & 15u) == 0 && (strides & 7u) == 0;
   cudaStream_t st = as_stream(stream);
-  return c->dtype == HQB_F16 ? launch_attention<__half>(p, vec, st) : launch_attention<__nv_bfloat16>(p, vec, st);
+  return c->dtype == HQB_F16 ? launch_attention<__half>(p, vec, tmem, st)
+                             : launch_attention<__nv_bfloat16>(p, vec, tmem, st);
 }
 
 }  // extern "C"

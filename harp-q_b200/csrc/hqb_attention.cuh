@@ -2,7 +2,7 @@
 //
 // An item is (request, key head, row tile): the row tile's query rows (row = node * group + head
 // in group, so every row of the tile reads the same keys) against the request's keys, which are
-// cut into blocks of 64: first the cached context, then the drafted nodes (the last block of
+// cut into blocks (64 or 128 keys): first the cached context, then the drafted nodes (the last block of
 // either may be partly filled).  Items lie in order request, key head, row tile; the blocks of
 // all items in that order are dealt to the CTAs in equal contiguous ranges, so ragged lengths
 // balance whatever their order.  An item that spans CTAs leaves one partial result per CTA
@@ -14,8 +14,6 @@
 
 namespace hqb {
 
-constexpr uint32_t kKeyBlock = 64;
-
 struct AttnParams {
   hqb_attention_args a;
   hqb_paged_cache c;
@@ -23,6 +21,7 @@ struct AttnParams {
   float* parts;         // [cta][2][row tile][dim_pad + 2]
   uint32_t group;       // query heads per key head
   uint32_t rows;        // rows of a row tile
+  uint32_t block;       // keys of a block
   uint32_t max_tiles;   // row tiles of max_new nodes
   uint32_t dim_pad;     // padded head dimension (columns of a partial row)
   uint32_t min_blocks;  // fewest blocks worth a CTA of its own
@@ -53,8 +52,8 @@ __device__ __forceinline__ Request load_request(const AttnParams& p, uint32_t r,
     bad |= HQB_DEVERR_PAGES;
     q.ctx = static_cast<uint32_t>(room);
   }
-  q.cached_blocks = (q.ctx + kKeyBlock - 1) / kKeyBlock;
-  q.blocks = q.nodes == 0 ? 0u : q.cached_blocks + (q.nodes + kKeyBlock - 1) / kKeyBlock;
+  q.cached_blocks = (q.ctx + p.block - 1) / p.block;
+  q.blocks = q.nodes == 0 ? 0u : q.cached_blocks + (q.nodes + p.block - 1) / p.block;
   q.tiles = (q.nodes * p.group + p.rows - 1) / p.rows;
   return q;
 }
@@ -200,5 +199,9 @@ __device__ __forceinline__ uint32_t node_mask(const AttnParams& p, const Request
   const int32_t live = static_cast<int32_t>(q.nodes) - static_cast<int32_t>(word * 32);
   return live >= 32 ? bits : live <= 0 ? 0u : bits & ((1u << live) - 1u);
 }
+
+// Launches attention_tmem_kernel (hqb_attention_tmem.cu): p.rows 256, p.block 128, p.dim_pad 64 or 128.
+template <typename T>
+cudaError_t launch_attention_tmem(const AttnParams& p, cudaStream_t st);
 
 }  // namespace hqb
