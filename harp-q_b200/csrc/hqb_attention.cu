@@ -430,10 +430,20 @@ bool aligned_rows(const hqb_paged_cache* c, const hqb_attention_args* a) {
   return (addresses & 15u) == 0 && (strides & 7u) == 0;
 }
 
-// Whether the tensor-memory kernel takes the call: heads of up to 128, aligned rows, more rows
-// than one tile of the rows kernel, a positive scale (its masked scores are -inf * scale).
+// Whether the tensor-memory kernel can take a shape: heads of up to 128, groups that fit a score
+// tile, more rows than one tile of the rows kernel.
+bool tmem_shape(const hqb_paged_cache* c, const hqb_attention_args* a) {
+  const uint32_t group = a->q_heads / c->kv_heads;
+  return c->head_dim <= 128 && group <= 128 && a->max_new * group > 16;
+}
+
+// ... and the call: its masked scores are -inf * scale; a stride of zero (a broadcast input) or
+// one past 2^39 elements has no tensor map.
 bool takes_tmem(const hqb_paged_cache* c, const hqb_attention_args* a, bool aligned) {
-  return aligned && c->head_dim <= 128 && a->scale > 0.0f && a->max_new * (a->q_heads / c->kv_heads) > 16;
+  auto mapped = [](uint64_t n, uint64_t stride) { return n <= 1 || (stride > 0 && stride < (1ull << 39)); };
+  return aligned && a->scale > 0.0f && tmem_shape(c, a) && mapped(a->q_heads, a->q_head_stride) &&
+         mapped(a->tokens, a->q_token_stride) && mapped(c->kv_heads, a->kv_head_stride) &&
+         mapped(a->tokens, a->kv_token_stride);
 }
 
 Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem, int sms) {
@@ -441,7 +451,7 @@ Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem,
   const uint32_t group = a->q_heads / c->kv_heads;
   s.dim_pad = c->head_dim <= 64 ? 64u : c->head_dim <= 128 ? 128u : 256u;
   s.tmem = tmem ? 1u : 0u;
-  s.rows = tmem ? 256u : 16u;
+  s.rows = tmem ? 2 * (128 / group * group) : 16u;  // a score tile holds whole nodes
   s.block = tmem ? 128u : kKeyBlock;
   s.max_tiles = (a->max_new * group + s.rows - 1) / s.rows;
   s.grid = static_cast<uint32_t>(sms) * (tmem || s.dim_pad == 256 ? 1u : 2u);
@@ -499,9 +509,9 @@ HQB_API uint64_t hqb_tree_attention_workspace_bytes(const hqb_paged_cache* c, co
   const int sms = device_sm_count(device);
   if (sms <= 0) return 0;
   // the call chooses its kernel by alignment and scale too: room for either
-  const uint64_t rows = shape_of(c, a, false, sms).parts_bytes, tmem = shape_of(c, a, true, sms).parts_bytes;
-  const bool may = c->head_dim <= 128 && a->max_new * (a->q_heads / c->kv_heads) > 16;
-  return 256 + round_up(may && tmem > rows ? tmem : rows, 256);
+  const uint64_t rows = shape_of(c, a, false, sms).parts_bytes;
+  const uint64_t tmem = tmem_shape(c, a) ? shape_of(c, a, true, sms).parts_bytes : 0;
+  return 256 + round_up(tmem > rows ? tmem : rows, 256);
 }
 
 HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_args* a, void* workspace,

@@ -200,7 +200,7 @@ __device__ __forceinline__ uint32_t node_mask(const AttnParams& p, const Request
   return live >= 32 ? bits : live <= 0 ? 0u : bits & ((1u << live) - 1u);
 }
 
-// Launches attention_tmem_kernel (hqb_attention_tmem.cu): p.rows 256, p.block 128, p.dim_pad 64 or 128.
+// Launches attention_tmem_kernel (hqb_attention_tmem.cu): p.rows 2 * (128 / group * group), p.block 128, p.dim_pad 64 or 128.
 template <typename T>
 cudaError_t launch_attention_tmem(const AttnParams& p, cudaStream_t st);
 

@@ -1,6 +1,7 @@
 // Attention of drafted trees over a paged cache on the tcgen05 tensor cores: tiles of up to 256
 // query rows of one (request, key head) against blocks of 128 keys (see hqb_attention.cuh for the
 // division of the work).
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "hqb_attention.cuh"
@@ -10,32 +11,42 @@ namespace hqb {
 namespace {
 
 constexpr uint32_t kKeys = 128;      // keys of a block
-constexpr uint32_t kRows = 128;      // rows of one score tile (tensor-memory lanes)
-constexpr uint32_t kStreams = 2;     // score tiles in flight, one per softmax warpgroup
-constexpr uint32_t kLoaders = 64;
+constexpr uint32_t kRows = 128;      // tensor-memory lanes: rows of one score tile
+constexpr uint32_t kCopyWarp = 9;  // plain copies and the values' last rows; warp 8: tensor-map copies
 constexpr uint32_t kMmaWarp = 10;
-constexpr uint32_t kTmemThreads = 384;  // 8 softmax warps, 2 loaders, the MMA issuer, one idle: 168 registers a thread
+constexpr uint32_t kTmemThreads = 384;  // warps 0-7 softmax, 8-10 as above, 11 idle
+// Registers: 384 threads start with 168 each; the softmax warpgroups take 208, the rest keep 80
+// (2 * 128 * 208 + 128 * 80 = 63488 of the launch's 64512).
+constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80;
 constexpr float kSlack = 8.0f;       // log2 of how far the maximum may grow before sums are rescaled
 
-template <int DP>
-struct TmemShape {
-  static constexpr uint32_t kQTile = kRows * DP * 2;            // one score tile's queries
-  static constexpr uint32_t kSlot = kKeys * DP * 2;             // one block of keys or of values
-  static constexpr uint32_t kSlots = DP == 128 ? 5 : 8;
-  static constexpr uint32_t kRing = kStreams * kQTile;
-  static constexpr uint32_t kBars = kRing + kSlots * kSlot;
-  static constexpr uint32_t kStats = kBars + 256;
-  static constexpr uint32_t kBytes = kStats + 256 * 8;
-  static constexpr uint32_t kLag = kSlots - 2;                  // slots a loader thread has in flight
-};
-
 struct Bars {
-  uint64_t kv_full[8], kv_empty[8];
+  uint64_t kv_full[8], kv_empty[8], fix_full[8];
   uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], o_free, joint, drain;
   uint32_t tmem, abort;
   uint32_t broken[8][8];  // by segment: drafted nodes with an infinity or NaN among their values
 };
-static_assert(sizeof(Bars) <= 512, "");
+
+template <int DP>
+struct TmemShape {
+  static constexpr uint32_t kHalf = kRows * 128;  // 128 rows of 64 columns
+  static constexpr uint32_t kTile = kRows * DP * 2;  // a score tile's queries; a block of keys or of values
+  static constexpr uint32_t kSlots = DP == 128 ? 5 : 8;
+  static constexpr uint32_t kRing = 2 * kTile;
+  static constexpr uint32_t kBars = kRing + kSlots * kTile;
+  static constexpr uint32_t kStats = kBars + (sizeof(Bars) + 15) / 16 * 16;
+  static constexpr uint32_t kBytes = kStats + 256 * 8;
+};
+
+// Tensor maps, all in boxes of 64 columns in 128-byte-swizzled rows: the cache's k and v as
+// (column, head, token, page) with boxes of box_rows tokens, a power of two from 8 to 128 that
+// divides the page size (0: the cache has no maps and comes by plain copies); the step's own q
+// (boxes of half a tile: the group's heads of kRows / group nodes), k and v (boxes of a block)
+// as (column, head, token).
+struct Maps {
+  CUtensorMap ck, cv, q, k, v;
+  uint32_t box_rows;
+};
 
 // Mathematics: the one-pass softmax of attention_rows_kernel.  A running reference m stands in
 // for the maximum: it follows the maximum only when that has grown by more than 8 in the
@@ -43,19 +54,22 @@ static_assert(sizeof(Bars) <= 512, "");
 // result is the same sum up to rounding.
 // Roles: 4 + 4 warps take the scores of two streams out of tensor memory (a thread a row: no
 // shuffles), turn them into weights and put those back, packed in 16 bits over the scores, as
-// the A operand of weights x values; 4 warps copy keys, values and queries into 128-byte-swizzled
-// shared memory through the page table; one thread issues the MMAs.  A tile of more than 128 rows
-// has its two halves as streams, over the same keys (each block is loaded once for 256 rows); a
-// smaller tile has the even and the odd blocks as streams, joined at the end, so that the scores of
-// one stream are computed while the other's weights are.
+// the A operand of weights x values; one warp brings keys, values and queries into
+// 128-byte-swizzled shared memory by tensor-map copies through the page table; one thread issues
+// the MMAs.  The last rows of values (past the context's end, drafted nodes) pass a warp that
+// zeroes what must not reach a sum.  A tile of more rows than one score tile has its two halves as
+// streams, over the same keys (each block is loaded once for both); a smaller tile has the even
+// and the odd blocks as streams, joined at the end, so that the scores of one stream are computed
+// while the other's weights are.
 // Tensor memory: scores 2 x 128 columns, sums 2 x DP columns.  Shared memory at DP 128: queries
 // 64 KB, a ring of five 32 KB blocks.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const __grid_constant__ AttnParams p,
+                                                                          const __grid_constant__ Maps maps) {
   using S = TmemShape<DP>;
   extern __shared__ __align__(1024) uint8_t sm[];
   Bars& bars = *reinterpret_cast<Bars*>(sm + S::kBars);
-  float2* stats = reinterpret_cast<float2*>(sm + S::kStats + 256);
+  float2* stats = reinterpret_cast<float2*>(sm + S::kStats);
   volatile uint32_t* abort = &bars.abort;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t bad = 0;
@@ -67,10 +81,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   if (tid < 64) bars.broken[tid >> 3][tid & 7] = 0;
   if (tid == 0) {
     for (uint32_t i = 0; i < S::kSlots; ++i) {
-      mbar_init(&bars.kv_full[i], kLoaders);
+      mbar_init(&bars.kv_full[i], 1);
       mbar_init(&bars.kv_empty[i], 1);
+      mbar_init(&bars.fix_full[i], 1);
     }
-    mbar_init(&bars.q_full, kLoaders);
+    mbar_init(&bars.q_full, 1);
     mbar_init(&bars.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
@@ -102,112 +117,140 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   // the same for a whole warp, whose lanes must go on or stop together
   auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
   Walk w;
-  if (w.begin(p, blockIdx.x, bad)) {
-    if (warp == 8 || warp == 9) {
-      // ---- loaders: a warp has two groups of 32 rows of a block; a lane looks up a key of each, and
-      // 8 or 16 lanes copy a row
-      const uint32_t lw = warp - 8;
+  const bool work = w.begin(p, blockIdx.x, bad);
+  const uint32_t half = p.rows / 2;  // rows of a tile's first score tile
+  if (warp >= 8) {
+    shrink_registers<kOtherRegs>();
+    if (work && warp < kMmaWarp) {
+      // ---- both walk the slots in the order in which the MMAs take them.  One of them fills all
+      // slots (a slot's turns can only be told apart by the warp that waits for each of them): the
+      // loading warp, or without maps of the cache the copying warp.  The copying warp hands on
+      // the values whose last rows have to be cleared.  Each slot is announced once on kv_full.
+      const bool copier = warp == kCopyWarp, filler = copier == (maps.box_rows == 0);
       constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
       const uint32_t dim = p.c.head_dim;
-      uint32_t issued = 0, done = 0, seg = 0;
+      uint32_t issued = 0, seg = 0, fixes = 0;
+      uint32_t sent_fix = 0, sent_turn = 0;  // filler, a bit a slot: its last copy goes to fix_full, that one's phase
       bool ok = true;
-      auto arrive_one = [&]() {
-        fence_proxy_async_smem();
-        mbar_arrive(&bars.kv_full[done % S::kSlots]);
-        ++done;
-      };
-      // copies rows r0 .. r0 + 31 from the lanes' element offsets `where`
-      auto rows_to = [&](uint32_t dst, uint32_t half_bytes, uint32_t r0, const T* src, uint64_t where, bool real) {
-        const uint32_t live = ballot(real);
-#pragma unroll
-        for (uint32_t x = 0; x < kPieces; ++x) {
-          const uint32_t at = x * 32 + lane, j = at / kPieces, c = at % kPieces, r = r0 + j;
-          const uint64_t row = __shfl_sync(0xffffffffu, where, j);
-          const bool copy = (live >> j & 1u) != 0 && c * 8 < dim;
-          cp_async16(dst + (c >> 3) * half_bytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
-                     copy ? 16u : 0u);
-        }
-      };
       while (ok && w.left != 0) {
         w.open(p);
         const Request q = w.q;
         const uint32_t rows = q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
-        const bool two = rows - row0 > kRows;
+        const bool two = rows - row0 > half;
         const int32_t* table = p.a.tables + static_cast<uint64_t>(w.r) * p.a.table_stride;
         uint32_t* broken = bars.broken[seg & 7];
         auto load = [&](uint32_t b, bool values) {
-          const uint32_t slot = issued % S::kSlots;
-          if (issued >= S::kSlots) ok = ok && wait_all(&bars.kv_empty[slot], issued / S::kSlots - 1);
+          const uint32_t slot = issued % S::kSlots, turn = issued / S::kSlots - 1;
+          const bool reuse = issued >= S::kSlots;
+          ++issued;
           if (!ok) return;
-          const uint32_t dst = smem_u32(sm + S::kRing + slot * S::kSlot);
-          constexpr uint32_t kHalf = kKeys * 128;
-          for (uint32_t r0 = lw * 64; r0 < lw * 64 + 64; r0 += 32) {
-            if (b < q.cached_blocks) {
-              const uint32_t key = b * kKeys + r0 + lane;
-              const bool real = key < q.ctx;
-              const uint64_t where = real ? key_offset(p, table, key, w.head, bad) : 0;
-              rows_to(dst, kHalf, r0, static_cast<const T*>(values ? p.c.v : p.c.k), where, real);
-            } else {
-              const uint32_t node = (b - q.cached_blocks) * kKeys + r0 + lane;
-              const bool real = node < q.nodes;
-              const uint64_t where = real ? (q.start + node) * p.a.kv_token_stride + w.head * p.a.kv_head_stride : 0;
-              if (!values) {
-                rows_to(dst, kHalf, r0, static_cast<const T*>(p.a.k), where, real);
-              } else {
-                // through registers: a weight of zero must cancel a hidden node's values whatever they
-                // are, so infinities and NaN become zeros here, and the rows that see the node get
-                // them at the end
-                const uint32_t live = ballot(real);
-  #pragma unroll 4
-                for (uint32_t x = 0; x < kPieces; ++x) {
-                  const uint32_t at = x * 32 + lane, j = at / kPieces, c = at % kPieces, r = r0 + j;
-                  const uint64_t row = __shfl_sync(0xffffffffu, where, j);
-                  uint4 v = make_uint4(0, 0, 0, 0);
-                  if ((live >> j & 1u) != 0 && c * 8 < dim)
-                    v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.v) + row + c * 8));
-                  uint32_t e[4] = {v.x, v.y, v.z, v.w};
-                  bool found = false;
-  #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    constexpr uint32_t kMask = Elem<T>::kExpMask;
-                    if ((e[i] & kMask) == kMask) e[i] &= 0xFFFF0000u, found = true;
-                    if ((e[i] >> 16 & kMask) == kMask) e[i] &= 0x0000FFFFu, found = true;
-                  }
-                  if (found) atomicOr(&broken[((b - q.cached_blocks) * kKeys + r) >> 5], 1u << (r & 31));
-                  *reinterpret_cast<uint4*>(sm + S::kRing + slot * S::kSlot + (c >> 3) * kHalf + r * 128 +
-                                            (((c & 7) ^ (r & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+          const bool cached = b < q.cached_blocks;
+          const uint32_t first = (cached ? b : b - q.cached_blocks) * kKeys;
+          const uint32_t valid = min(kKeys, (cached ? q.ctx : q.nodes) - first);
+          const bool fix = values && (!cached || valid < kKeys);  // rows to clear
+          uint8_t* const at = sm + S::kRing + slot * S::kTile;
+          const uint32_t dst = smem_u32(at);
+          if (filler && reuse) ok = wait_all(&bars.kv_empty[slot], turn);
+          if (!ok) return;
+          if (cached && maps.box_rows == 0) {
+            if (!filler) return;
+            const T* src = static_cast<const T*>(values ? p.c.v : p.c.k);
+            for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
+              const uint64_t where = r0 + lane < valid ? key_offset(p, table, first + r0 + lane, w.head, bad) : 0;
+#pragma unroll 4
+              for (uint32_t x = 0; x < kPieces; ++x) {
+                const uint32_t i = x * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
+                const uint64_t row = __shfl_sync(0xffffffffu, where, j);
+                const bool copy = r < valid && c * 8 < dim;
+                cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
+                           copy ? 16u : 0u);
+              }
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
+            return;
+          }
+          if (filler) {
+            uint64_t* bar = fix ? &bars.fix_full[slot] : &bars.kv_full[slot];
+            sent_fix = fix ? sent_fix | 1u << slot : sent_fix & ~(1u << slot);
+            if (fix) sent_turn ^= 1u << slot;
+            if (cached) {
+              // a lane a box; boxes past the end of the context are left out (scores of what lies there
+              // are hidden, values are cleared)
+              const uint32_t boxes = kKeys / maps.box_rows, real = (valid + maps.box_rows - 1) / maps.box_rows;
+              const uint32_t box = lane % boxes, h = lane / boxes;
+              if (lane == 0) mbar_expect_tx(bar, real * maps.box_rows * DP * 2);
+              __syncwarp();
+              if (h < DP / 64 && box < real) {
+                const uint32_t key = first + box * maps.box_rows, column = key / p.c.page_size;
+                uint32_t page = static_cast<uint32_t>(__ldg(table + column));
+                if (page >= p.c.num_pages) {
+                  bad |= HQB_DEVERR_PAGES;
+                  page = 0;
                 }
+                tma_load_4d(dst + h * S::kHalf + box * maps.box_rows * 128, values ? &maps.cv : &maps.ck, bar, h * 64, w.head,
+                            key - column * p.c.page_size, page);
+              }
+            } else {
+              if (lane == 0) mbar_expect_tx(bar, S::kTile);
+              __syncwarp();
+              if (lane < DP / 64)
+                tma_load_3d(dst + lane * S::kHalf, values ? &maps.v : &maps.k, bar, lane * 64, w.head, q.start + first);
+            }
+          }
+          if (!copier || !fix) return;
+          ok = wait_all(&bars.fix_full[slot], fixes >> slot);
+          if (!ok) return;
+          fixes ^= 1u << slot;
+          // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
+          // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
+          // node get at the end
+          for (uint32_t i = lane; i < kKeys * kPieces; i += 32) {
+            const uint32_t r = i / kPieces, c = i % kPieces;
+            uint4* e = reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            if (r >= valid) {
+              *e = make_uint4(0, 0, 0, 0);
+            } else if (!cached) {
+              constexpr uint32_t kMask = Elem<T>::kExpMask;
+              const uint4 v = *e;
+              uint32_t u[4] = {v.x, v.y, v.z, v.w};
+              bool found = false;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if ((u[k] & kMask) == kMask) u[k] &= 0xFFFF0000u, found = true;
+                if ((u[k] >> 16 & kMask) == kMask) u[k] &= 0x0000FFFFu, found = true;
+              }
+              if (found) {
+                atomicOr(&broken[(first + r) >> 5], 1u << (r & 31));
+                *e = make_uint4(u[0], u[1], u[2], u[3]);
               }
             }
           }
-          cp_async_commit();
-          ++issued;
-          if (issued - done > S::kLag) {
-            cp_async_wait<S::kLag>();
-            arrive_one();
-          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
         };
-        // the first keys, then the queries (the last segment's must have been read), then the rest in
-        // the order in which the MMAs take them
+        // the first keys, then the queries (the last segment's must have been read), then the rest.  Only
+        // the loading warp may wait for q_empty: a warp that the MMAs do not wait for in every segment
+        // could find it two phases on.
         load(w.b0, false);
-        if (seg > 0) ok = ok && wait_all(&bars.q_empty, seg - 1);
-        if (!ok) break;
-        // past here the epilogue of segment seg - 3 is over: the flags of segment seg - 4 are free
-        if (lw == 0 && lane < 8) bars.broken[(seg + 4) & 7][lane] = 0;
-        for (uint32_t r0 = lw * 64; r0 < (two ? 2 * kRows : kRows); r0 += (r0 & 32) ? 96 : 32) {
-          const uint32_t row = row0 + r0 + lane;
-          const bool real = row < rows;
-          const uint32_t node = real ? row / p.group : 0u;
-          const uint64_t where = real ? (q.start + node) * p.a.q_token_stride +
-                                            static_cast<uint64_t>(w.head * p.group + row - node * p.group) * p.a.q_head_stride
-                                      : 0;
-          rows_to(smem_u32(sm + (r0 / kRows) * S::kQTile), kRows * 128, r0 % kRows, static_cast<const T*>(p.a.q), where, real);
+        if (!copier) {
+          if (seg > 0) ok = ok && wait_all(&bars.q_empty, seg - 1);
+          if (!ok) break;
+          // past here the epilogue of segment seg - 3 is over: the flags of segment seg - 4 are free
+          if (lane < 8) bars.broken[(seg + 4) & 7][lane] = 0;
+          const uint32_t tiles = two ? 2u : 1u;
+          if (lane == 0) mbar_expect_tx(&bars.q_full, tiles * half * DP * 2);
+          __syncwarp();
+          if (lane < tiles * (DP / 64)) {
+            const uint32_t t = lane / (DP / 64), h = lane % (DP / 64);
+            tma_load_3d(smem_u32(sm + t * S::kTile + h * S::kHalf), &maps.q, &bars.q_full, h * 64, w.head * p.group,
+                        q.start + (row0 + t * half) / p.group);
+          }
         }
-        cp_async_commit();
-        cp_async_wait<0>();
-        while (done < issued) arrive_one();
-        fence_proxy_async_smem();
-        mbar_arrive(&bars.q_full);
         if (two) {
           for (uint32_t i = 0; ok && i < n; ++i) {
             if (i > 0) load(w.b0 + i, false);
@@ -220,14 +263,18 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             if (i + 2 < n) load(w.b0 + i + 2, false);
           }
         }
-        // the tail of the segment must not wait for the next segment's loads
-        cp_async_wait<0>();
-        while (done < issued) arrive_one();
         ++seg;
         w.advance(p, bad);
       }
-      cp_async_wait<0>();
-    } else if (warp == kMmaWarp) {
+      if (!ok && filler && maps.box_rows != 0) {  // copies in flight end before the CTA does
+        for (uint32_t i = issued > S::kSlots ? issued - S::kSlots : 0; i < issued; ++i) {
+          const uint32_t slot = i % S::kSlots;
+          if (sent_fix >> slot & 1u) mbar_wait(&bars.fix_full[slot], (sent_turn >> slot & 1u) ^ 1u, p.error);
+          else mbar_wait(&bars.kv_full[slot], i / S::kSlots & 1u, p.error);
+        }
+      }
+      if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
+    } else if (work && warp == kMmaWarp) {
       // ---- MMA issuer
       if (lane == 0) {
         constexpr uint32_t kType = sizeof(T) == 2 && Elem<T>::kExpMask == 0x7F80u ? 1u : 0u;  // BF16 : FP16
@@ -237,21 +284,22 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         uint32_t slot_at = 0, seg = 0, p_at[2] = {0, 0};
         bool ok = true;
         auto slot_wait = [&](uint32_t n) { return wait(&bars.kv_full[n % S::kSlots], n / S::kSlots); };
-        auto slot_addr = [&](uint32_t n) { return smem_u32(sm + S::kRing + (n % S::kSlots) * S::kSlot); };
+        auto slot_addr = [&](uint32_t n) { return smem_u32(sm + S::kRing + (n % S::kSlots) * S::kTile); };
+        // descriptors step by their address field (16-byte units)
         auto scores = [&](uint32_t s, uint32_t tile, uint32_t slot) {
-          const uint32_t qa = smem_u32(sm + tile * S::kQTile), ka = slot_addr(slot);
+          const uint64_t qd = umma_desc_sw128(smem_u32(sm + tile * S::kTile), 16), kd = umma_desc_sw128(slot_addr(slot), 16);
 #pragma unroll
-          for (uint32_t k = 0; k < DP / 16; ++k)
-            tc_mma_f16_ss(tmem + s * 128, umma_desc_sw128(qa + (k >> 2) * (kRows * 128) + (k & 3) * 32, 16),
-                          umma_desc_sw128(ka + (k >> 2) * (kKeys * 128) + (k & 3) * 32, 16), kScores, k > 0 ? 1u : 0u);
+          for (uint32_t k = 0; k < DP / 16; ++k) {
+            const uint32_t step = (k >> 2) * (S::kHalf >> 4) + (k & 3) * 2;
+            tc_mma_f16_ss(tmem + s * 128, qd + step, kd + step, kScores, k > 0 ? 1u : 0u);
+          }
           tc_commit(&bars.s_full[s]);
         };
         auto sums = [&](uint32_t s, uint32_t slot, bool first) {
-          const uint32_t va = slot_addr(slot);
+          const uint64_t vd = umma_desc_sw128(slot_addr(slot), S::kHalf);
 #pragma unroll
           for (uint32_t k = 0; k < kKeys / 16; ++k)
-            tc_mma_f16_ts(tmem + 256 + s * DP, tmem + s * 128 + k * 8, umma_desc_sw128(va + k * 2048, kKeys * 128), kSums,
-                          k > 0 || !first ? 1u : 0u);
+            tc_mma_f16_ts(tmem + 256 + s * DP, tmem + s * 128 + k * 8, vd + k * 128, kSums, k > 0 || !first ? 1u : 0u);
         };
         auto weights_wait = [&](uint32_t s) {
           const bool r = wait(&bars.p_full[s], p_at[s]);
@@ -262,7 +310,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         while (ok && w.left != 0) {
           w.open(p);
           const uint32_t n = w.b1 - w.b0;
-          const bool two = w.q.nodes * p.group - w.tile * p.rows > kRows;
+          const bool two = w.q.nodes * p.group - w.tile * p.rows > half;
           ok = wait(&bars.q_full, seg);
           if (!ok) break;
           if (two) {
@@ -343,7 +391,10 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           mbar_wait(&bars.drain, 0, p.error);
         }
       }
-    } else if (warp < 8) {
+    }
+  } else {
+    grow_registers<kSoftmaxRegs>();
+    if (work) {
       // ---- softmax: stream s, row = tensor-memory lane
       const uint32_t s = warp >> 2, lrow = (warp & 3) * 32 + lane;
       const uint32_t lanes = ((warp & 3) * 32u) << 16;
@@ -356,9 +407,9 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         w.open(p);
         const Request q = w.q;
         const uint32_t rows = q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
-        const bool two = rows - row0 > kRows;
-        const uint32_t row = row0 + (two ? s * kRows : 0u) + lrow;
-        const bool live = row < rows;
+        const bool two = rows - row0 > half;
+        const uint32_t row = row0 + (two ? s * half : 0u) + lrow;
+        const bool live = lrow < half && row < rows;
         const uint32_t node = live ? row / p.group : 0u;
         const uint32_t mine = two ? n : (n + 1 - s) / 2;
         float m = -INFINITY, l = 0.0f;
@@ -385,24 +436,19 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           if (!(ok = wait_all(&bars.s_full[s], s_at))) break;
           ++s_at;
           tc_fence_after();
-          float top = -INFINITY;
+          uint32_t v[128];
+          tc_ld_x128(sc, v);
+          if (!all) {
 #pragma unroll
-          for (uint32_t x = 0; x < 4; ++x) {
-            uint32_t v[32];
-            tc_ld_x32(sc + x * 32, v);
-            float t0 = -INFINITY, t1 = -INFINITY;
-            if (all) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                t0 = fmaxf(t0, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                t1 = fmaxf(t1, fmaxf(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])));
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) t0 = fmaxf(t0, (sees[x] >> e & 1u) ? __uint_as_float(v[e]) : -INFINITY);
-            }
-            top = fmaxf(top, fmaxf(t0, t1));
+            for (int e = 0; e < 128; ++e) v[e] = (sees[e >> 5] >> (e & 31) & 1u) ? v[e] : 0xFF800000u;
           }
+          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 128; e += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              t4[k] = fmaxf(t4[k], fmaxf(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])));
+          const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
           const float tops = top * c;
           const bool grow = tops > m + kSlack || (m == -INFINITY && tops > m);
           if (ballot(grow) != 0) {
@@ -413,11 +459,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             if (i > 0) {  // the sums of the blocks before this one are complete: their MMAs precede this score's
 #pragma unroll
               for (uint32_t x = 0; x < DP / 32; ++x) {
-                uint32_t v[32];
-                tc_ld_x32(oc + x * 32, v);
+                uint32_t o[32];
+                tc_ld_x32(oc + x * 32, o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                tc_st_x32(oc + x * 32, v);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc_st_x32(oc + x * 32, o);
               }
             }
           }
@@ -426,15 +472,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           uint64_t sum2 = pack2(0.0f, 0.0f);
 #pragma unroll
           for (uint32_t x = 0; x < 4; ++x) {
-            uint32_t v[32], w16[16];
-            tc_ld_x32(sc + x * 32, v);
-            if (!all) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = (sees[x] >> e & 1u) ? v[e] : 0xFF800000u;
-            }
+            uint32_t w16[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float2 t = unpack2(fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, u2));
+              const float2 t = unpack2(
+                  fma2(pack2(__uint_as_float(v[x * 32 + 2 * e]), __uint_as_float(v[x * 32 + 2 * e + 1])), c2, u2));
               const float a = fast_exp2(t.x), d = fast_exp2(t.y);
               sum2 = add2(sum2, pack2(a, d));
               w16[e] = Elem<T>::pack(a, d);
@@ -540,14 +582,48 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled f = [] {
+    void* at = nullptr;
+    cudaDriverEntryPointQueryResult found{};
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &at, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return static_cast<EncodeTiled>(nullptr);
+    }
+    return reinterpret_cast<EncodeTiled>(at);
+  }();
+  return f;
+}
+
+// A map of boxes of 64 columns; dims, box: the dimensions after the columns.  false: no such map.
+bool encode_map(CUtensorMap* map, const AttnParams& p, const void* base, uint32_t rank, const uint64_t* dims,
+                const uint64_t* strides, const uint32_t* box) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  cuuint64_t size[4] = {p.c.head_dim}, step[3];
+  cuuint32_t boxes[4] = {64}, ones[4] = {1, 1, 1, 1};
+  for (uint32_t i = 0; i + 1 < rank; ++i) {
+    size[i + 1] = dims[i];
+    step[i] = dims[i] > 1 ? strides[i] * 2 : 16;  // the stride of a dimension of one element is never used
+    boxes[i + 1] = box[i];
+    if (step[i] == 0 || step[i] % 16 != 0 || step[i] >= (1ull << 40)) return false;
+  }
+  return encode(map, p.c.dtype == HQB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                const_cast<void*>(base), size, step, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP>
-cudaError_t launch(const AttnParams& p, cudaStream_t st) {
+cudaError_t launch(const AttnParams& p, const Maps& maps, cudaStream_t st) {
   static DeviceOnce once;
-  constexpr uint32_t smem = TmemShape<DP>::kBytes + 512;
+  constexpr uint32_t smem = TmemShape<DP>::kBytes;
   static_assert(smem <= 232448, "one CTA's shared memory");
   const cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_tmem_kernel<T, DP>), smem);
   if (e != cudaSuccess) return e;
-  attention_tmem_kernel<T, DP><<<p.grid, kTmemThreads, smem, st>>>(p);
+  attention_tmem_kernel<T, DP><<<p.grid, kTmemThreads, smem, st>>>(p, maps);
   return cudaGetLastError();
 }
 
@@ -555,7 +631,24 @@ cudaError_t launch(const AttnParams& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_attention_tmem(const AttnParams& p, cudaStream_t st) {
-  return p.dim_pad == 64 ? launch<T, 64>(p, st) : launch<T, 128>(p, st);
+  Maps m{};
+  const uint64_t q_dims[2] = {p.a.q_heads, p.a.tokens}, q_strides[2] = {p.a.q_head_stride, p.a.q_token_stride};
+  const uint64_t n_dims[2] = {p.c.kv_heads, p.a.tokens}, n_strides[2] = {p.a.kv_head_stride, p.a.kv_token_stride};
+  const uint32_t q_box[2] = {p.group, kRows / p.group}, n_box[2] = {1, kKeys};
+  if (!encode_map(&m.q, p, p.a.q, 3, q_dims, q_strides, q_box) || !encode_map(&m.k, p, p.a.k, 3, n_dims, n_strides, n_box) ||
+      !encode_map(&m.v, p, p.a.v, 3, n_dims, n_strides, n_box))
+    return cudaErrorNotSupported;
+  // the largest power of two that divides the page size; the swizzle repeats every 8 rows, so
+  // smaller pieces of a page come by plain copies
+  uint32_t rows = p.c.page_size & (~p.c.page_size + 1);
+  rows = rows > kKeys ? kKeys : rows;
+  const uint64_t c_dims[3] = {p.c.kv_heads, p.c.page_size, p.c.num_pages};
+  const uint64_t c_strides[3] = {p.c.head_stride, p.c.token_stride, p.c.page_stride};
+  const uint32_t c_box[3] = {1, rows, 1};
+  if (rows >= 8 && encode_map(&m.ck, p, p.c.k, 4, c_dims, c_strides, c_box) &&
+      encode_map(&m.cv, p, p.c.v, 4, c_dims, c_strides, c_box))
+    m.box_rows = rows;
+  return p.dim_pad == 64 ? launch<T, 64>(p, m, st) : launch<T, 128>(p, m, st);
 }
 template cudaError_t launch_attention_tmem<__half>(const AttnParams&, cudaStream_t);
 template cudaError_t launch_attention_tmem<__nv_bfloat16>(const AttnParams&, cudaStream_t);

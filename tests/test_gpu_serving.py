@@ -395,6 +395,9 @@ SHAPES = [
     ([3000, 50], [31, 64], 64, 8, 128, 64), ([100, 200], [7, 9], 6, 2, 96, 16), ([777], [20], 5, 5, 40, 7),
     ([90, 300], [3, 2], 4, 2, 256, 16), ([1500], [30], 16, 1, 160, 300), ([33], [2], 3, 1, 8, 1), ([513], [100], 40, 1, 64, 16),
     ([64 * k for k in range(20)], [1 + k % 5 for k in range(20)], 16, 4, 128, 16),
+    # many short pieces of items a CTA, with and without an item's end in them
+    ([4096 - 131 * k for k in range(16)], [8 - k % 6 for k in range(16)], 64, 8, 128, 32),
+    ([1024 + 128 * k for k in range(24)], [3] * 24, 32, 4, 64, 64), ([640] * 30, [40] * 30, 8, 2, 128, 128),
 ]
 
 
