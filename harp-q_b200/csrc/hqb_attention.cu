@@ -43,7 +43,9 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
   griddep_launch_dependents();
   griddep_wait();
   Walk w;
-  if (!w.begin(p, blockIdx.x, bad)) return;
+  const bool work = w.begin(p, blockIdx.x, bad);
+  if (threadIdx.x == 0 && !p.whole) note_split(p, w, blockIdx.x, work, bad);
+  if (!work) return;
   const uint32_t dim = p.c.head_dim;
   const T* const kc = static_cast<const T*>(p.c.k);
   const T* const vc = static_cast<const T*>(p.c.v);
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
         const uint32_t nd = at / p.group, h = w.head * p.group + at - nd * p.group;
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
         T* out = static_cast<T*>(p.a.out) + (q.start + nd) * p.a.out_token_stride + h * p.a.out_head_stride;
-        float* keep = part_row(p, blockIdx.x, w.b0 == 0 ? 1u : 0u, row);
+        float* keep = part_sums(p, blockIdx.x, w.b0 == 0 ? 1u : 0u) + row * 4;
         for (uint32_t d = part * 2; d < DP; d += 16) {
           float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -337,11 +339,11 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
               if (d + 1 < dim) out[d + 1] = Elem<T>::from_float(ll == 0.0f ? 0.0f : o.y * inv);
             }
           } else {
-            *reinterpret_cast<float2*>(keep + d) = o;
+            *reinterpret_cast<float2*>(keep + (d >> 2) * p.rows * 4 + (d & 3)) = o;
           }
         }
         if (part == 0) {
-          if (!complete) *reinterpret_cast<float2*>(keep + DP) = make_float2(mm, ll);
+          if (!complete) part_stats(p, blockIdx.x, w.b0 == 0 ? 1u : 0u)[row] = make_float2(mm, ll);
           else if (p.a.lse != nullptr)
             p.a.lse[static_cast<uint64_t>(q.start + nd) * p.a.q_heads + h] =
                 ll == 0.0f ? -INFINITY : (mu + log2f(ll)) * 0.6931471805599453f;
@@ -354,60 +356,64 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
   if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
 }
 
-// One CTA per (item, 16 of its rows): the partial results of the CTAs that the item spans, in
-// their order, joined by their maxima.  An item that one CTA finished is left alone.
+constexpr uint32_t kJoinRows = 32;
+constexpr uint32_t kJoinThreads = 512;
+
+// One CTA per (CTA of the attention, 32 rows): the partial results of the item that begins there
+// and spans later CTAs, in their order, joined by their maxima.  A thread has 4 columns of a row
+// and reads 8 partial results at once, so the whole is three trips to memory long.
 template <typename T>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnParams p) {
-  const uint32_t per_request = p.max_tiles * p.c.kv_heads;
-  const uint32_t r = blockIdx.x / per_request, in_request = blockIdx.x - r * per_request;
-  uint32_t bad = 0;
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
+  const uint32_t first = blockIdx.x;
   griddep_wait();
-  const Request q = load_request(p, r, bad);
-  if (in_request >= q.tiles * p.c.kv_heads) return;
-  const uint32_t head = in_request / q.tiles, tile = in_request - head * q.tiles;
-  uint64_t before;
-  const uint64_t units = total_units(p, r, &before, bad);
-  const uint32_t ctas = busy_ctas(p, units);
-  const uint64_t u0 = before + static_cast<uint64_t>(in_request) * q.blocks;
-  const uint32_t first = cta_of_unit(u0, units, ctas), last = cta_of_unit(u0 + q.blocks - 1, units, ctas);
-  if (first == last) return;
-  const uint32_t row = blockIdx.y * 16 + (threadIdx.x >> 3), part = threadIdx.x & 7;
-  const uint32_t at = tile * p.rows + row;
+  const Split q = p.splits[first];
+  if (q.last == first) return;
+  const uint32_t row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, at = q.tile * p.rows + row;
   if (row >= p.rows || at >= q.nodes * p.group) return;
-  float mm = -INFINITY;
-#pragma unroll 4
-  for (uint32_t c = first; c <= last; ++c) mm = fmaxf(mm, part_row(p, c, c == first ? 1u : 0u, row)[p.dim_pad]);
-  const float mu = mm == -INFINITY ? 0.0f : mm;
-  float ll = 0.0f;
-#pragma unroll 4
-  for (uint32_t c = first; c <= last; ++c) {
-    const float2 s = *reinterpret_cast<const float2*>(part_row(p, c, c == first ? 1u : 0u, row) + p.dim_pad);
-    ll += fast_exp2(s.x - mu) * s.y;
-  }
-  const uint32_t nd = at / p.group, h = head * p.group + at - nd * p.group, dim = p.c.head_dim;
-  T* out = static_cast<T*>(p.a.out) + (q.start + nd) * p.a.out_token_stride + h * p.a.out_head_stride;
-  const float inv = 1.0f / ll;
-  for (uint32_t d = part * 2; d < dim; d += 16) {
-    float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-    for (uint32_t c = first; c <= last; ++c) {
-      const float* x = part_row(p, c, c == first ? 1u : 0u, row);
-      const float f = fast_exp2(x[p.dim_pad] - mu);
-      const float2 v = *reinterpret_cast<const float2*>(x + d);
-      o.x += f * v.x;
-      o.y += f * v.y;
+  const uint32_t nd = at / p.group, h = q.head * p.group + at - nd * p.group, dim = p.c.head_dim;
+  for (uint32_t d = threadIdx.x / kJoinRows * 4; d < dim; d += kJoinThreads / kJoinRows * 4) {
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t c0 = first; c0 <= q.last; c0 += 8) {
+      float2 s[8];
+      float4 v[8];
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t c = min(c0 + k, q.last), slot = c == first ? 1u : 0u;
+        s[k] = part_stats(p, c, slot)[row];
+        v[k] = *reinterpret_cast<const float4*>(part_sums(p, c, slot) + ((d >> 2) * p.rows + row) * 4);
+      }
+      float top = m;
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
+      const float use = top == -INFINITY ? 0.0f : top, old = fast_exp2(m - use);
+      l *= old;
+      o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+      m = top;
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        if (c0 + k > q.last) break;
+        const float f = fast_exp2(s[k].x - use);
+        l += f * s[k].y;
+        o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+      }
     }
-    out[d] = Elem<T>::from_float(ll == 0.0f ? 0.0f : o.x * inv);
-    if (d + 1 < dim) out[d + 1] = Elem<T>::from_float(ll == 0.0f ? 0.0f : o.y * inv);
+    T* out = static_cast<T*>(p.a.out) + (q.start + nd) * p.a.out_token_stride + h * p.a.out_head_stride;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      if (d + i < dim) out[d + i] = Elem<T>::from_float(l == 0.0f ? 0.0f : e[i]);
+    if (d == 0 && p.a.lse != nullptr)
+      p.a.lse[static_cast<uint64_t>(q.start + nd) * p.a.q_heads + h] =
+          l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
-  if (part == 0 && p.a.lse != nullptr)
-    p.a.lse[static_cast<uint64_t>(q.start + nd) * p.a.q_heads + h] =
-        ll == 0.0f ? -INFINITY : (mu + log2f(ll)) * 0.6931471805599453f;
 }
 
 struct Shape {
   uint32_t rows, block, max_tiles, dim_pad, grid, whole, tmem;
-  uint64_t parts_bytes;
+  uint64_t splits_bytes, parts_bytes;
+  uint64_t bytes() const { return 256 + round_up(splits_bytes + parts_bytes, 256); }  // with the error word
 };
 
 bool shape_ok(const hqb_paged_cache* c, const hqb_attention_args* a) {
@@ -460,6 +466,7 @@ Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem,
   // would add a second launch
   s.whole = static_cast<uint64_t>(a->max_context) + a->max_new <= 512 ? 1u : 0u;
   if (s.whole) s.grid = static_cast<uint32_t>(items < s.grid * 4ull ? (items > 0 ? items : 1) : s.grid * 4ull);
+  s.splits_bytes = s.whole ? 0 : static_cast<uint64_t>(s.grid) * sizeof(Split);
   s.parts_bytes = s.whole ? 0 : static_cast<uint64_t>(s.grid) * 2 * s.rows * (s.dim_pad + 2) * 4;
   return s;
 }
@@ -486,8 +493,9 @@ cudaError_t launch_attention(const AttnParams& p, bool vec, bool tmem, cudaStrea
   cudaError_t e = tmem ? launch_attention_tmem<T>(p, st) : vec ? launch_dim<T, true>(p, st) : launch_dim<T, false>(p, st);
   if (e != cudaSuccess || p.whole) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.a.requests * p.c.kv_heads * p.max_tiles, (p.rows + 15) / 16);
-  cfg.blockDim = dim3(128);
+  const uint32_t rows = p.rows < p.a.max_new * p.group ? p.rows : p.a.max_new * p.group;
+  cfg.gridDim = dim3(p.grid, (rows + kJoinRows - 1) / kJoinRows);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -509,9 +517,8 @@ HQB_API uint64_t hqb_tree_attention_workspace_bytes(const hqb_paged_cache* c, co
   const int sms = device_sm_count(device);
   if (sms <= 0) return 0;
   // the call chooses its kernel by alignment and scale too: room for either
-  const uint64_t rows = shape_of(c, a, false, sms).parts_bytes;
-  const uint64_t tmem = tmem_shape(c, a) ? shape_of(c, a, true, sms).parts_bytes : 0;
-  return 256 + round_up(tmem > rows ? tmem : rows, 256);
+  const uint64_t rows = shape_of(c, a, false, sms).bytes(), tmem = tmem_shape(c, a) ? shape_of(c, a, true, sms).bytes() : 0;
+  return tmem > rows ? tmem : rows;
 }
 
 HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_args* a, void* workspace,
@@ -535,14 +542,15 @@ HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_arg
   const bool vec = aligned_rows(c, a), tmem = takes_tmem(c, a, vec);
   const Shape s = shape_of(c, a, tmem, sms);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 ||
-      workspace_bytes < 256 + s.parts_bytes)
+      workspace_bytes < s.bytes())
     return HQB_ERR_INVALID;
   if (static_cast<uint64_t>(a->requests) * c->kv_heads * s.max_tiles > 0x7FFFFFFFull) return HQB_ERR_UNSUPPORTED;
   AttnParams p{};
   p.a = *a;
   p.c = *c;
   p.error = static_cast<int*>(workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
+  p.splits = reinterpret_cast<Split*>(static_cast<uint8_t*>(workspace) + 256);
+  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256 + s.splits_bytes);
   p.group = a->q_heads / c->kv_heads;
   p.rows = s.rows;
   p.block = s.block;

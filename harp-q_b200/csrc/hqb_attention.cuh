@@ -14,11 +14,14 @@
 
 namespace hqb {
 
+struct Split;
+
 struct AttnParams {
   hqb_attention_args a;
   hqb_paged_cache c;
   int* error;
-  float* parts;         // [cta][2][row tile][dim_pad + 2]
+  Split* splits;       // [cta] the item that begins in the CTA and ends in a later one
+  float* parts;         // [cta][2] partial results: see part_sums
   uint32_t group;       // query heads per key head
   uint32_t rows;        // rows of a row tile
   uint32_t block;       // keys of a block
@@ -28,6 +31,13 @@ struct AttnParams {
   uint32_t whole;       // 1: items are not cut (a unit is an item, no partials)
   uint32_t grid;        // CTAs of the attention kernel
   float scale_log2;     // scale * log2(e)
+};
+
+// What attention_join_kernel has to know of an item whose parts are in CTAs c .. last.
+struct Split {
+  uint32_t last;  // c itself: nothing to join
+  uint32_t start, nodes, head, tile;
+  uint32_t pad[3];
 };
 
 struct Request {
@@ -62,67 +72,64 @@ __device__ __forceinline__ uint64_t request_units(const AttnParams& p, const Req
   return static_cast<uint64_t>(q.tiles) * p.c.kv_heads * (p.whole ? 1u : q.blocks);
 }
 
-// Sum of the units of all requests, and of those before `until`; a whole warp calls it.
-__device__ __forceinline__ uint64_t total_units(const AttnParams& p, uint32_t until, uint64_t* before, uint32_t& bad) {
-  uint64_t all = 0, early = 0;
-  for (uint32_t r = threadIdx.x & 31; r < p.a.requests; r += 32) {
-    const uint64_t u = request_units(p, load_request(p, r, bad));
-    all += u;
-    if (r < until) early += u;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    early += __shfl_xor_sync(0xffffffffu, early, o);
-  }
-  *before = early;
-  return all;
+// 64-bit quotients cost a few hundred cycles; nearly all of them fit 32 bits.
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
+  return (a | b) >> 32 == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
 // CTAs that get units: at least min_blocks each, so that short work is not cut into pieces
 // smaller than the cost of joining them.
 __device__ __forceinline__ uint32_t busy_ctas(const AttnParams& p, uint64_t units) {
-  const uint64_t most = p.whole ? units : (units + p.min_blocks - 1) / p.min_blocks;
+  const uint64_t most = p.whole ? units : quotient(units + p.min_blocks - 1, p.min_blocks);
   return static_cast<uint32_t>(most < p.grid ? most : p.grid);
 }
 
 __device__ __forceinline__ uint64_t first_unit(uint32_t cta, uint64_t units, uint32_t ctas) {
-  return units * cta / ctas;
+  return quotient(units * cta, ctas);
 }
 // The CTA whose range [first_unit(i), first_unit(i + 1)) holds unit u.
 __device__ __forceinline__ uint32_t cta_of_unit(uint64_t u, uint64_t units, uint32_t ctas) {
-  return static_cast<uint32_t>(((u + 1) * ctas - 1) / units);
+  return static_cast<uint32_t>(quotient((u + 1) * ctas - 1, units));
 }
 
 // A CTA's walk over its units, one segment (a range of one item's blocks) at a time.  Every
 // thread keeps its own copy; begin() is called by whole warps.
 struct Walk {
-  uint64_t left;   // units not yet handed out
+  uint64_t left;         // units not yet handed out
+  uint64_t units, past;  // of the whole call; the first after this CTA's
+  uint32_t ctas;
   uint32_t r, head, tile, unit;
   Request q;
   // the current segment
   uint32_t b0, b1;
 
   __device__ __forceinline__ bool begin(const AttnParams& p, uint32_t cta, uint32_t& bad) {
-    uint64_t before;
-    const uint64_t units = total_units(p, 0, &before, bad);
-    const uint32_t ctas = busy_ctas(p, units);
-    left = 0;
-    if (cta >= ctas) return false;
-    const uint64_t u0 = first_unit(cta, units, ctas);
-    left = first_unit(cta + 1, units, ctas) - u0;
-    // the request that holds unit u0
-    uint64_t carry = 0;
     const uint32_t lane = threadIdx.x & 31;
-    for (uint32_t r0 = 0; r0 < p.a.requests; r0 += 32) {
-      uint64_t mine = 0;
-      if (r0 + lane < p.a.requests) mine = request_units(p, load_request(p, r0 + lane, bad));
-      uint64_t inc = mine;
+    uint64_t mine = 0, inc = 0;  // inc: inclusive sum of a round of 32 requests
+    units = 0;
+    auto round = [&](uint32_t r0) {
+      mine = r0 + lane < p.a.requests ? request_units(p, load_request(p, r0 + lane, bad)) : 0;
+      inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= static_cast<uint32_t>(o)) inc += up;
       }
+    };
+    for (uint32_t r0 = 0; r0 < p.a.requests; r0 += 32) {
+      round(r0);
+      units += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    ctas = busy_ctas(p, units);
+    left = 0;
+    if (cta >= ctas) return false;
+    const uint64_t u0 = first_unit(cta, units, ctas);
+    past = first_unit(cta + 1, units, ctas);
+    left = past - u0;
+    // the request that holds unit u0
+    uint64_t carry = 0;
+    for (uint32_t r0 = 0; r0 < p.a.requests; r0 += 32) {
+      if (p.a.requests > 32) round(r0);  // else the one round's sums are at hand
       const uint32_t past = ballot(carry + inc > u0);
       if (past != 0) {
         const uint32_t at = __ffs(past) - 1;
@@ -130,9 +137,9 @@ struct Walk {
         r = r0 + at;
         q = load_request(p, r, bad);
         const uint32_t per_item = p.whole ? 1u : q.blocks;
-        const uint64_t item = skip / per_item;
+        const uint64_t item = quotient(skip, per_item);
         unit = static_cast<uint32_t>(skip - item * per_item);
-        head = static_cast<uint32_t>(item / q.tiles);
+        head = static_cast<uint32_t>(quotient(item, q.tiles));
         tile = static_cast<uint32_t>(item - static_cast<uint64_t>(head) * q.tiles);
         return true;
       }
@@ -170,9 +177,38 @@ struct Walk {
   __device__ __forceinline__ bool complete() const { return b0 == 0 && b1 == q.blocks; }
 };
 
-// Slot (of a CTA's two) of a partial segment: 1 where the item begins in this CTA, else 0.
-__device__ __forceinline__ float* part_row(const AttnParams& p, uint32_t cta, uint32_t slot, uint32_t row) {
-  return p.parts + ((static_cast<uint64_t>(cta) * 2 + slot) * p.rows + row) * (p.dim_pad + 2);
+// Writes down a CTA's split item: every CTA once, by one thread, after begin().  Only a CTA's last
+// item can begin in it and end in a later one.
+__device__ __forceinline__ void note_split(const AttnParams& p, Walk w, uint32_t cta, bool work, uint32_t& bad) {
+  Split s{};
+  s.last = cta;
+  if (work) {
+    const uint32_t begun = w.unit;  // blocks of the first item that lie in earlier CTAs
+    bool head_of_item = begun == 0;
+    uint64_t left = w.left;
+    while (left > w.q.blocks - w.unit) {
+      left -= w.q.blocks - w.unit;
+      w.left = left;
+      w.advance(p, bad);
+      head_of_item = true;
+    }
+    uint64_t rest = w.q.blocks - w.unit - left;  // the item's blocks in later CTAs
+    if (head_of_item && rest != 0) {
+      s.start = w.q.start, s.nodes = w.q.nodes, s.head = w.head, s.tile = w.tile;
+      s.last = cta_of_unit(w.past + rest - 1, w.units, w.ctas);
+    }
+  }
+  p.splits[cta] = s;
+}
+
+// A partial result: sums [dim_pad / 4][rows][4] (neighbouring rows' 16 bytes adjacent, as a thread a
+// row stores them) and statistics [rows] {maximum, sum of weights}.  Of a CTA's two, slot 1 is that
+// of an item that begins in it, 0 that of one that began before.
+__device__ __forceinline__ float* part_sums(const AttnParams& p, uint32_t cta, uint32_t slot) {
+  return p.parts + (static_cast<uint64_t>(cta) * 2 + slot) * p.rows * (p.dim_pad + 2);
+}
+__device__ __forceinline__ float2* part_stats(const AttnParams& p, uint32_t cta, uint32_t slot) {
+  return reinterpret_cast<float2*>(part_sums(p, cta, slot) + p.rows * p.dim_pad);
 }
 
 // Address of one cached key's row in k or v (elements from the base), its page checked.

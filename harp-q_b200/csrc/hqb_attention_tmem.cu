@@ -15,16 +15,25 @@ constexpr uint32_t kRows = 128;      // tensor-memory lanes: rows of one score t
 constexpr uint32_t kCopyWarp = 9;  // plain copies and the values' last rows; warp 8: tensor-map copies
 constexpr uint32_t kMmaWarp = 10;
 constexpr uint32_t kTmemThreads = 384;  // warps 0-7 softmax, 8-10 as above, 11 idle
-// Registers: 384 threads start with 168 each; the softmax warpgroups take 208, the rest keep 80
-// (2 * 128 * 208 + 128 * 80 = 63488 of the launch's 64512).
-constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80;
+// Pairs of weights, of every 8, that go by the polynomial: the special-function unit alone would
+// take 1024 cycles a block and warp, as long as half of both streams' MMAs.
+constexpr int kPolyPairs = 3;
 constexpr float kSlack = 8.0f;       // log2 of how far the maximum may grow before sums are rescaled
+
+// One segment as the MMA and softmax warps see it, written by the loading warp.
+struct Segment {
+  Request q;
+  uint32_t head, row0, b0, n;  // n 0: there are no more
+  uint32_t two;                // the tile has rows for both score tiles
+  uint32_t pad;
+};
 
 struct Bars {
   uint64_t kv_full[8], kv_empty[8], fix_full[8];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], o_free, joint, drain;
+  uint64_t q_full[2], q_empty, s_full[2], p_full[2], o_full[2], o_free, joint, drain;
   uint32_t tmem, abort;
   uint32_t broken[8][8];  // by segment: drafted nodes with an infinity or NaN among their values
+  Segment segments[4];
 };
 
 template <int DP>
@@ -78,6 +87,10 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
     if (tid == 0) atomicOr(p.error, HQB_DEVERR_LAUNCH);
     return;
   }
+  if (warp == kMmaWarp && lane < 5) {
+    const CUtensorMap* all[5] = {&maps.q, &maps.k, &maps.v, &maps.ck, &maps.cv};
+    if (lane < 3 || maps.box_rows != 0) prefetch_map(all[lane]);
+  }
   if (tid < 64) bars.broken[tid >> 3][tid & 7] = 0;
   if (tid == 0) {
     for (uint32_t i = 0; i < S::kSlots; ++i) {
@@ -85,9 +98,9 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
       mbar_init(&bars.kv_empty[i], 1);
       mbar_init(&bars.fix_full[i], 1);
     }
-    mbar_init(&bars.q_full, 1);
     mbar_init(&bars.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 128);
       mbar_init(&bars.o_full[i], 1);
@@ -108,293 +121,313 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   const uint32_t tmem = bars.tmem;
   griddep_wait();
   // a wait that runs out ends every role's loop; nothing is left in flight but this CTA's copies
-  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (*abort) return false;
-    if (mbar_wait(bar, parity & 1u, p.error)) return true;
-    *abort = 1u;
-    return false;
+  // (for a whole warp, whose lanes must go on or stop together)
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity & 1u))) return true;
+    const bool stop = *abort != 0;
+    const bool got = !stop && mbar_wait(bar, parity & 1u, p.error);
+    if (!stop && !got) *abort = 1u;
+    return __all_sync(0xffffffffu, got);
   };
-  // the same for a whole warp, whose lanes must go on or stop together
-  auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
-  Walk w;
-  const bool work = w.begin(p, blockIdx.x, bad);
   const uint32_t half = p.rows / 2;  // rows of a tile's first score tile
+  // Segment seg is announced by phase seg / 2 of q_full[seg & 1].  No warp can be two phases of one
+  // barrier late: segment seg + 2 is announced after q_empty of segment seg + 1, which is committed
+  // after o_free of segment seg, to which every softmax warp arrives at its end.  For the same
+  // reason segments[seg & 3] stays while it is read.
+  auto segment = [&](uint32_t seg) -> const Segment* {
+    if (!wait_all(&bars.q_full[seg & 1], seg >> 1)) return nullptr;
+    const Segment* s = &bars.segments[seg & 3];
+    return *const_cast<const volatile uint32_t*>(&s->n) == 0 ? nullptr : s;
+  };
   if (warp >= 8) {
-    shrink_registers<kOtherRegs>();
-    if (work && warp < kMmaWarp) {
-      // ---- both walk the slots in the order in which the MMAs take them.  One of them fills all
-      // slots (a slot's turns can only be told apart by the warp that waits for each of them): the
-      // loading warp, or without maps of the cache the copying warp.  The copying warp hands on
-      // the values whose last rows have to be cleared.  Each slot is announced once on kv_full.
-      const bool copier = warp == kCopyWarp, filler = copier == (maps.box_rows == 0);
-      constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
-      const uint32_t dim = p.c.head_dim;
-      uint32_t issued = 0, seg = 0, fixes = 0;
-      uint32_t sent_fix = 0, sent_turn = 0;  // filler, a bit a slot: its last copy goes to fix_full, that one's phase
-      bool ok = true;
-      while (ok && w.left != 0) {
-        w.open(p);
-        const Request q = w.q;
-        const uint32_t rows = q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
-        const bool two = rows - row0 > half;
-        const int32_t* table = p.a.tables + static_cast<uint64_t>(w.r) * p.a.table_stride;
-        uint32_t* broken = bars.broken[seg & 7];
-        auto load = [&](uint32_t b, bool values) {
-          const uint32_t slot = issued % S::kSlots, turn = issued / S::kSlots - 1;
-          const bool reuse = issued >= S::kSlots;
-          ++issued;
-          if (!ok) return;
-          const bool cached = b < q.cached_blocks;
-          const uint32_t first = (cached ? b : b - q.cached_blocks) * kKeys;
-          const uint32_t valid = min(kKeys, (cached ? q.ctx : q.nodes) - first);
-          const bool fix = values && (!cached || valid < kKeys);  // rows to clear
-          uint8_t* const at = sm + S::kRing + slot * S::kTile;
-          const uint32_t dst = smem_u32(at);
-          if (filler && reuse) ok = wait_all(&bars.kv_empty[slot], turn);
-          if (!ok) return;
-          if (cached && maps.box_rows == 0) {
-            if (!filler) return;
-            const T* src = static_cast<const T*>(values ? p.c.v : p.c.k);
-            for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
-              const uint64_t where = r0 + lane < valid ? key_offset(p, table, first + r0 + lane, w.head, bad) : 0;
+    if (warp != kMmaWarp) {
+      Walk w;
+      const bool work = w.begin(p, blockIdx.x, bad);
+      if (tid == 11 * 32 && !p.whole) note_split(p, w, blockIdx.x, work, bad);  // the otherwise idle warp
+      if (!work) w.left = 0;
+      if (warp < kMmaWarp) {
+        // ---- both walk the slots in the order in which the MMAs take them.  One of them fills all
+        // slots (a slot's turns can only be told apart by the warp that waits for each of them): the
+        // loading warp, or without maps of the cache the copying warp.  The copying warp hands on
+        // the values whose last rows have to be cleared.  Each slot is announced once on kv_full.
+        const bool copier = warp == kCopyWarp, filler = copier == (maps.box_rows == 0);
+        constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
+        const uint32_t dim = p.c.head_dim;
+        uint32_t issued = 0, seg = 0, fixes = 0;
+        uint32_t sent_fix = 0, sent_turn = 0;  // filler, a bit a slot: its last copy goes to fix_full, that one's phase
+        bool ok = true;
+        while (ok && w.left != 0) {
+          w.open(p);
+          const Request q = w.q;
+          const uint32_t rows = q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
+          const bool two = rows - row0 > half;
+          const int32_t* table = p.a.tables + static_cast<uint64_t>(w.r) * p.a.table_stride;
+          uint32_t* broken = bars.broken[seg & 7];
+          auto load = [&](uint32_t b, bool values) {
+            const uint32_t slot = issued % S::kSlots, turn = issued / S::kSlots - 1;
+            const bool reuse = issued >= S::kSlots;
+            ++issued;
+            if (!ok) return;
+            const bool cached = b < q.cached_blocks;
+            const uint32_t first = (cached ? b : b - q.cached_blocks) * kKeys;
+            const uint32_t valid = min(kKeys, (cached ? q.ctx : q.nodes) - first);
+            const bool fix = values && (!cached || valid < kKeys);  // rows to clear
+            uint8_t* const at = sm + S::kRing + slot * S::kTile;
+            const uint32_t dst = smem_u32(at);
+            if (filler && reuse) ok = wait_all(&bars.kv_empty[slot], turn);
+            if (!ok) return;
+            if (cached && maps.box_rows == 0) {
+              if (!filler) return;
+              const T* src = static_cast<const T*>(values ? p.c.v : p.c.k);
+              for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
+                const uint64_t where = r0 + lane < valid ? key_offset(p, table, first + r0 + lane, w.head, bad) : 0;
 #pragma unroll 4
-              for (uint32_t x = 0; x < kPieces; ++x) {
-                const uint32_t i = x * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
-                const uint64_t row = __shfl_sync(0xffffffffu, where, j);
-                const bool copy = r < valid && c * 8 < dim;
-                cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
-                           copy ? 16u : 0u);
+                for (uint32_t x = 0; x < kPieces; ++x) {
+                  const uint32_t i = x * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
+                  const uint64_t row = __shfl_sync(0xffffffffu, where, j);
+                  const bool copy = r < valid && c * 8 < dim;
+                  cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
+                             copy ? 16u : 0u);
+                }
+              }
+              cp_async_commit();
+              cp_async_wait<0>();
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
+              return;
+            }
+            if (filler) {
+              uint64_t* bar = fix ? &bars.fix_full[slot] : &bars.kv_full[slot];
+              sent_fix = fix ? sent_fix | 1u << slot : sent_fix & ~(1u << slot);
+              if (fix) sent_turn ^= 1u << slot;
+              if (cached) {
+                // a lane a box; boxes past the end of the context are left out (scores of what lies there
+                // are hidden, values are cleared)
+                const uint32_t boxes = kKeys / maps.box_rows, real = (valid + maps.box_rows - 1) / maps.box_rows;
+                const uint32_t box = lane % boxes, h = lane / boxes;
+                if (lane == 0) mbar_expect_tx(bar, real * maps.box_rows * DP * 2);
+                __syncwarp();
+                if (h < DP / 64 && box < real) {
+                  const uint32_t key = first + box * maps.box_rows, column = key / p.c.page_size;
+                  uint32_t page = static_cast<uint32_t>(__ldg(table + column));
+                  if (page >= p.c.num_pages) {
+                    bad |= HQB_DEVERR_PAGES;
+                    page = 0;
+                  }
+                  tma_load_4d(dst + h * S::kHalf + box * maps.box_rows * 128, values ? &maps.cv : &maps.ck, bar, h * 64, w.head,
+                              key - column * p.c.page_size, page);
+                }
+              } else {
+                if (lane == 0) mbar_expect_tx(bar, S::kTile);
+                __syncwarp();
+                if (lane < DP / 64)
+                  tma_load_3d(dst + lane * S::kHalf, values ? &maps.v : &maps.k, bar, lane * 64, w.head, q.start + first);
               }
             }
-            cp_async_commit();
-            cp_async_wait<0>();
+            if (!copier || !fix) return;
+            ok = wait_all(&bars.fix_full[slot], fixes >> slot);
+            if (!ok) return;
+            fixes ^= 1u << slot;
+            // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
+            // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
+            // node get at the end
+            auto piece = [&](uint32_t i) {
+              const uint32_t r = i / kPieces, c = i % kPieces;
+              return reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            };
+            // (the sums' MMAs stop after the 16 keys that hold the last one)
+            for (uint32_t i = valid * kPieces + lane; i < ((valid + 15) & ~15u) * kPieces; i += 32) *piece(i) = make_uint4(0, 0, 0, 0);
+            for (uint32_t i0 = lane; !cached && i0 < valid * kPieces; i0 += 32 * 8) {
+              uint4 v[8];
+#pragma unroll
+              for (uint32_t k = 0; k < 8; ++k)
+                v[k] = i0 + k * 32 < valid * kPieces ? *piece(i0 + k * 32) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (uint32_t k = 0; k < 8; ++k) {
+                constexpr uint32_t kMask = Elem<T>::kExpMask;
+                uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                bool found = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if ((u[e] & kMask) == kMask) u[e] &= 0xFFFF0000u, found = true;
+                  if ((u[e] >> 16 & kMask) == kMask) u[e] &= 0x0000FFFFu, found = true;
+                }
+                if (found) {
+                  const uint32_t node = first + (i0 + k * 32) / kPieces;
+                  atomicOr(&broken[node >> 5], 1u << (node & 31));
+                  *piece(i0 + k * 32) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+              }
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
-            return;
-          }
-          if (filler) {
-            uint64_t* bar = fix ? &bars.fix_full[slot] : &bars.kv_full[slot];
-            sent_fix = fix ? sent_fix | 1u << slot : sent_fix & ~(1u << slot);
-            if (fix) sent_turn ^= 1u << slot;
-            if (cached) {
-              // a lane a box; boxes past the end of the context are left out (scores of what lies there
-              // are hidden, values are cleared)
-              const uint32_t boxes = kKeys / maps.box_rows, real = (valid + maps.box_rows - 1) / maps.box_rows;
-              const uint32_t box = lane % boxes, h = lane / boxes;
-              if (lane == 0) mbar_expect_tx(bar, real * maps.box_rows * DP * 2);
-              __syncwarp();
-              if (h < DP / 64 && box < real) {
-                const uint32_t key = first + box * maps.box_rows, column = key / p.c.page_size;
-                uint32_t page = static_cast<uint32_t>(__ldg(table + column));
-                if (page >= p.c.num_pages) {
-                  bad |= HQB_DEVERR_PAGES;
-                  page = 0;
-                }
-                tma_load_4d(dst + h * S::kHalf + box * maps.box_rows * 128, values ? &maps.cv : &maps.ck, bar, h * 64, w.head,
-                            key - column * p.c.page_size, page);
-              }
-            } else {
-              if (lane == 0) mbar_expect_tx(bar, S::kTile);
-              __syncwarp();
-              if (lane < DP / 64)
-                tma_load_3d(dst + lane * S::kHalf, values ? &maps.v : &maps.k, bar, lane * 64, w.head, q.start + first);
+          };
+          // K0 V0 K1 V1 ... for two score tiles over the same keys, K0 K1 V0 K2 V1 ... Vn-2 Vn-1 for two
+          // streams of blocks.  The queries go after the first keys, once the last segment's have been
+          // read.  Only the loading warp may wait for q_empty: a warp that the MMAs do not wait for in
+          // every segment could find it two phases on.  (One call of load: instructions are fetched from
+          // as far as L2, so the loops here are kept short.)
+          for (uint32_t x = 0; ok && x < 2 * n; ++x) {
+            const bool last = x == 2 * n - 1;
+            const bool values = two ? (x & 1) != 0 : last || (x != 0 && (x & 1) == 0);
+            const uint32_t i = two ? x / 2 : last ? n - 1 : values ? x / 2 - 1 : (x + 1) / 2;
+            load(w.b0 + i, values);
+            if (x != 0 || copier) continue;
+            if (seg > 0) ok = ok && wait_all(&bars.q_empty, seg - 1);
+            if (!ok) break;
+            uint64_t* q_full = &bars.q_full[seg & 1];
+            // past here the epilogue of segment seg - 3 is over: the flags of segment seg - 4 are free
+            if (lane < 8) bars.broken[(seg + 4) & 7][lane] = 0;
+            const uint32_t tiles = two ? 2u : 1u;
+            if (lane == 0) {
+              bars.segments[seg & 3] = Segment{q, w.head, row0, w.b0, n, two ? 1u : 0u, 0u};
+              mbar_expect_tx(q_full, tiles * half * DP * 2);
+            }
+            __syncwarp();
+            if (lane < tiles * (DP / 64)) {
+              const uint32_t t = lane / (DP / 64), h = lane % (DP / 64);
+              tma_load_3d(smem_u32(sm + t * S::kTile + h * S::kHalf), &maps.q, q_full, h * 64, w.head * p.group,
+                          q.start + (row0 + t * half) / p.group);
             }
           }
-          if (!copier || !fix) return;
-          ok = wait_all(&bars.fix_full[slot], fixes >> slot);
-          if (!ok) return;
-          fixes ^= 1u << slot;
-          // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
-          // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
-          // node get at the end
-          for (uint32_t i = lane; i < kKeys * kPieces; i += 32) {
-            const uint32_t r = i / kPieces, c = i % kPieces;
-            uint4* e = reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-            if (r >= valid) {
-              *e = make_uint4(0, 0, 0, 0);
-            } else if (!cached) {
-              constexpr uint32_t kMask = Elem<T>::kExpMask;
-              const uint4 v = *e;
-              uint32_t u[4] = {v.x, v.y, v.z, v.w};
-              bool found = false;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if ((u[k] & kMask) == kMask) u[k] &= 0xFFFF0000u, found = true;
-                if ((u[k] >> 16 & kMask) == kMask) u[k] &= 0x0000FFFFu, found = true;
-              }
-              if (found) {
-                atomicOr(&broken[(first + r) >> 5], 1u << (r & 31));
-                *e = make_uint4(u[0], u[1], u[2], u[3]);
-              }
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
-        };
-        // the first keys, then the queries (the last segment's must have been read), then the rest.  Only
-        // the loading warp may wait for q_empty: a warp that the MMAs do not wait for in every segment
-        // could find it two phases on.
-        load(w.b0, false);
-        if (!copier) {
-          if (seg > 0) ok = ok && wait_all(&bars.q_empty, seg - 1);
-          if (!ok) break;
-          // past here the epilogue of segment seg - 3 is over: the flags of segment seg - 4 are free
-          if (lane < 8) bars.broken[(seg + 4) & 7][lane] = 0;
-          const uint32_t tiles = two ? 2u : 1u;
-          if (lane == 0) mbar_expect_tx(&bars.q_full, tiles * half * DP * 2);
-          __syncwarp();
-          if (lane < tiles * (DP / 64)) {
-            const uint32_t t = lane / (DP / 64), h = lane % (DP / 64);
-            tma_load_3d(smem_u32(sm + t * S::kTile + h * S::kHalf), &maps.q, &bars.q_full, h * 64, w.head * p.group,
-                        q.start + (row0 + t * half) / p.group);
-          }
-        }
-        if (two) {
-          for (uint32_t i = 0; ok && i < n; ++i) {
-            if (i > 0) load(w.b0 + i, false);
-            load(w.b0 + i, true);
-          }
-        } else {
-          if (n > 1) load(w.b0 + 1, false);
-          for (uint32_t i = 0; ok && i < n; ++i) {
-            load(w.b0 + i, true);
-            if (i + 2 < n) load(w.b0 + i + 2, false);
-          }
-        }
-        ++seg;
-        w.advance(p, bad);
-      }
-      if (!ok && filler && maps.box_rows != 0) {  // copies in flight end before the CTA does
-        for (uint32_t i = issued > S::kSlots ? issued - S::kSlots : 0; i < issued; ++i) {
-          const uint32_t slot = i % S::kSlots;
-          if (sent_fix >> slot & 1u) mbar_wait(&bars.fix_full[slot], (sent_turn >> slot & 1u) ^ 1u, p.error);
-          else mbar_wait(&bars.kv_full[slot], i / S::kSlots & 1u, p.error);
-        }
-      }
-      if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
-    } else if (work && warp == kMmaWarp) {
-      // ---- MMA issuer
-      if (lane == 0) {
-        constexpr uint32_t kType = sizeof(T) == 2 && Elem<T>::kExpMask == 0x7F80u ? 1u : 0u;  // BF16 : FP16
-        constexpr uint32_t kBase = (1u << 4) | (kType << 7) | (kType << 10) | ((kRows >> 4) << 24);
-        constexpr uint32_t kScores = kBase | ((kKeys >> 3) << 17);
-        constexpr uint32_t kSums = kBase | (1u << 16) | ((DP >> 3) << 17);  // B (values) MN-major
-        uint32_t slot_at = 0, seg = 0, p_at[2] = {0, 0};
-        bool ok = true;
-        auto slot_wait = [&](uint32_t n) { return wait(&bars.kv_full[n % S::kSlots], n / S::kSlots); };
-        auto slot_addr = [&](uint32_t n) { return smem_u32(sm + S::kRing + (n % S::kSlots) * S::kTile); };
-        // descriptors step by their address field (16-byte units)
-        auto scores = [&](uint32_t s, uint32_t tile, uint32_t slot) {
-          const uint64_t qd = umma_desc_sw128(smem_u32(sm + tile * S::kTile), 16), kd = umma_desc_sw128(slot_addr(slot), 16);
-#pragma unroll
-          for (uint32_t k = 0; k < DP / 16; ++k) {
-            const uint32_t step = (k >> 2) * (S::kHalf >> 4) + (k & 3) * 2;
-            tc_mma_f16_ss(tmem + s * 128, qd + step, kd + step, kScores, k > 0 ? 1u : 0u);
-          }
-          tc_commit(&bars.s_full[s]);
-        };
-        auto sums = [&](uint32_t s, uint32_t slot, bool first) {
-          const uint64_t vd = umma_desc_sw128(slot_addr(slot), S::kHalf);
-#pragma unroll
-          for (uint32_t k = 0; k < kKeys / 16; ++k)
-            tc_mma_f16_ts(tmem + 256 + s * DP, tmem + s * 128 + k * 8, vd + k * 128, kSums, k > 0 || !first ? 1u : 0u);
-        };
-        auto weights_wait = [&](uint32_t s) {
-          const bool r = wait(&bars.p_full[s], p_at[s]);
-          ++p_at[s];
-          tc_fence_after();
-          return r;
-        };
-        while (ok && w.left != 0) {
-          w.open(p);
-          const uint32_t n = w.b1 - w.b0;
-          const bool two = w.q.nodes * p.group - w.tile * p.rows > half;
-          ok = wait(&bars.q_full, seg);
-          if (!ok) break;
-          if (two) {
-            // slots: K0 V0 K1 V1 ...
-            if (!(ok = slot_wait(slot_at))) break;
-            tc_fence_after();
-            scores(0, 0, slot_at);
-            scores(1, 1, slot_at);
-            tc_commit(&bars.kv_empty[slot_at % S::kSlots]);
-            if (n == 1) tc_commit(&bars.q_empty);
-            if (seg > 0 && !(ok = wait(&bars.o_free, seg - 1))) break;
-            for (uint32_t i = 0; i < n; ++i) {
-              const uint32_t v = slot_at + 2 * i + 1, k = v + 1;
-              const bool more = i + 1 < n;
-              ok = slot_wait(v) && weights_wait(0);
-              if (!ok) break;
-              sums(0, v, i == 0);
-              if (more) {
-                if (!(ok = slot_wait(k))) break;
-                tc_fence_after();
-                scores(0, 0, k);
-              } else {
-                tc_commit(&bars.o_full[0]);
-              }
-              if (!(ok = weights_wait(1))) break;
-              sums(1, v, i == 0);
-              tc_commit(&bars.kv_empty[v % S::kSlots]);
-              if (more) {
-                scores(1, 1, k);
-                tc_commit(&bars.kv_empty[k % S::kSlots]);
-                if (i + 2 == n) tc_commit(&bars.q_empty);
-              } else {
-                tc_commit(&bars.o_full[1]);
-              }
-            }
-          } else {
-            // slots: K0 K1 V0 K2 V1 K3 ...
-            if (!(ok = slot_wait(slot_at))) break;
-            tc_fence_after();
-            scores(0, 0, slot_at);
-            tc_commit(&bars.kv_empty[slot_at % S::kSlots]);
-            uint32_t next = slot_at + 1;
-            if (n > 1) {
-              if (!(ok = slot_wait(next))) break;
-              tc_fence_after();
-              scores(1, 0, next);
-              tc_commit(&bars.kv_empty[next % S::kSlots]);
-              ++next;
-            }
-            if (n <= 2) tc_commit(&bars.q_empty);
-            if (seg > 0 && !(ok = wait(&bars.o_free, seg - 1))) break;
-            for (uint32_t j = 0; j < n; ++j) {
-              const uint32_t s = j & 1, v = next++;
-              ok = slot_wait(v) && weights_wait(s);
-              if (!ok) break;
-              sums(s, v, j < 2);
-              tc_commit(&bars.kv_empty[v % S::kSlots]);
-              if (j + 2 < n) {
-                const uint32_t k = next++;
-                if (!(ok = slot_wait(k))) break;
-                tc_fence_after();
-                scores(s, 0, k);
-                tc_commit(&bars.kv_empty[k % S::kSlots]);
-                if (j + 3 == n) tc_commit(&bars.q_empty);
-              }
-            }
-            if (ok) {
-              tc_commit(&bars.o_full[0]);
-              tc_commit(&bars.o_full[1]);
-            }
-          }
-          slot_at += 2 * n;
           ++seg;
           w.advance(p, bad);
         }
-        if (!ok) {  // MMAs that were issued end before the tensor memory is freed
-          tc_commit(&bars.drain);
-          mbar_wait(&bars.drain, 0, p.error);
+        if (ok && !copier) {  // the end: with the last queries read, so that no announcement is overtaken
+          if (seg > 0) ok = wait_all(&bars.q_empty, seg - 1);
+          if (ok && lane == 0) {
+            bars.segments[seg & 3].n = 0;
+            mbar_arrive(&bars.q_full[seg & 1]);
+          }
         }
+        if (!ok && filler && maps.box_rows != 0) {  // copies in flight end before the CTA does
+          for (uint32_t i = issued > S::kSlots ? issued - S::kSlots : 0; i < issued; ++i) {
+            const uint32_t slot = i % S::kSlots;
+            if (sent_fix >> slot & 1u) mbar_wait(&bars.fix_full[slot], (sent_turn >> slot & 1u) ^ 1u, p.error);
+            else mbar_wait(&bars.kv_full[slot], i / S::kSlots & 1u, p.error);
+          }
+        }
+        if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
+      }
+    } else {
+      // ---- MMA issuer: the whole warp keeps the schedule, one elected lane issues
+      constexpr uint32_t kType = sizeof(T) == 2 && Elem<T>::kExpMask == 0x7F80u ? 1u : 0u;  // BF16 : FP16
+      constexpr uint32_t kBase = (1u << 4) | (kType << 7) | (kType << 10) | ((kRows >> 4) << 24);
+      constexpr uint32_t kScores = kBase | ((kKeys >> 3) << 17);
+      constexpr uint32_t kSums = kBase | (1u << 16) | ((DP >> 3) << 17);  // B (values) MN-major
+      uint32_t slot_at = 0, seg = 0, p_at[2] = {0, 0};
+      bool ok = true;
+      auto slot_wait = [&](uint32_t n) { return wait_all(&bars.kv_full[n % S::kSlots], n / S::kSlots); };
+      auto slot_addr = [&](uint32_t n) { return smem_u32(sm + S::kRing + (n % S::kSlots) * S::kTile); };
+      // descriptors step by their address field (16-byte units)
+      auto scores = [&](uint32_t s, uint32_t tile, uint32_t slot) {
+        const uint64_t qd = umma_desc_sw128(smem_u32(sm + tile * S::kTile), 16), kd = umma_desc_sw128(slot_addr(slot), 16);
+#pragma unroll 1
+        for (uint32_t k = 0; k < DP / 16; ++k) {
+          const uint32_t step = (k >> 2) * (S::kHalf >> 4) + (k & 3) * 2;
+          warp_mma_f16_ss(tmem + s * 128, qd + step, kd + step, kScores, k > 0 ? 1u : 0u);
+        }
+        warp_commit(&bars.s_full[s]);
+      };
+      auto sums = [&](const Segment* g, uint32_t s, uint32_t i, uint32_t slot, bool first) {
+        const uint64_t vd = umma_desc_sw128(slot_addr(slot), S::kHalf);
+        const uint32_t b = g->b0 + i;
+        const bool cached = b < g->q.cached_blocks;
+        const uint32_t left = (cached ? g->q.ctx : g->q.nodes) - (cached ? b : b - g->q.cached_blocks) * kKeys;
+        const uint32_t steps = left >= kKeys ? kKeys / 16 : (left + 15) / 16;
+#pragma unroll 1
+        for (uint32_t k = 0; k < steps; ++k)
+          warp_mma_f16_ts(tmem + 256 + s * DP, tmem + s * 128 + k * 8, vd + k * 128, kSums, k > 0 || !first ? 1u : 0u);
+      };
+      auto weights_wait = [&](uint32_t s) {
+        const bool r = wait_all(&bars.p_full[s], p_at[s]);
+        ++p_at[s];
+        tc_fence_after();
+        return r;
+      };
+      for (const Segment* g; ok && (g = segment(seg)) != nullptr;) {
+        const uint32_t n = g->n;
+        if (g->two) {
+          // slots: K0 V0 K1 V1 ...
+          if (!(ok = slot_wait(slot_at))) break;
+          tc_fence_after();
+          scores(0, 0, slot_at);
+          scores(1, 1, slot_at);
+          warp_commit(&bars.kv_empty[slot_at % S::kSlots]);
+          if (seg > 0 && !(ok = wait_all(&bars.o_free, seg - 1))) break;
+          if (n == 1) warp_commit(&bars.q_empty);
+          for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t v = slot_at + 2 * i + 1, k = v + 1;
+            const bool more = i + 1 < n;
+            ok = slot_wait(v) && weights_wait(0);
+            if (!ok) break;
+            sums(g, 0, i, v, i == 0);
+            if (more) {
+              if (!(ok = slot_wait(k))) break;
+              tc_fence_after();
+              scores(0, 0, k);
+            } else {
+              warp_commit(&bars.o_full[0]);
+            }
+            if (!(ok = weights_wait(1))) break;
+            sums(g, 1, i, v, i == 0);
+            warp_commit(&bars.kv_empty[v % S::kSlots]);
+            if (more) {
+              scores(1, 1, k);
+              warp_commit(&bars.kv_empty[k % S::kSlots]);
+              if (i + 2 == n) warp_commit(&bars.q_empty);
+            } else {
+              warp_commit(&bars.o_full[1]);
+            }
+          }
+        } else {
+          // slots: K0 K1 V0 K2 V1 K3 ...
+          if (!(ok = slot_wait(slot_at))) break;
+          tc_fence_after();
+          scores(0, 0, slot_at);
+          warp_commit(&bars.kv_empty[slot_at % S::kSlots]);
+          uint32_t next = slot_at + 1;
+          if (n > 1) {
+            if (!(ok = slot_wait(next))) break;
+            tc_fence_after();
+            scores(1, 0, next);
+            warp_commit(&bars.kv_empty[next % S::kSlots]);
+            ++next;
+          }
+          if (seg > 0 && !(ok = wait_all(&bars.o_free, seg - 1))) break;
+          if (n <= 2) warp_commit(&bars.q_empty);
+          for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t s = j & 1, v = next++;
+            ok = slot_wait(v) && weights_wait(s);
+            if (!ok) break;
+            sums(g, s, j, v, j < 2);
+            warp_commit(&bars.kv_empty[v % S::kSlots]);
+            if (j + 2 < n) {
+              const uint32_t k = next++;
+              if (!(ok = slot_wait(k))) break;
+              tc_fence_after();
+              scores(s, 0, k);
+              warp_commit(&bars.kv_empty[k % S::kSlots]);
+              if (j + 3 == n) warp_commit(&bars.q_empty);
+            }
+          }
+          if (ok) {
+            warp_commit(&bars.o_full[0]);
+            warp_commit(&bars.o_full[1]);
+          }
+        }
+        slot_at += 2 * n;
+        ++seg;
+      }
+      if (!ok) {  // MMAs that were issued end before the tensor memory is freed
+        warp_commit(&bars.drain);
+        mbar_wait(&bars.drain, 0, p.error);
       }
     }
   } else {
-    grow_registers<kSoftmaxRegs>();
-    if (work) {
+    {
       // ---- softmax: stream s, row = tensor-memory lane
       const uint32_t s = warp >> 2, lrow = (warp & 3) * 32 + lane;
       const uint32_t lanes = ((warp & 3) * 32u) << 16;
@@ -403,18 +436,17 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
       const uint32_t dim = p.c.head_dim;
       uint32_t s_at = 0, seg = 0, joints = 0;
       bool ok = true;
-      while (ok && w.left != 0) {
-        w.open(p);
-        const Request q = w.q;
-        const uint32_t rows = q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
-        const bool two = rows - row0 > half;
+      for (const Segment* g; ok && (g = segment(seg)) != nullptr;) {
+        const Request q = g->q;
+        const uint32_t rows = q.nodes * p.group, row0 = g->row0, n = g->n, b0 = g->b0;
+        const bool two = g->two != 0;
         const uint32_t row = row0 + (two ? s * half : 0u) + lrow;
         const bool live = lrow < half && row < rows;
         const uint32_t node = live ? row / p.group : 0u;
         const uint32_t mine = two ? n : (n + 1 - s) / 2;
         float m = -INFINITY, l = 0.0f;
         for (uint32_t i = 0; i < mine; ++i) {
-          const uint32_t b = w.b0 + (two ? i : 2 * i + s);
+          const uint32_t b = b0 + (two ? i : 2 * i + s);
           // which of the block's keys the row sees
           uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
           bool all = true;
@@ -436,19 +468,28 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           if (!(ok = wait_all(&bars.s_full[s], s_at))) break;
           ++s_at;
           tc_fence_after();
-          uint32_t v[128];
-          tc_ld_x128(sc, v);
-          if (!all) {
+          // two passes over the scores, 32 at a time, in loops that stay short: unrolled over all 128 the
+          // softmax waits for instructions
+          float top = -INFINITY;
+#pragma unroll 1
+          for (uint32_t x = 0; x < 4; ++x) {
+            uint32_t v[32];
+            tc_ld_x32(sc + x * 32, v);
+            const uint32_t seen = x < 2 ? (x == 0 ? sees[0] : sees[1]) : (x == 2 ? sees[2] : sees[3]);
+            if (!all) {  // the same for the whole warp, as the store back needs
 #pragma unroll
-            for (int e = 0; e < 128; ++e) v[e] = (sees[e >> 5] >> (e & 31) & 1u) ? v[e] : 0xFF800000u;
+              for (int e = 0; e < 32; ++e) v[e] = (seen >> e & 1u) ? v[e] : 0xFF800000u;
+              tc_st_x32(sc + x * 32, v);
+            }
+            float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                t4[k] = fmaxf(t4[k], fmaxf(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])));
+            top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
           }
-          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int e = 0; e < 128; e += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              t4[k] = fmaxf(t4[k], fmaxf(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])));
-          const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+          if (!all) tc_wait_st();
           const float tops = top * c;
           const bool grow = tops > m + kSlack || (m == -INFINITY && tops > m);
           if (ballot(grow) != 0) {
@@ -457,29 +498,31 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             l *= f;
             m = next;
             if (i > 0) {  // the sums of the blocks before this one are complete: their MMAs precede this score's
+#pragma unroll 1
+              for (uint32_t x = 0; x < DP / 16; ++x) {  // few at a time: the scores stay in registers
+                uint32_t o[16];
+                tc_ld_x16(oc + x * 16, o);
 #pragma unroll
-              for (uint32_t x = 0; x < DP / 32; ++x) {
-                uint32_t o[32];
-                tc_ld_x32(oc + x * 32, o);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tc_st_x32(oc + x * 32, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc_st_x16(oc + x * 16, o);
               }
             }
           }
           const float use = m == -INFINITY ? 0.0f : m;
           const uint64_t c2 = pack2(c, c), u2 = pack2(-use, -use);
           uint64_t sum2 = pack2(0.0f, 0.0f);
-#pragma unroll
+#pragma unroll 1
           for (uint32_t x = 0; x < 4; ++x) {
-            uint32_t w16[16];
+            uint32_t v[32], w16[16];
+            tc_ld_x32(sc + x * 32, v);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float2 t = unpack2(
-                  fma2(pack2(__uint_as_float(v[x * 32 + 2 * e]), __uint_as_float(v[x * 32 + 2 * e + 1])), c2, u2));
-              const float a = fast_exp2(t.x), d = fast_exp2(t.y);
-              sum2 = add2(sum2, pack2(a, d));
-              w16[e] = Elem<T>::pack(a, d);
+              const float2 t = unpack2(fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, u2));
+              float2 y;
+              if (e % 8 < kPolyPairs) y = poly_exp2(t);
+              else y = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+              sum2 = add2(sum2, pack2(y.x, y.y));
+              w16[e] = Elem<T>::pack(y.x, y.y);
             }
             tc_st_x16(sc + x * 16, w16);
           }
@@ -510,16 +553,17 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           x0 = s * (DP / 64);  // each warpgroup writes half of the columns
           x1 = x0 + DP / 64;
         }
-        const bool complete = w.complete();
-        const uint32_t h = w.head * p.group + row - node * p.group;
+        const bool complete = b0 == 0 && n == q.blocks;
+        const uint32_t head = g->head, h = head * p.group + row - node * p.group;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T* out = static_cast<T*>(p.a.out) + (q.start + node) * p.a.out_token_stride + h * p.a.out_head_stride;
-        float* keep = part_row(p, blockIdx.x, w.b0 == 0 ? 1u : 0u, row - row0);
+        float* keep = part_sums(p, blockIdx.x, b0 == 0 ? 1u : 0u) + (row - row0) * 4;
         const uint32_t base = tmem + lanes + 256 + (two ? s * DP : 0u);
         const volatile uint32_t* broken = bars.broken[seg & 7];
         uint32_t any = 0;
-        if (w.b1 > q.cached_blocks)
+        if (b0 + n > q.cached_blocks)
           for (uint32_t x = 0; x < (q.nodes + 31) / 32; ++x) any |= broken[x];
+#pragma unroll 1
         for (uint32_t x = x0; x < x1; ++x) {
           uint32_t v[32];
           tc_ld_x32(base + x * 32, v);
@@ -534,9 +578,9 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           if (any != 0 && live) {
             for (uint32_t j = 0; j < q.nodes; ++j) {
               const uint32_t b = q.cached_blocks + j / kKeys;
-              if (b < w.b0 || b >= w.b1 || !(broken[j >> 5] >> (j & 31) & 1u)) continue;
+              if (b < b0 || b >= b0 + n || !(broken[j >> 5] >> (j & 31) & 1u)) continue;
               if (!(node_mask(p, q, node, j >> 5) >> (j & 31) & 1u)) continue;
-              const T* src = static_cast<const T*>(p.a.v) + (q.start + j) * p.a.kv_token_stride + w.head * p.a.kv_head_stride;
+              const T* src = static_cast<const T*>(p.a.v) + (q.start + j) * p.a.kv_token_stride + head * p.a.kv_head_stride;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const float add = x * 32 + e < dim ? Elem<T>::to_float(src[x * 32 + e]) : 0.0f;
@@ -557,12 +601,13 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2*>(keep + x * 32 + e) = make_float2(o[e], o[e + 1]);
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(keep + (x * 8 + e / 4) * p.rows * 4) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
         }
         if (live && (two || s == 0)) {
-          if (!complete) *reinterpret_cast<float2*>(keep + DP) = make_float2(m, l);
+          if (!complete) part_stats(p, blockIdx.x, b0 == 0 ? 1u : 0u)[row - row0] = make_float2(m, l);
           else if (p.a.lse != nullptr)
             p.a.lse[static_cast<uint64_t>(q.start + node) * p.a.q_heads + h] =
                 l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -570,9 +615,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         tc_fence_before();
         mbar_arrive(&bars.o_free);
         ++seg;
-        w.advance(p, bad);
       }
-      if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
     }
   }
   __syncwarp();
