@@ -361,52 +361,79 @@ constexpr uint32_t kJoinThreads = 512;
 
 // One CTA per (CTA of the attention, 32 rows): the partial results of the item that begins there
 // and spans later CTAs, in their order, joined by their maxima.  A thread has 4 columns of a row
-// and reads 8 partial results at once, so the whole is three trips to memory long.
+// and reads up to 8 partial results at once, a warp 32 neighbouring rows; the outputs are turned in
+// shared memory so that they leave in whole rows (2-byte stores of 32 rows at once took four
+// times as long as all the rest).
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ __align__(16) T turned[kJoinRows][HQB_MAX_HEAD_DIM + 8];
   const uint32_t first = blockIdx.x;
   griddep_wait();
   const Split q = p.splits[first];
   if (q.last == first) return;
-  const uint32_t row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, at = q.tile * p.rows + row;
-  if (row >= p.rows || at >= q.nodes * p.group) return;
-  const uint32_t nd = at / p.group, h = q.head * p.group + at - nd * p.group, dim = p.c.head_dim;
-  for (uint32_t d = threadIdx.x / kJoinRows * 4; d < dim; d += kJoinThreads / kJoinRows * 4) {
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t c0 = first; c0 <= q.last; c0 += 8) {
-      float2 s[8];
-      float4 v[8];
+  const uint32_t row0 = blockIdx.y * kJoinRows, lrow = threadIdx.x % kJoinRows, row = row0 + lrow;
+  const uint32_t rows = q.nodes * p.group, dim = p.c.head_dim;
+  if (q.tile * p.rows + row0 >= rows) return;
+  auto place = [&](uint32_t r, uint32_t& token, uint32_t& head) {
+    const uint32_t at = q.tile * p.rows + r, node = at / p.group;
+    token = q.start + node;
+    head = q.head * p.group + at - node * p.group;
+  };
+  if (row < p.rows) {
+    for (uint32_t d = threadIdx.x / kJoinRows * 4; d < dim; d += kJoinThreads / kJoinRows * 4) {
+      float m = -INFINITY, l = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (uint32_t c0 = first; c0 <= q.last; c0 += 8) {
+        float2 s[8];
+        float4 v[8];
 #pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) {
-        const uint32_t c = min(c0 + k, q.last), slot = c == first ? 1u : 0u;
-        s[k] = part_stats(p, c, slot)[row];
-        v[k] = *reinterpret_cast<const float4*>(part_sums(p, c, slot) + ((d >> 2) * p.rows + row) * 4);
+        for (uint32_t k = 0; k < 8; ++k) {
+          s[k] = make_float2(-INFINITY, 0.0f);
+          v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (c0 + k <= q.last) {
+            const uint32_t c = c0 + k, slot = c == first ? 1u : 0u;
+            s[k] = part_stats(p, c, slot)[row];
+            v[k] = *reinterpret_cast<const float4*>(part_sums(p, c, slot) + ((d >> 2) * p.rows + row) * 4);
+          }
+        }
+        float top = m;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
+        const float use = top == -INFINITY ? 0.0f : top, old = fast_exp2(m - use);
+        l *= old;
+        o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+        m = top;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+          if (c0 + k > q.last) break;
+          const float f = fast_exp2(s[k].x - use);
+          l += f * s[k].y;
+          o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+        }
       }
-      float top = m;
-#pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
-      const float use = top == -INFINITY ? 0.0f : top, old = fast_exp2(m - use);
-      l *= old;
-      o.x *= old, o.y *= old, o.z *= old, o.w *= old;
-      m = top;
-#pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) {
-        if (c0 + k > q.last) break;
-        const float f = fast_exp2(s[k].x - use);
-        l += f * s[k].y;
-        o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      uint2 r;
+      r.x = l == 0.0f ? 0u : Elem<T>::pack(o.x * inv, o.y * inv);
+      r.y = l == 0.0f ? 0u : Elem<T>::pack(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(&turned[lrow][d]) = r;
+      if (d == 0 && p.a.lse != nullptr && q.tile * p.rows + row < rows) {
+        uint32_t token, head;
+        place(row, token, head);
+        p.a.lse[static_cast<uint64_t>(token) * p.a.q_heads + head] =
+            l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       }
     }
-    T* out = static_cast<T*>(p.a.out) + (q.start + nd) * p.a.out_token_stride + h * p.a.out_head_stride;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-      if (d + i < dim) out[d + i] = Elem<T>::from_float(l == 0.0f ? 0.0f : e[i]);
-    if (d == 0 && p.a.lse != nullptr)
-      p.a.lse[static_cast<uint64_t>(q.start + nd) * p.a.q_heads + h] =
-          l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  __syncthreads();
+  const uint32_t pieces = p.vec ? dim / 8 : dim;
+  for (uint32_t i = threadIdx.x; i < kJoinRows * pieces; i += kJoinThreads) {
+    const uint32_t r = i / pieces, c = i - r * pieces;
+    if (row0 + r >= p.rows || q.tile * p.rows + row0 + r >= rows) break;
+    uint32_t token, head;
+    place(row0 + r, token, head);
+    T* out = static_cast<T*>(p.a.out) + token * p.a.out_token_stride + head * p.a.out_head_stride;
+    if (p.vec) *reinterpret_cast<uint4*>(out + c * 8) = *reinterpret_cast<const uint4*>(&turned[r][c * 8]);
+    else out[c] = turned[r][c];
   }
 }
 
@@ -559,6 +586,7 @@ HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_arg
   p.min_blocks = 4;
   p.whole = s.whole;
   p.grid = s.grid;
+  p.vec = vec ? 1u : 0u;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   cudaStream_t st = as_stream(stream);
   return c->dtype == HQB_F16 ? launch_attention<__half>(p, vec, tmem, st)
