@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   Bars& bars = *reinterpret_cast<Bars*>(sm + S::kBars);
   float2* stats = reinterpret_cast<float2*>(sm + S::kStats);
   volatile uint32_t* abort = &bars.abort;
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   uint32_t bad = 0;
   griddep_launch_dependents();
   if ((smem_u32(sm) & 1023u) != 0) {  // the swizzle goes by address bits
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem = uniform(bars.tmem);
   griddep_wait();
   // a wait that runs out ends every role's loop; nothing is left in flight but this CTA's copies
   // (for a whole warp, whose lanes must go on or stop together)
@@ -323,23 +323,25 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
       auto slot_addr = [&](uint32_t n) { return smem_u32(sm + S::kRing + (n % S::kSlots) * S::kTile); };
       // descriptors step by their address field (16-byte units)
       auto scores = [&](uint32_t s, uint32_t tile, uint32_t slot) {
-        const uint64_t qd = umma_desc_sw128(smem_u32(sm + tile * S::kTile), 16), kd = umma_desc_sw128(slot_addr(slot), 16);
-#pragma unroll 1
+        const uint32_t qd = uniform(umma_sw128_low(smem_u32(sm + tile * S::kTile), 16));
+        const uint32_t kd = uniform(umma_sw128_low(slot_addr(slot), 16)), to = uniform(tmem + s * 128);
+#pragma unroll
         for (uint32_t k = 0; k < DP / 16; ++k) {
           const uint32_t step = (k >> 2) * (S::kHalf >> 4) + (k & 3) * 2;
-          warp_mma_f16_ss(tmem + s * 128, qd + step, kd + step, kScores, k > 0 ? 1u : 0u);
+          warp_mma_f16_ss(to, qd + step, kd + step, kScores, k > 0 ? 1u : 0u);
         }
         warp_commit(&bars.s_full[s]);
       };
       auto sums = [&](const Segment* g, uint32_t s, uint32_t i, uint32_t slot, bool first) {
-        const uint64_t vd = umma_desc_sw128(slot_addr(slot), S::kHalf);
+        const uint32_t vd = uniform(umma_sw128_low(slot_addr(slot), S::kHalf));
+        const uint32_t to = uniform(tmem + 256 + s * DP), from = uniform(tmem + s * 128);
         const uint32_t b = g->b0 + i;
         const bool cached = b < g->q.cached_blocks;
-        const uint32_t left = (cached ? g->q.ctx : g->q.nodes) - (cached ? b : b - g->q.cached_blocks) * kKeys;
-        const uint32_t steps = left >= kKeys ? kKeys / 16 : (left + 15) / 16;
-#pragma unroll 1
-        for (uint32_t k = 0; k < steps; ++k)
-          warp_mma_f16_ts(tmem + 256 + s * DP, tmem + s * 128 + k * 8, vd + k * 128, kSums, k > 0 || !first ? 1u : 0u);
+        const uint32_t left = uniform((cached ? g->q.ctx : g->q.nodes) - (cached ? b : b - g->q.cached_blocks) * kKeys);
+        const uint32_t keep = uniform(first ? 0u : 1u);
+#pragma unroll
+        for (uint32_t k = 0; k < kKeys / 16; ++k)
+          if (k * 16 < left) warp_mma_f16_ts(to, from + k * 8, vd + k * 128, kSums, k > 0 ? 1u : keep);
       };
       auto weights_wait = [&](uint32_t s) {
         const bool r = wait_all(&bars.p_full[s], p_at[s]);

@@ -130,22 +130,35 @@ __device__ __forceinline__ float2 poly_exp2(float2 x) {
   return unpack2(mul2(y, pack2(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23))));
 }
 
+// Shared-memory descriptor of an operand in 128-byte-swizzled rows (64 16-bit elements a row, the
+// 16-byte piece c of row r at piece c ^ (r & 7)): 8-row groups 1024 bytes apart.  For an operand
+// whose rows run along its other dimension (MN-major), `lbo` is the distance between 64-element
+// halves of that dimension.
+// (The low word alone depends on the address: kUmmaSw128High is the other.)
+constexpr uint32_t kUmmaSw128High = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t umma_sw128_low(uint32_t smem_addr, uint32_t lbo) {
+  return ((smem_addr >> 4) & 0x3FFFu) | (((lbo >> 4) & 0x3FFFu) << 16);
+}
+
 // D[tmem] (+)= A[smem or tmem] x B[smem], kind::f16, and the commit of what was issued: a whole warp
 // calls them, one elected lane issues (the operands then stay in uniform registers).
-__device__ __forceinline__ void warp_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+// Descriptors are given by their low words.
+__device__ __forceinline__ void warp_mma_f16_ss(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                                 uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kUmmaSw128High)
       : "memory");
 }
-__device__ __forceinline__ void warp_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+__device__ __forceinline__ void warp_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc,
                                                 uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kUmmaSw128High)
       : "memory");
 }
 __device__ __forceinline__ void warp_commit(uint64_t* bar) {
@@ -156,14 +169,6 @@ __device__ __forceinline__ void warp_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void prefetch_map(const void* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
-// Shared-memory descriptor of an operand in 128-byte-swizzled rows (64 16-bit elements a row, the
-// 16-byte piece c of row r at piece c ^ (r & 7)): 8-row groups 1024 bytes apart.  For an operand
-// whose rows run along its other dimension (MN-major), `lbo` is the distance between 64-element
-// halves of that dimension.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t lbo) {
-  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
-         (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // 32 consecutive 32-bit columns of this thread's lane, complete on return (one block, so that
 // nothing reads the registers before the wait).
@@ -215,6 +220,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint6
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// A value that is the same in all lanes, as the compiler can see: it may live in a uniform register.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 __device__ __forceinline__ uint32_t ballot(bool p) { return __ballot_sync(0xffffffffu, p); }
 
 }  // namespace hqb
