@@ -102,11 +102,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 128);
+      mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.o_full[i], 1);
     }
-    mbar_init(&bars.o_free, 256);
-    mbar_init(&bars.joint, 256);
+    mbar_init(&bars.o_free, 8);
+    mbar_init(&bars.joint, 8);
     mbar_init(&bars.drain, 1);
     bars.abort = 0;
     fence_barrier_init();
@@ -128,6 +128,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
     const bool got = !stop && mbar_wait(bar, parity & 1u, p.error);
     if (!stop && !got) *abort = 1u;
     return __all_sync(0xffffffffu, got);
+  };
+  // a warp's one arrival: 32 lanes' would queue at the barrier
+  auto arrive_warp = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
   };
   const uint32_t half = p.rows / 2;  // rows of a tile's first score tile
   // Segment seg is announced by phase seg / 2 of q_full[seg & 1].  No warp can be two phases of one
@@ -360,29 +365,27 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           warp_commit(&bars.kv_empty[slot_at % S::kSlots]);
           if (seg > 0 && !(ok = wait_all(&bars.o_free, seg - 1))) break;
           if (n == 1) warp_commit(&bars.q_empty);
+          // (the slots of the next turn are waited for before its weights, so that nothing stands between
+          // weights that are ready and their MMAs)
+          if (!(ok = slot_wait(slot_at + 1) && (n == 1 || slot_wait(slot_at + 2)))) break;
           for (uint32_t i = 0; i < n; ++i) {
             const uint32_t v = slot_at + 2 * i + 1, k = v + 1;
             const bool more = i + 1 < n;
-            ok = slot_wait(v) && weights_wait(0);
-            if (!ok) break;
+            if (!(ok = weights_wait(0))) break;
             sums(g, 0, i, v, i == 0);
-            if (more) {
-              if (!(ok = slot_wait(k))) break;
-              tc_fence_after();
-              scores(0, 0, k);
-            } else {
-              warp_commit(&bars.o_full[0]);
-            }
+            if (more) scores(0, 0, k);
+            else warp_commit(&bars.o_full[0]);
             if (!(ok = weights_wait(1))) break;
             sums(g, 1, i, v, i == 0);
             warp_commit(&bars.kv_empty[v % S::kSlots]);
-            if (more) {
-              scores(1, 1, k);
-              warp_commit(&bars.kv_empty[k % S::kSlots]);
-              if (i + 2 == n) warp_commit(&bars.q_empty);
-            } else {
+            if (!more) {
               warp_commit(&bars.o_full[1]);
+              break;
             }
+            scores(1, 1, k);
+            warp_commit(&bars.kv_empty[k % S::kSlots]);
+            if (i + 2 == n) warp_commit(&bars.q_empty);
+            if (!(ok = slot_wait(v + 2) && (i + 2 == n || slot_wait(k + 2)))) break;
           }
         } else {
           // slots: K0 K1 V0 K2 V1 K3 ...
@@ -402,16 +405,14 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           if (n <= 2) warp_commit(&bars.q_empty);
           for (uint32_t j = 0; j < n; ++j) {
             const uint32_t s = j & 1, v = next++;
-            ok = slot_wait(v) && weights_wait(s);
-            if (!ok) break;
+            const bool more = j + 2 < n;
+            if (!(ok = slot_wait(v) && (!more || slot_wait(next)) && weights_wait(s))) break;
             sums(g, s, j, v, j < 2);
             warp_commit(&bars.kv_empty[v % S::kSlots]);
-            if (j + 2 < n) {
-              const uint32_t k = next++;
-              if (!(ok = slot_wait(k))) break;
-              tc_fence_after();
-              scores(s, 0, k);
-              warp_commit(&bars.kv_empty[k % S::kSlots]);
+            if (more) {
+              scores(s, 0, next);
+              warp_commit(&bars.kv_empty[next % S::kSlots]);
+              ++next;
               if (j + 3 == n) warp_commit(&bars.q_empty);
             }
           }
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           l += sum.x + sum.y;
           tc_wait_st();
           tc_fence_before();
-          mbar_arrive(&bars.p_full[s]);
+          arrive_warp(&bars.p_full[s]);
         }
         if (!ok) break;
         // ---- the segment's end
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         const bool pair = !two && n > 1;
         if (!two) {
           stats[s * 128 + lrow] = make_float2(m, l);
-          mbar_arrive(&bars.joint);
+          arrive_warp(&bars.joint);
           if (!(ok = wait_all(&bars.joint, joints))) break;
           ++joints;
           const float2 a = stats[lrow], d = stats[128 + lrow];
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
                 l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         }
         tc_fence_before();
-        mbar_arrive(&bars.o_free);
+        arrive_warp(&bars.o_free);
         ++seg;
       }
     }
