@@ -471,28 +471,36 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           if (!(ok = wait_all(&bars.s_full[s], s_at))) break;
           ++s_at;
           tc_fence_after();
-          // two passes over the scores, 32 at a time, in loops that stay short: unrolled over all 128 the
-          // softmax waits for instructions
-          float top = -INFINITY;
+          // Two passes over the scores, 32 columns a piece, in loops that stay short: unrolled over all 128
+          // the softmax waits for instructions.  The first pass ends with the first two pieces in registers,
+          // where the second begins; the weights of pieces 0, 1 lie over the scores of piece 0, those of
+          // 2, 3 over piece 1.
+          if (!all) {  // hidden scores become -inf where they lie
 #pragma unroll 1
-          for (uint32_t x = 0; x < 4; ++x) {
-            uint32_t v[32];
-            tc_ld_x32(sc + x * 32, v);
-            const uint32_t seen = x < 2 ? (x == 0 ? sees[0] : sees[1]) : (x == 2 ? sees[2] : sees[3]);
-            if (!all) {  // the same for the whole warp, as the store back needs
+            for (uint32_t x = 0; x < 4; ++x) {
+              uint32_t v[32];
+              tc_ld_x32(sc + x * 32, v);
+              const uint32_t seen = x < 2 ? (x == 0 ? sees[0] : sees[1]) : (x == 2 ? sees[2] : sees[3]);
 #pragma unroll
               for (int e = 0; e < 32; ++e) v[e] = (seen >> e & 1u) ? v[e] : 0xFF800000u;
               tc_st_x32(sc + x * 32, v);
             }
+            tc_wait_st();
+          }
+          uint32_t va[32], vb[32];
+          float top = -INFINITY;
+#pragma unroll 1
+          for (uint32_t x = 0; x < 2; ++x) {
+            tc_ld_start_x32(sc + (x == 0 ? 64 : 0), va);
+            tc_ld_start_x32(sc + (x == 0 ? 96 : 32), vb);
+            tc_join(va, vb);
             float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
+            for (int e = 0; e < 32; e += 4)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                t4[k] = fmaxf(t4[k], fmaxf(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])));
+              for (int k = 0; k < 4; ++k) t4[k] = fmaxf(t4[k], fmaxf(__uint_as_float(va[e + k]), __uint_as_float(vb[e + k])));
             top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
           }
-          if (!all) tc_wait_st();
           const float tops = top * c;
           const bool grow = tops > m + kSlack || (m == -INFINITY && tops > m);
           if (ballot(grow) != 0) {
@@ -514,10 +522,8 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           const float use = m == -INFINITY ? 0.0f : m;
           const uint64_t c2 = pack2(c, c), u2 = pack2(-use, -use);
           uint64_t sum2 = pack2(0.0f, 0.0f);
-#pragma unroll 1
-          for (uint32_t x = 0; x < 4; ++x) {
-            uint32_t v[32], w16[16];
-            tc_ld_x32(sc + x * 32, v);
+          auto weigh = [&](const uint32_t(&v)[32], uint32_t to) {
+            uint32_t w16[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const float2 t = unpack2(fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, u2));
@@ -527,7 +533,17 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
               sum2 = add2(sum2, pack2(y.x, y.y));
               w16[e] = Elem<T>::pack(y.x, y.y);
             }
-            tc_st_x16(sc + x * 16, w16);
+            tc_st_x16(to, w16);
+          };
+#pragma unroll 1
+          for (uint32_t x = 0; x < 2; ++x) {
+            weigh(va, sc + x * 32);
+            if (x == 0) tc_ld_start_x32(sc + 64, va);
+            weigh(vb, sc + x * 32 + 16);
+            if (x == 0) {
+              tc_ld_start_x32(sc + 96, vb);
+              tc_join(va, vb);
+            }
           }
           const float2 sum = unpack2(sum2);
           l += sum.x + sum.y;
