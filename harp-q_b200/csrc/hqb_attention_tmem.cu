@@ -15,9 +15,6 @@ constexpr uint32_t kRows = 128;      // tensor-memory lanes: rows of one score t
 constexpr uint32_t kCopyWarp = 9;  // plain copies and the values' last rows; warp 8: tensor-map copies
 constexpr uint32_t kMmaWarp = 10;
 constexpr uint32_t kTmemThreads = 384;  // warps 0-7 softmax, 8-10 as above, 11 idle
-// Pairs of weights, of every 8, that go by the polynomial: the special-function unit alone would
-// take 1024 cycles a block and warp, as long as half of both streams' MMAs.
-constexpr int kPolyPairs = 3;
 constexpr float kSlack = 8.0f;       // log2 of how far the maximum may grow before sums are rescaled
 
 // One segment as the MMA and softmax warps see it, written by the loading warp.
@@ -30,7 +27,7 @@ struct Segment {
 
 struct Bars {
   uint64_t kv_full[8], kv_empty[8], fix_full[8];
-  uint64_t q_full[2], q_empty, s_full[2], p_full[2], o_full[2], o_free, joint, drain;
+  uint64_t q_full[2], q_empty, s_full[2], p_full[2][2], o_full[2], o_free, joint, drain;
   uint32_t tmem, abort;
   uint32_t broken[8][8];  // by segment: drafted nodes with an infinity or NaN among their values
   Segment segments[4];
@@ -102,7 +99,8 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.p_full[i][0], 4);
+      mbar_init(&bars.p_full[i][1], 4);
       mbar_init(&bars.o_full[i], 1);
     }
     mbar_init(&bars.o_free, 8);
@@ -337,7 +335,14 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         }
         warp_commit(&bars.s_full[s]);
       };
-      auto sums = [&](const Segment* g, uint32_t s, uint32_t i, uint32_t slot, bool first) {
+      auto weights_wait = [&](uint32_t s, uint32_t half_of) {
+        const bool r = wait_all(&bars.p_full[s][half_of], p_at[s]);
+        p_at[s] += half_of;
+        tc_fence_after();
+        return r;
+      };
+      // the sums of block i, half of its keys as soon as those weights are there
+      auto sums = [&](const Segment* g, uint32_t s, uint32_t i, uint32_t slot, bool first) -> bool {
         const uint32_t vd = uniform(umma_sw128_low(slot_addr(slot), S::kHalf));
         const uint32_t to = uniform(tmem + 256 + s * DP), from = uniform(tmem + s * 128);
         const uint32_t b = g->b0 + i;
@@ -345,14 +350,13 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         const uint32_t left = uniform((cached ? g->q.ctx : g->q.nodes) - (cached ? b : b - g->q.cached_blocks) * kKeys);
         const uint32_t keep = uniform(first ? 0u : 1u);
 #pragma unroll
-        for (uint32_t k = 0; k < kKeys / 16; ++k)
-          if (k * 16 < left) warp_mma_f16_ts(to, from + k * 8, vd + k * 128, kSums, k > 0 ? 1u : keep);
-      };
-      auto weights_wait = [&](uint32_t s) {
-        const bool r = wait_all(&bars.p_full[s], p_at[s]);
-        ++p_at[s];
-        tc_fence_after();
-        return r;
+        for (uint32_t x = 0; x < 2; ++x) {
+          if (!weights_wait(s, x)) return false;
+#pragma unroll
+          for (uint32_t k = x * 4; k < x * 4 + 4; ++k)
+            if (k * 16 < left) warp_mma_f16_ts(to, from + k * 8, vd + k * 128, kSums, k > 0 ? 1u : keep);
+        }
+        return true;
       };
       for (const Segment* g; ok && (g = segment(seg)) != nullptr;) {
         const uint32_t n = g->n;
@@ -371,12 +375,10 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           for (uint32_t i = 0; i < n; ++i) {
             const uint32_t v = slot_at + 2 * i + 1, k = v + 1;
             const bool more = i + 1 < n;
-            if (!(ok = weights_wait(0))) break;
-            sums(g, 0, i, v, i == 0);
+            if (!(ok = sums(g, 0, i, v, i == 0))) break;
             if (more) scores(0, 0, k);
             else warp_commit(&bars.o_full[0]);
-            if (!(ok = weights_wait(1))) break;
-            sums(g, 1, i, v, i == 0);
+            if (!(ok = sums(g, 1, i, v, i == 0))) break;
             warp_commit(&bars.kv_empty[v % S::kSlots]);
             if (!more) {
               warp_commit(&bars.o_full[1]);
@@ -406,8 +408,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           for (uint32_t j = 0; j < n; ++j) {
             const uint32_t s = j & 1, v = next++;
             const bool more = j + 2 < n;
-            if (!(ok = slot_wait(v) && (!more || slot_wait(next)) && weights_wait(s))) break;
-            sums(g, s, j, v, j < 2);
+            if (!(ok = slot_wait(v) && (!more || slot_wait(next)) && sums(g, s, j, v, j < 2))) break;
             warp_commit(&bars.kv_empty[v % S::kSlots]);
             if (more) {
               scores(s, 0, next);
@@ -527,9 +528,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const float2 t = unpack2(fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, u2));
-              float2 y;
-              if (e % 8 < kPolyPairs) y = poly_exp2(t);
-              else y = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+              const float2 y = make_float2(fast_exp2(t.x), fast_exp2(t.y));
               sum2 = add2(sum2, pack2(y.x, y.y));
               w16[e] = Elem<T>::pack(y.x, y.y);
             }
@@ -540,6 +539,10 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             weigh(va, sc + x * 32);
             if (x == 0) tc_ld_start_x32(sc + 64, va);
             weigh(vb, sc + x * 32 + 16);
+            // half of the weights at a time: the first half's products run under the second's exponentials
+            tc_wait_st();
+            tc_fence_before();
+            arrive_warp(&bars.p_full[s][x]);
             if (x == 0) {
               tc_ld_start_x32(sc + 96, vb);
               tc_join(va, vb);
@@ -547,9 +550,6 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           }
           const float2 sum = unpack2(sum2);
           l += sum.x + sum.y;
-          tc_wait_st();
-          tc_fence_before();
-          arrive_warp(&bars.p_full[s]);
         }
         if (!ok) break;
         // ---- the segment's end

@@ -106,30 +106,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// 2^x of two values without the special-function unit, relative error 3e-6: x = n + f with n the
-// nearest whole number (read off the low bits of x + 1.5 * 2^23, biased by 127), 2^f on [-1/2, 1/2]
-// by the polynomial of degree 4 of least relative error (Remez exchange), times 2^n.  Below
-// -127 the factor's bits are zero, so -inf gives 0 exactly; NaN stays NaN; x must be below 128.
-__device__ __forceinline__ float2 poly_exp2(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
-  const uint64_t t = pack2(x.x, x.y);
-  const float magic = 12582912.0f + 127.0f;
-  const uint64_t r = add2(t, pack2(magic, magic));
-  const uint64_t f = fma2(add2(r, pack2(-magic, -magic)), pack2(-1.0f, -1.0f), t);
-  uint64_t y = fma2(f, pack2(9.570101911e-3f, 9.570101911e-3f), pack2(5.591786032e-2f, 5.591786032e-2f));
-  y = fma2(y, f, pack2(2.402474483e-1f, 2.402474483e-1f));
-  y = fma2(y, f, pack2(6.931218147e-1f, 6.931218147e-1f));
-  y = fma2(y, f, pack2(9.999992614e-1f, 9.999992614e-1f));
-  const float2 n = unpack2(r);
-  return unpack2(mul2(y, pack2(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23))));
-}
-
 // Shared-memory descriptor of an operand in 128-byte-swizzled rows (64 16-bit elements a row, the
 // 16-byte piece c of row r at piece c ^ (r & 7)): 8-row groups 1024 bytes apart.  For an operand
 // whose rows run along its other dimension (MN-major), `lbo` is the distance between 64-element
