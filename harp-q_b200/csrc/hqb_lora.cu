@@ -1,6 +1,10 @@
 // Low-rank adapters of many requests beside a shared projection (hqb_lora).
-//   lora_kernel       y = base + scale * B (A x) for one tile of tokens of one adapter a cluster
-//   lora_plan_kernel  groups the tokens of a large call by adapter into tiles
+//   lora_kernel         y = base + scale * B (A x) for up to 16 tokens of one adapter a cluster, in one
+//                       launch: decode steps, and rows that no 16-byte access fits
+// Calls of many tokens, three launches:
+//   lora_plan_kernel    groups the tokens by adapter into tiles
+//   lora_shrink_kernel  t = A x
+//   lora_expand_kernel  y = base + scale * B t
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -38,6 +42,9 @@ struct LoraParams {
   uint32_t planned;
   uint32_t in_place;  // base is y: tokens without an adapter need no work
   uint32_t tile_rows;
+  uint32_t max_tiles;
+  uint32_t splits;    // column ranges of the first product
+  float* inner;       // [splits][max_tiles][tile_rows][padded rank]
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -101,42 +108,253 @@ struct LoraShape {
 template <typename T, typename Y>
 constexpr int kTerms = std::is_same<Y, float>::value ? (std::is_same<T, __half>::value ? 2 : 3) : 1;
 
+// A row of t as terms of T: v[i] is rank i * 32 + lane, already zero past the adapter's rank.  FP16
+// terms are of the row scaled by a power of two to its largest magnitude (exact), so that neither
+// large nor small activations leave the type's range; BF16 has FP32's range.  put(k, rank, bits)
+// takes the terms; the row's factor is returned.
+template <typename T, int RP, int KN, typename Put>
+__device__ __forceinline__ float split_row(const float (&v)[(RP + 31) / 32], uint32_t lane, float scale, Put put) {
+  constexpr int kPer = (RP + 31) / 32;
+  int e = 0;
+  if (std::is_same<T, __half>::value) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top > 0.0f && top < INFINITY) e = max(-100, min(100, ilogbf(top) - 14));
+  }
+  const float down = ldexpf(1.0f, -e);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t r = i * 32 + lane;
+    float rest = v[i] * down;
+#pragma unroll
+    for (int k = 0; k < KN; ++k) {
+      const T term = Elem<T>::from_float(rest);
+      const float back = Elem<T>::to_float(term);
+      if (r < RP) put(k, r, *reinterpret_cast<const uint16_t*>(&term));
+      rest = fabsf(back) < INFINITY ? rest - back : 0.0f;  // an infinity or NaN is all in its first term
+    }
+  }
+  return scale * ldexpf(1.0f, e);
+}
+
+// The second product for one tile: steps of 32 outputs, a warp a step.  The four 8-row tiles of B of
+// a step take rows 8(g/2)+2j+(g%2) of it, which gives each lane 8 adjacent outputs of a token.
+// B and base come by asynchronous copies into a ring of which every lane reads back exactly what
+// it copied itself, so the loop has no barrier, and the first stages can be in flight before t is
+// known (start() may run under the first product).
 template <typename T, typename Y, int RP, int M>
-constexpr uint32_t kLoraSmem = 64 * 4 + M * 4 + M * 4 + kTerms<T, Y> * M * LoraShape<RP>::kPitch * 2 + M * RP * 4 +
-                               (M == 16 ? 8 : 4) * M * RP * 4;
-
-// Mathematics: t = A x (FP32 sums of exact 16-bit products), y = base + scale B t.
-// Split: a cluster of 8 CTAs takes one tile of up to M tokens of one adapter.  First its CTAs and
-// their warps divide the columns of x and A (every element of x is read once, straight into MMA
-// fragments: the columns of a 32-column step may be taken in any order, so a lane's 16 bytes are
-// both k-halves of two MMAs); the partial t are summed in warp order, then through distributed
-// shared memory in CTA order, so the bits do not depend on timing.  Then the CTAs divide the rows
-// of B and of the output: the four 8-row tiles of a 32-row step take rows 8(g/2)+2j+(g%2), which
-// gives each lane 8 adjacent outputs of a token.  One launch, no scratch, no atomics.
-// Bound by bytes: x, base and y once, A and B once a tile (from L2 for every tile but the first).
-template <typename T, typename Y, int RP, int M, bool VEC>
-__global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ LoraParams p) {
+struct Expand {
   using S = LoraShape<RP>;
-  constexpr int kMW = M == 16 ? 1 : 2;               // 16-row tiles a warp multiplies in the first product
-  constexpr uint32_t kWM = M == 16 ? 1 : 2;          // warps along the rows
-  constexpr uint32_t kSlices = 8 / kWM;              // warps along the columns
-  constexpr int kN = kTerms<T, Y>;
-  extern __shared__ __align__(128) uint8_t sm[];
-  uint32_t* s_info = reinterpret_cast<uint32_t*>(sm);                       // 64 words
-  int32_t* s_token = reinterpret_cast<int32_t*>(sm + 256);                  // [M], -1: no row
-  float* s_factor = reinterpret_cast<float*>(s_token + M);                  // [M]
-  T* s_terms = reinterpret_cast<T*>(s_factor + M);                          // [kN][M][kPitch]
-  float* s_sum = reinterpret_cast<float*>(s_terms + kN * M * S::kPitch);    // [M][RP] this CTA's t
-  float* s_part = s_sum + M * RP;                                           // [kSlices][M][RP]
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const uint32_t cta = cluster_rank(), tile = blockIdx.x / kCluster;
-  uint32_t bad = 0;
-  griddep_wait();
+  static constexpr int kN = kTerms<T, Y>;
+  static constexpr int kBaseVecs = sizeof(Y) == 4 ? 2 : 1;             // 16-byte pieces of 8 outputs
+  static constexpr uint32_t kBBytes = RP == 16 ? 4 * 8 : 4 * S::kGroups * 16;  // a lane's B of a step
+  static constexpr uint32_t kBaseBytes = M / 16 * 2 * kBaseVecs * 16;
+  static constexpr uint32_t kStage = 32 * (kBBytes + kBaseBytes);      // a warp's bytes of a step
 
-  // ---- the tile: an adapter and its tokens
-  uint32_t group, count;
+  static constexpr int kRowsEach = M / 8;  // rows of a lane: g and g + 8 of every 16
+  // terms of a lane that stay in registers over the steps, where they are few
+  static constexpr bool kHold = kN == 1 && RP > 16 && M / 16 * S::kGroups <= 8;
+
+  const T* b;                  // the lane's first B row of step 0
+  const Y* base[kRowsEach];    // the lane's rows at its first output of step 0; null: no row, no base
+  Y* y[kRowsEach];
+  uint64_t rows;
+  uint32_t pitch, rank, count, ring, stages, lane;
+
+  __device__ __forceinline__ void prepare(const LoraParams& p, uint32_t group, uint32_t rank_, uint32_t count_,
+                                          const int32_t* s_token, uint32_t ring_, uint32_t stages_) {
+    lane = threadIdx.x & 31;
+    const uint32_t g = lane >> 2, q = lane & 3;
+    rows = p.s.rows, pitch = p.s.max_rank, rank = rank_, count = count_, ring = ring_, stages = stages_;
+    b = static_cast<const T*>(p.s.b) + (static_cast<uint64_t>(min(group, p.s.adapters - 1)) * rows + 8 * (g >> 1) + (g & 1)) * pitch +
+        q * (RP == 16 ? 4 : 8);
+#pragma unroll
+    for (int i = 0; i < kRowsEach; ++i) {
+      const int32_t t = s_token[(i >> 1) * 16 + g + 8 * (i & 1)];
+      const uint64_t row = static_cast<uint64_t>(max(t, 0));
+      base[i] = t < 0 || p.base == nullptr ? nullptr : static_cast<const Y*>(p.base) + row * p.base_stride + q * 8;
+      y[i] = t < 0 ? nullptr : static_cast<Y*>(p.y) + row * p.y_stride + q * 8;
+    }
+  }
+  // copies of step st into stage at `to` (shared address)
+  __device__ __forceinline__ void load(uint32_t st, uint32_t to) const {
+    const uint32_t g = lane >> 2, q = lane & 3;
+    const uint64_t n0 = static_cast<uint64_t>(st) * 32;
+    const uint32_t left = rows - n0 < 32 ? static_cast<uint32_t>(rows - n0) : 32u;  // outputs of the step
+    if (rank != 0) {
+      const T* row = b + n0 * pitch;
+#pragma unroll
+      for (int j = 0; j < 4; ++j, row += 2 * pitch) {
+        const bool inside = 8 * (g >> 1) + 2 * j + (g & 1) < left;
+        if constexpr (RP == 16) {
+          const bool real = inside && q * 4 < rank;
+          cp_async8(to + (j * 32 + lane) * 8, real ? row : b, real ? 8u : 0u);
+        } else {
+#pragma unroll
+          for (int k = 0; k < S::kGroups; ++k) {
+            const bool real = inside && k * 32 + q * 8 < rank;
+            cp_async16(to + ((j * S::kGroups + k) * 32 + lane) * 16, real ? row + k * 32 : b, real ? 16u : 0u);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsEach; ++i)
+      if (base[i] != nullptr && q * 8 < left) {
+#pragma unroll
+        for (int v = 0; v < kBaseVecs; ++v)
+          cp_async16(to + 32 * kBBytes + ((i * kBaseVecs + v) * 32 + lane) * 16, base[i] + n0 + v * 4, 16u);
+      }
+  }
+  // the first stages - 1 steps of a warp that takes steps first, first + 8, ... below end
+  __device__ __forceinline__ void start(uint32_t first, uint32_t end) const {
+    for (uint32_t s = 0; s + 1 < stages; ++s) {
+      if (first + s * 8 < end) load(first + s * 8, ring + s * kStage);
+      cp_async_commit();
+    }
+  }
+  __device__ __forceinline__ void run(uint32_t first, uint32_t end, const T* terms, const float* factor) const {
+    const uint32_t g = lane >> 2, q = lane & 3;
+    uint32_t stage = 0;
+    float f[kRowsEach];
+    uint4 held[kHold ? M / 16 : 1][kHold ? S::kGroups : 1][2];
+    if (rank != 0) {
+#pragma unroll
+      for (int i = 0; i < kRowsEach; ++i) f[i] = factor[(i >> 1) * 16 + g + 8 * (i & 1)];
+      if constexpr (kHold) {
+#pragma unroll
+        for (int mt = 0; mt < M / 16; ++mt)
+#pragma unroll
+          for (int k = 0; k < S::kGroups; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              held[mt][k][e] = *reinterpret_cast<const uint4*>(terms + (mt * 16 + g + 8 * e) * S::kPitch + k * 32 + q * 8);
+      }
+    }
+    for (uint32_t st = first; st < end; st += 8) {
+      {
+        const uint32_t ahead = st + (stages - 1) * 8, to = stage == 0 ? stages - 1 : stage - 1;
+        if (ahead < end) load(ahead, ring + to * kStage);
+        cp_async_commit();
+      }
+      cp_async_wait_dynamic(stages - 1);
+      const uint32_t at = ring + stage * kStage;
+      stage = stage + 1 == stages ? 0 : stage + 1;
+      uint4 bv[4][S::kGroups];
+      if (rank != 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < S::kGroups; ++k) {
+            if constexpr (RP == 16) {
+              const uint2 v = lds64a(at + (j * 32 + lane) * 8);
+              bv[j][k] = make_uint4(v.x, v.y, 0, 0);
+            } else {
+              bv[j][k] = lds128a(at + ((j * S::kGroups + k) * 32 + lane) * 16);
+            }
+          }
+        if (rank < RP) {  // columns past the adapter's rank may hold anything
+#pragma unroll
+          for (int k = 0; k < S::kGroups; ++k) {
+            const int32_t left = static_cast<int32_t>(rank) - static_cast<int32_t>(RP == 16 ? q * 4 : k * 32 + q * 8);
+            const uint32_t m0 = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u, m1 = left >= 4 ? 0xFFFFFFFFu : left == 3 ? 0xFFFFu : 0u;
+            const uint32_t m2 = left >= 6 ? 0xFFFFFFFFu : left == 5 ? 0xFFFFu : 0u, m3 = left >= 8 ? 0xFFFFFFFFu : left == 7 ? 0xFFFFu : 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bv[j][k].x &= m0, bv[j][k].y &= m1, bv[j][k].z &= m2, bv[j][k].w &= m3;
+          }
+        }
+      }
+      const uint64_t n0 = static_cast<uint64_t>(st) * 32;
+      const bool inside = n0 + q * 8 < rows;
+#pragma unroll
+      for (int mt = 0; mt < M / 16; ++mt) {
+        if (mt * 16 >= static_cast<int>(count)) break;
+        float acc[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+        if (rank != 0) {
+#pragma unroll
+          for (int t = kN - 1; t >= 0; --t) {  // small terms first
+            const T* lo = terms + (t * M + mt * 16 + g) * S::kPitch;
+            const T* hi = lo + 8 * S::kPitch;
+#pragma unroll
+            for (int k = 0; k < S::kGroups; ++k) {
+              if constexpr (RP == 16) {
+                const uint2 u = *reinterpret_cast<const uint2*>(lo + q * 4), v = *reinterpret_cast<const uint2*>(hi + q * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) Elem<T>::mma(acc[j], u.x, v.x, u.y, v.y, bv[j][k].x, bv[j][k].y);
+              } else {
+                uint4 u, v;
+                if constexpr (kHold) u = held[mt][k][0], v = held[mt][k][1];
+                else u = *reinterpret_cast<const uint4*>(lo + k * 32 + q * 8), v = *reinterpret_cast<const uint4*>(hi + k * 32 + q * 8);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  Elem<T>::mma(acc[j], u.x, v.x, u.y, v.y, bv[j][k].x, bv[j][k].y);
+                  Elem<T>::mma(acc[j], u.z, v.z, u.w, v.w, bv[j][k].z, bv[j][k].w);
+                }
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = mt * 2 + e;
+          if (y[i] == nullptr || !inside) continue;
+          float out[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) out[x] = 0.0f;
+          if (base[i] != nullptr) {
+            const uint32_t from = at + 32 * kBBytes + i * kBaseVecs * 512 + lane * 16;
+            const uint4 v = lds128a(from);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            if constexpr (sizeof(Y) == 4) {
+              const uint4 u = lds128a(from + 512);
+              const uint32_t z[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int x = 0; x < 4; ++x) out[x] = __uint_as_float(w[x]), out[4 + x] = __uint_as_float(z[x]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 h = Elem<T>::unpack(w[x]);
+                out[2 * x] = h.x, out[2 * x + 1] = h.y;
+              }
+            }
+          }
+          if (rank != 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              out[2 * j] = fmaf(f[i], acc[j][2 * e], out[2 * j]);
+              out[2 * j + 1] = fmaf(f[i], acc[j][2 * e + 1], out[2 * j + 1]);
+            }
+          }
+          Y* dst = y[i] + n0;
+          if constexpr (sizeof(Y) == 4) {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(out[0], out[1], out[2], out[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(out[4], out[5], out[6], out[7]);
+          } else {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(Elem<T>::pack(out[0], out[1]), Elem<T>::pack(out[2], out[3]),
+                                                        Elem<T>::pack(out[4], out[5]), Elem<T>::pack(out[6], out[7]));
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+  }
+};
+
+// The tile of a planned call, or the tile that a cluster finds by itself: an adapter (`adapters`:
+// none), its tokens in s_token (-1 past them) and their count; false: nothing to do.
+template <int M>
+__device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, int32_t* s_token, uint32_t* s_info, uint32_t& group,
+                                          uint32_t& count, uint32_t& bad) {
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (p.planned) {
-    if (tile >= *p.tile_count) return;
+    if (tile >= *p.tile_count) return false;
     const LoraTile t = p.tiles[tile];
     group = t.group;
     count = t.count;
@@ -159,59 +377,109 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
       if (w == (tile >> 5)) before += __popc(v & ((1u << (tile & 31)) - 1u));
       if (w < warp) mine += n;
     }
-    if (before % M != 0) return;
+    if (before % M != 0) return false;
     mine += __popc(votes & ((1u << lane) - 1u));
     if (same && mine >= before && mine < before + M) s_token[mine - before] = static_cast<int32_t>(tid);
     count = min(static_cast<uint32_t>(M), all - before);
   }
   __syncthreads();
-  uint32_t rank = 0;
-  float scale = 0.0f;
-  if (group < p.s.adapters) {
-    const int32_t v = p.s.ranks != nullptr ? __ldg(p.s.ranks + group) : static_cast<int32_t>(p.s.max_rank);
-    if (v < 0 || v > static_cast<int32_t>(p.s.max_rank)) bad |= HQB_DEVERR_INDEX;
-    rank = v < 0 ? 0u : min(static_cast<uint32_t>(v), p.s.max_rank);
-    scale = p.s.scales != nullptr ? __ldg(p.s.scales + group) : 1.0f;
-  }
+  return true;
+}
+
+// An adapter's rank (0 for none) and factor.
+__device__ __forceinline__ uint32_t adapter(const LoraParams& p, uint32_t group, float& scale, uint32_t& bad) {
+  scale = 0.0f;
+  if (group >= p.s.adapters) return 0;
+  const int32_t v = p.s.ranks != nullptr ? __ldg(p.s.ranks + group) : static_cast<int32_t>(p.s.max_rank);
+  if (v < 0 || v > static_cast<int32_t>(p.s.max_rank)) bad |= HQB_DEVERR_INDEX;
+  scale = p.s.scales != nullptr ? __ldg(p.s.scales + group) : 1.0f;
+  return v < 0 ? 0u : min(static_cast<uint32_t>(v), p.s.max_rank);
+}
+
+constexpr uint32_t kSliceWarps = 8;  // warps along the columns in lora_kernel
+
+template <typename T, typename Y, int RP>
+struct LoraSmem {
+  static constexpr uint32_t kToken = 256, kFactor = kToken + 64, kTermsAt = kFactor + 64;
+  static constexpr uint32_t kSum = kTermsAt + kTerms<T, Y> * 16 * LoraShape<RP>::kPitch * 2;
+  static constexpr uint32_t kPart = kSum + 16 * RP * 4;
+  static constexpr uint32_t kRing = kPart + kSliceWarps * 16 * RP * 4;
+  // as many stages as leave room for two CTAs an SM, else as fit one
+  static constexpr uint32_t kTwo = kRing < 110 * 1024 ? (110 * 1024 - kRing) / (8 * Expand<T, Y, RP, 16>::kStage) : 0;
+  static constexpr uint32_t kOne = (227 * 1024 - kRing) / (8 * Expand<T, Y, RP, 16>::kStage);
+  static constexpr uint32_t kStages = kTwo > 6 ? 6 : kTwo >= 2 ? kTwo : kOne >= 2 ? 2 : 1;
+  static_assert(kOne >= 1, "a stage fits");
+  static constexpr uint32_t kBytes = kRing + 8 * kStages * Expand<T, Y, RP, 16>::kStage;
+};
+
+// Mathematics: t = A x (FP32 sums of exact 16-bit products), y = base + scale B t.
+// Split: a cluster of 8 CTAs takes one tile of up to 16 tokens of one adapter.  First its CTAs and
+// their warps divide the columns of x and A (every element of x is read once, straight into MMA
+// fragments: the columns of a 32-column step may be taken in any order, so a lane's 16 bytes are
+// both k-halves of two MMAs); the partial t are summed in warp order, then through distributed
+// shared memory in CTA order, so the bits do not depend on timing.  Then the CTAs divide the rows
+// of B and of the output; their first rows of B and of base are under way from the start.  One
+// launch, no scratch, no atomics.
+// Bound by latency (two trips to memory and two cluster barriers) up to a few adapters, then by the
+// adapters' bytes.
+template <typename T, typename Y, int RP, bool VEC>
+__global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ LoraParams p) {
+  using S = LoraShape<RP>;
+  using L = LoraSmem<T, Y, RP>;
+  constexpr int kN = kTerms<T, Y>;
+  constexpr uint32_t M = 16;
+  extern __shared__ __align__(128) uint8_t sm[];
+  uint32_t* s_info = reinterpret_cast<uint32_t*>(sm);             // 64 words
+  int32_t* s_token = reinterpret_cast<int32_t*>(sm + L::kToken);  // [M], -1: no row
+  float* s_factor = reinterpret_cast<float*>(sm + L::kFactor);    // [M]
+  T* s_terms = reinterpret_cast<T*>(sm + L::kTermsAt);            // [kN][M][kPitch]
+  float* s_sum = reinterpret_cast<float*>(sm + L::kSum);          // [M][RP] this CTA's t
+  float* s_part = reinterpret_cast<float*>(sm + L::kPart);        // [kSliceWarps][M][RP]
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const uint32_t cta = cluster_rank(), tile = blockIdx.x / kCluster;
+  uint32_t bad = 0, group, count;
+  griddep_wait();
+  if (!find_tile<M>(p, tile, s_token, s_info, group, count, bad)) return;
+  float scale;
+  const uint32_t rank = adapter(p, group, scale, bad);
   if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
   if (rank == 0 && p.in_place) return;
   const uint64_t cols = p.s.cols, rows = p.s.rows;
+  const T* b = static_cast<const T*>(p.s.b) + static_cast<uint64_t>(min(group, p.s.adapters - 1)) * p.s.max_rank * rows;
+  const uint32_t n_steps = static_cast<uint32_t>((rows + 31) / 32);
+  const uint32_t n0 = static_cast<uint64_t>(n_steps) * cta / kCluster, n1 = static_cast<uint64_t>(n_steps) * (cta + 1) / kCluster;
+  Expand<T, Y, RP, M> x2;
+  x2.prepare(p, group, rank, count, s_token, smem_u32(sm) + L::kRing + warp * L::kStages * Expand<T, Y, RP, M>::kStage, L::kStages);
+  if (VEC) x2.start(n0 + warp, n1);
 
   if (rank != 0) {
     // ---- t = A x, this CTA's columns
     const T* a = static_cast<const T*>(p.s.a) + static_cast<uint64_t>(group) * p.s.max_rank * cols;
-    const uint32_t wm = warp % kWM, slice = warp / kWM;
-    const T* xr[kMW][2];
-    bool xl[kMW][2];
+    const T* xr[2];
+    bool xl[2];
 #pragma unroll
-    for (int i = 0; i < kMW; ++i)
+    for (int e = 0; e < 2; ++e) {
+      const int32_t t = s_token[g + 8 * e];
+      xl[e] = t >= 0;
+      xr[e] = static_cast<const T*>(p.x) + static_cast<uint64_t>(max(t, 0)) * p.x_stride;
+    }
+    float acc[S::kTiles8][4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int32_t t = s_token[(wm * kMW + i) * 16 + g + 8 * e];
-        xl[i][e] = t >= 0;
-        xr[i][e] = static_cast<const T*>(p.x) + static_cast<uint64_t>(max(t, 0)) * p.x_stride;
-      }
-    float acc[kMW][S::kTiles8][4];
+    for (int n = 0; n < S::kTiles8; ++n)
 #pragma unroll
-    for (int i = 0; i < kMW; ++i)
-#pragma unroll
-      for (int n = 0; n < S::kTiles8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
     const uint32_t steps = static_cast<uint32_t>((cols + 31) / 32);
     const uint32_t step0 = static_cast<uint64_t>(steps) * cta / kCluster, step1 = static_cast<uint64_t>(steps) * (cta + 1) / kCluster;
-    constexpr int kAhead = RP <= 32 ? (M == 16 ? 4 : 2) : (M == 16 && RP == 64 ? 2 : 1);
-    for (uint32_t st = step0 + slice; st < step1; st += kSlices * kAhead) {
-      uint4 xv[kAhead][kMW][2], av[kAhead][S::kTiles8];
+    constexpr int kAhead = RP <= 32 ? 4 : RP == 64 ? 2 : 1;
+    for (uint32_t st = step0 + warp; st < step1; st += kSliceWarps * kAhead) {
+      uint4 xv[kAhead][2], av[kAhead][S::kTiles8];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const uint32_t s = st + u * kSlices;
+        const uint32_t s = st + u * kSliceWarps;
         const uint64_t col = static_cast<uint64_t>(s) * 32 + q * 8;
         const int64_t real = s < step1 ? static_cast<int64_t>(cols) - static_cast<int64_t>(col) : 0;
 #pragma unroll
-        for (int i = 0; i < kMW; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) xv[u][i][e] = load8<VEC>(xr[i][e] + col, xl[i][e] ? real : 0);
+        for (int e = 0; e < 2; ++e) xv[u][e] = load8<VEC>(xr[e] + col, xl[e] ? real : 0);
 #pragma unroll
         for (int n = 0; n < S::kTiles8; ++n)
           av[u][n] = load8<VEC>(a + (n * 8 + g) * cols + col, n * 8 + g < rank ? real : 0);
@@ -219,35 +487,31 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-        for (int n = 0; n < S::kTiles8; ++n)
-#pragma unroll
-          for (int i = 0; i < kMW; ++i) {
-            Elem<T>::mma(acc[i][n], xv[u][i][0].x, xv[u][i][1].x, xv[u][i][0].y, xv[u][i][1].y, av[u][n].x, av[u][n].y);
-            Elem<T>::mma(acc[i][n], xv[u][i][0].z, xv[u][i][1].z, xv[u][i][0].w, xv[u][i][1].w, av[u][n].z, av[u][n].w);
-          }
+        for (int n = 0; n < S::kTiles8; ++n) {
+          Elem<T>::mma(acc[n], xv[u][0].x, xv[u][1].x, xv[u][0].y, xv[u][1].y, av[u][n].x, av[u][n].y);
+          Elem<T>::mma(acc[n], xv[u][0].z, xv[u][1].z, xv[u][0].w, xv[u][1].w, av[u][n].z, av[u][n].w);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < kMW; ++i)
+    for (int n = 0; n < S::kTiles8; ++n)
 #pragma unroll
-      for (int n = 0; n < S::kTiles8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float2*>(s_part + (slice * M + (wm * kMW + i) * 16 + g + 8 * e) * RP + n * 8 + q * 2) =
-              make_float2(acc[i][n][2 * e], acc[i][n][2 * e + 1]);
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<float2*>(s_part + (warp * M + g + 8 * e) * RP + n * 8 + q * 2) =
+            make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
     __syncthreads();
     for (uint32_t i = tid; i < M * RP; i += kThreads) {
       float v = 0.0f;
 #pragma unroll
-      for (uint32_t k = 0; k < kSlices; ++k) v += s_part[k * M * RP + i];
+      for (uint32_t k = 0; k < kSliceWarps; ++k) v += s_part[k * M * RP + i];
       s_sum[i] = v;
     }
     cluster_sync();
-    // ---- sum over the CTAs; each owns M / 8 rows, a warp a row, and hands the row's terms and
-    // factor to all of them
-    for (uint32_t own = warp; own < M / kCluster; own += kThreads / 32) {
-      const uint32_t row = cta * (M / kCluster) + own;
+    // ---- sum over the CTAs; each owns 2 rows, a warp a row, and hands the row's terms and factor to
+    // all of them
+    if (warp < M / kCluster) {
+      const uint32_t row = cta * (M / kCluster) + warp;
       constexpr int kPer = (RP + 31) / 32;
-      float v[kPer], top = 0.0f;
+      float v[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const uint32_t r = i * 32 + lane;
@@ -258,179 +522,205 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
           for (uint32_t c = 0; c < kCluster; ++c) sum += peer_load(peer_smem(at, c));
         }
         v[i] = r < rank ? sum : 0.0f;
-        top = fmaxf(top, fabsf(v[i]));
       }
-      // FP16 terms: the row scaled by a power of two to its largest magnitude (exact), so that
-      // neither large nor small activations leave the type's range; BF16 has FP32's range
-      int e = 0;
-      if (std::is_same<T, __half>::value) {
+      const float f = split_row<T, RP, kN>(v, lane, scale, [&](int k, uint32_t r, uint16_t bits) {
+        const uint32_t at = smem_u32(s_terms + (k * M + row) * S::kPitch + r);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (top > 0.0f && top < INFINITY) e = max(-100, min(100, ilogbf(top) - 14));
-      }
-      const float down = ldexpf(1.0f, -e);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const uint32_t r = i * 32 + lane;
-        float rest = v[i] * down;
-#pragma unroll
-        for (int k = 0; k < kN; ++k) {
-          const T term = Elem<T>::from_float(rest);
-          const float back = Elem<T>::to_float(term);
-          if (r < RP) {
-            const uint32_t at = smem_u32(s_terms + (k * M + row) * S::kPitch + r);
-#pragma unroll
-            for (uint32_t c = 0; c < kCluster; ++c) peer_store16(peer_smem(at, c), *reinterpret_cast<const uint16_t*>(&term));
-          }
-          // an infinity or NaN is all in its first term
-          rest = fabsf(back) < INFINITY ? rest - back : 0.0f;
-        }
-      }
-      if (lane < kCluster) peer_store(peer_smem(smem_u32(s_factor + row), lane), scale * ldexpf(1.0f, e));
+        for (uint32_t c = 0; c < kCluster; ++c) peer_store16(peer_smem(at, c), bits);
+      });
+      if (lane < kCluster) peer_store(peer_smem(smem_u32(s_factor + row), lane), f);
     }
     cluster_sync();
   }
-
-  // ---- y = base + factor * B t, this CTA's rows of B
-  const T* b = static_cast<const T*>(p.s.b) + static_cast<uint64_t>(min(group, p.s.adapters - 1)) * p.s.max_rank * rows;
-  const uint32_t steps = static_cast<uint32_t>((rows + 31) / 32);
-  const uint32_t step0 = static_cast<uint64_t>(steps) * cta / kCluster, step1 = static_cast<uint64_t>(steps) * (cta + 1) / kCluster;
-  for (uint32_t st = step0 + warp; st < step1; st += kThreads / 32) {
-    uint4 bv[4][S::kGroups];
-    if (rank != 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint64_t n = static_cast<uint64_t>(st) * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
-        const T* row = b + n * p.s.max_rank;
-#pragma unroll
-        for (int k = 0; k < S::kGroups; ++k) {
-          if constexpr (RP == 16) {
-            const int32_t left = n < rows ? static_cast<int32_t>(rank) - static_cast<int32_t>(q * 4) : 0;
-            uint2 v = make_uint2(0, 0);
-            if (VEC) {
-              if (left > 0) v = __ldg(reinterpret_cast<const uint2*>(row + q * 4));
-              if (left < 4) v.y &= left == 3 ? 0xFFFFu : 0u;
-              if (left < 2) v.x &= left == 1 ? 0xFFFFu : 0u;
-            } else {
-              const uint4 w = load8<false>(row + q * 4, left < 4 ? left : 4);
-              v = make_uint2(w.x, w.y);
-            }
-            bv[j][k] = make_uint4(v.x, v.y, 0, 0);
-          } else {
-            const int32_t left = n < rows ? static_cast<int32_t>(rank) - static_cast<int32_t>(k * 32 + q * 8) : 0;
-            uint4 v = load8<VEC>(row + k * 32 + q * 8, left);
-            if (VEC && left < 8) {  // columns past the adapter's rank may hold anything
-              v.x &= left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
-              v.y &= left >= 4 ? 0xFFFFFFFFu : left == 3 ? 0xFFFFu : 0u;
-              v.z &= left >= 6 ? 0xFFFFFFFFu : left == 5 ? 0xFFFFu : 0u;
-              v.w &= left == 7 ? 0xFFFFu : 0u;
-            }
-            bv[j][k] = v;
-          }
-        }
+  if constexpr (VEC) {
+    x2.run(n0 + warp, n1, s_terms, s_factor);
+  } else {
+    // ---- y = base + factor * B t element by element, this CTA's rows of B
+    for (uint64_t i = static_cast<uint64_t>(n0) * 32 * count + tid; i < static_cast<uint64_t>(n1) * 32 * count; i += kThreads) {
+      const uint64_t n = i / count;
+      const uint32_t m = static_cast<uint32_t>(i - n * count);
+      if (n >= rows) break;
+      const uint64_t t = static_cast<uint64_t>(s_token[m]);
+      float v = 0.0f;
+      for (uint32_t r = 0; r < rank; ++r) {
+        float term = 0.0f;
+  #pragma unroll
+        for (int k = kN - 1; k >= 0; --k) term += Elem<T>::to_float(s_terms[(k * M + m) * S::kPitch + r]);
+        v = fmaf(term, Elem<T>::to_float(b[n * p.s.max_rank + r]), v);
       }
-    }
-    const uint64_t n0 = static_cast<uint64_t>(st) * 32 + q * 8;
-    const int64_t real = static_cast<int64_t>(rows) - static_cast<int64_t>(n0);
-#pragma unroll
-    for (int mt = 0; mt < M / 16; ++mt) {
-      if (mt * 16 >= static_cast<int>(count)) break;
-      float out[2][8];
-      int32_t token[2];
-      // base first: its loads run under the products
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        token[e] = s_token[mt * 16 + g + 8 * e];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[e][i] = 0.0f;
-        if (token[e] >= 0 && p.base != nullptr) {
-          const Y* src = static_cast<const Y*>(p.base) + static_cast<uint64_t>(token[e]) * p.base_stride + n0;
-          if (VEC && real > 0) {
-            if constexpr (sizeof(Y) == 4) {
-              const float4 lo = reinterpret_cast<const float4*>(src)[0], hi = reinterpret_cast<const float4*>(src)[1];
-              out[e][0] = lo.x; out[e][1] = lo.y; out[e][2] = lo.z; out[e][3] = lo.w;
-              out[e][4] = hi.x; out[e][5] = hi.y; out[e][6] = hi.z; out[e][7] = hi.w;
-            } else {
-              const uint4 v = *reinterpret_cast<const uint4*>(src);
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 f = Elem<T>::unpack(w[i]);
-                out[e][2 * i] = f.x;
-                out[e][2 * i + 1] = f.y;
-              }
-            }
-          } else if (!VEC) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i < real) {
-                if constexpr (sizeof(Y) == 4) out[e][i] = src[i];
-                else out[e][i] = Elem<T>::to_float(src[i]);
-              }
-          }
-        }
-      }
-      if (rank != 0) {
-        float acc[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-#pragma unroll
-        for (int t = kN - 1; t >= 0; --t) {  // small terms first
-          const T* lo = s_terms + (t * M + mt * 16 + g) * S::kPitch;
-          const T* hi = lo + 8 * S::kPitch;
-#pragma unroll
-          for (int k = 0; k < S::kGroups; ++k) {
-            if constexpr (RP == 16) {
-              const uint2 u = *reinterpret_cast<const uint2*>(lo + q * 4), v = *reinterpret_cast<const uint2*>(hi + q * 4);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) Elem<T>::mma(acc[j], u.x, v.x, u.y, v.y, bv[j][k].x, bv[j][k].y);
-            } else {
-              const uint4 u = *reinterpret_cast<const uint4*>(lo + k * 32 + q * 8);
-              const uint4 v = *reinterpret_cast<const uint4*>(hi + k * 32 + q * 8);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                Elem<T>::mma(acc[j], u.x, v.x, u.y, v.y, bv[j][k].x, bv[j][k].y);
-                Elem<T>::mma(acc[j], u.z, v.z, u.w, v.w, bv[j][k].z, bv[j][k].w);
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float f = s_factor[mt * 16 + g + 8 * e];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            out[e][2 * j] += f * acc[j][2 * e];
-            out[e][2 * j + 1] += f * acc[j][2 * e + 1];
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (token[e] < 0) continue;
-        Y* dst = static_cast<Y*>(p.y) + static_cast<uint64_t>(token[e]) * p.y_stride + n0;
-        if (VEC) {
-          if (real <= 0) continue;
-          if constexpr (sizeof(Y) == 4) {
-            reinterpret_cast<float4*>(dst)[0] = make_float4(out[e][0], out[e][1], out[e][2], out[e][3]);
-            reinterpret_cast<float4*>(dst)[1] = make_float4(out[e][4], out[e][5], out[e][6], out[e][7]);
-          } else {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(Elem<T>::pack(out[e][0], out[e][1]), Elem<T>::pack(out[e][2], out[e][3]),
-                                                        Elem<T>::pack(out[e][4], out[e][5]), Elem<T>::pack(out[e][6], out[e][7]));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < real) {
-              if constexpr (sizeof(Y) == 4) dst[i] = out[e][i];
-              else dst[i] = Elem<T>::from_float(out[e][i]);
-            }
-        }
+      float out = rank != 0 ? s_factor[m] * v : 0.0f;
+      if constexpr (sizeof(Y) == 4) {
+        if (p.base != nullptr) out += static_cast<const float*>(p.base)[t * p.base_stride + n];
+        static_cast<float*>(p.y)[t * p.y_stride + n] = out;
+      } else {
+        if (p.base != nullptr) out += Elem<T>::to_float(static_cast<const T*>(p.base)[t * p.base_stride + n]);
+        static_cast<T*>(p.y)[t * p.y_stride + n] = Elem<T>::from_float(out);
       }
     }
   }
+}
+
+// Rows of a tile of a planned call: 64, or half of that where two stages of the expand kernel's ring
+// would not fit shared memory.
+template <int RP, int YBytes>
+constexpr int kTileRows = RP <= 32 || (RP == 64 && YBytes == 2) ? 64 : 32;
+constexpr uint32_t kShrinkCols = 128, kShrinkStages = 3;
+
+template <int RP, int M>
+constexpr uint32_t kShrinkSmem = 512 + kShrinkStages * (M + RP) * kShrinkCols * 2;
+
+// t = A x of one tile and one range of columns, FP32, to the workspace [split][tile row][RP].
+// Split: 16 rows by RP / (8 / row tiles) ranks a warp; x and A come in chunks of 64 columns by
+// asynchronous copies, four chunks deep.  A lane reads 16 bytes of a row at a time (both k-halves of
+// two MMAs); piece c of row r lies at c ^ 4(r & 1), which those reads meet without conflicts.
+// Bound by the bytes of x (A comes from L2).
+template <typename T, int RP, int M>
+__global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+  constexpr uint32_t kWM = M / 16, kWN = 8 / kWM;                 // warps along rows, along ranks
+  constexpr int kNT = RP / 8 / kWN;                               // 8-rank tiles of a warp
+  constexpr uint32_t kStage = (M + RP) * kShrinkCols * 2, kPieces = kShrinkCols / 8;
+  extern __shared__ __align__(128) uint8_t sm[];
+  int32_t* s_token = reinterpret_cast<int32_t*>(sm);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const uint32_t tile = blockIdx.x / p.splits, split = blockIdx.x - tile * p.splits;
+  uint32_t bad = 0, group, count;
+  griddep_launch_dependents();
+  griddep_wait();
+  if (!find_tile<M>(p, tile, s_token, nullptr, group, count, bad)) return;
+  float scale;
+  const uint32_t rank = adapter(p, group, scale, bad);
+  if (rank == 0) return;
+  const uint64_t cols = p.s.cols;
+  const T* a = static_cast<const T*>(p.s.a) + static_cast<uint64_t>(group) * p.s.max_rank * cols;
+  const T* x = static_cast<const T*>(p.x);
+  const uint32_t chunks = static_cast<uint32_t>((cols + kShrinkCols - 1) / kShrinkCols);
+  const uint32_t c0 = static_cast<uint64_t>(chunks) * split / p.splits, c1 = static_cast<uint64_t>(chunks) * (split + 1) / p.splits;
+  const uint32_t ring = smem_u32(sm) + 512;
+  auto load = [&](uint32_t chunk, uint32_t stage) {
+    const uint32_t to = ring + stage * kStage;
+#pragma unroll
+    for (uint32_t i = tid; i < (M + RP) * kPieces; i += kThreads) {
+      const uint32_t r = i / kPieces, c = i % kPieces;
+      const uint64_t col = static_cast<uint64_t>(chunk) * kShrinkCols + c * 8;
+      const int32_t t = r < M ? s_token[r] : static_cast<int32_t>(r - M);
+      const bool real = col < cols && (r < M ? t >= 0 : t < static_cast<int32_t>(rank));
+      const T* src = r < M ? x + (real ? t * p.x_stride + col : 0) : a + (real ? t * cols + col : 0);
+      cp_async16(to + r * (kShrinkCols * 2) + ((c ^ ((r & 1) << 2)) << 4), src, real ? 16u : 0u);
+    }
+  };
+  const uint32_t wm = warp % kWM, wn = warp / kWM;
+  float acc[kNT][4];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+  for (uint32_t s = 0; s + 1 < kShrinkStages; ++s) {
+    if (c0 + s < c1) load(c0 + s, s);
+    cp_async_commit();
+  }
+  uint32_t stage = 0;
+  for (uint32_t c = c0; c < c1; ++c) {
+    cp_async_wait<kShrinkStages - 2>();
+    __syncthreads();
+    const uint32_t ahead = c + kShrinkStages - 1;
+    if (ahead < c1) load(ahead, stage == 0 ? kShrinkStages - 1 : stage - 1);
+    cp_async_commit();
+    const uint32_t at = ring + stage * kStage;
+    stage = stage + 1 == kShrinkStages ? 0 : stage + 1;
+#pragma unroll
+    for (uint32_t h = 0; h < kShrinkCols / 32; ++h) {
+      const uint32_t swap = (g & 1) << 2, piece = ((h * 4 + q) ^ swap) << 4;
+      const uint4 u = lds128a(at + (wm * 16 + g) * (kShrinkCols * 2) + piece);
+      const uint4 v = lds128a(at + (wm * 16 + g + 8) * (kShrinkCols * 2) + piece);
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        const uint4 w = lds128a(at + (M + (wn * kNT + n) * 8 + g) * (kShrinkCols * 2) + piece);
+        Elem<T>::mma(acc[n], u.x, v.x, u.y, v.y, w.x, w.y);
+        Elem<T>::mma(acc[n], u.z, v.z, u.w, v.w, w.z, w.w);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  float* to = p.inner + (static_cast<uint64_t>(split) * p.max_tiles + tile) * M * RP;
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float2*>(to + (wm * 16 + g + 8 * e) * RP + (wn * kNT + n) * 8 + q * 2) =
+          make_float2(acc[n][2 * e], acc[n][2 * e + 1]);
+}
+
+template <typename T, typename Y, int RP>
+struct ExpandSmem {
+  static constexpr int M = kTileRows<RP, sizeof(Y)>;
+  static constexpr uint32_t kToken = 0, kFactor = M * 4, kTermsAt = 2 * M * 4;
+  static constexpr uint32_t kRing = kTermsAt + kTerms<T, Y> * M * LoraShape<RP>::kPitch * 2;
+  static constexpr uint32_t kFit = (226 * 1024 - kRing) / (8 * Expand<T, Y, RP, M>::kStage);
+  static constexpr uint32_t kStages = kFit > 4 ? 4 : kFit;
+  static constexpr uint32_t kBytes = kRing + 8 * kStages * Expand<T, Y, RP, M>::kStage;
+  static_assert(kStages >= 2, "a ring has two stages at least");
+};
+
+// y = base + scale B t for the tiles of a planned call: the steps of 32 outputs of all tiles in order
+// are dealt to the CTAs (one an SM) in equal contiguous ranges.  At each tile's start the warps sum
+// the tile's t over the column ranges in their order and split it into terms, while the ring's
+// first copies of B and base are under way.
+// Bound by the bytes of base and y.
+template <typename T, typename Y, int RP>
+__global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+  using S = LoraShape<RP>;
+  using L = ExpandSmem<T, Y, RP>;
+  constexpr int M = L::M, kN = kTerms<T, Y>, kPer = (RP + 31) / 32, kRowsEach = M / 8;
+  extern __shared__ __align__(128) uint8_t sm[];
+  int32_t* s_token = reinterpret_cast<int32_t*>(sm + L::kToken);
+  float* s_factor = reinterpret_cast<float*>(sm + L::kFactor);
+  T* s_terms = reinterpret_cast<T*>(sm + L::kTermsAt);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t bad = 0;
+  griddep_wait();
+  const uint32_t steps = static_cast<uint32_t>((p.s.rows + 31) / 32);
+  const uint64_t units = static_cast<uint64_t>(*p.tile_count) * steps;
+  uint64_t u = units * blockIdx.x / gridDim.x;
+  const uint64_t u1 = units * (blockIdx.x + 1) / gridDim.x;
+  while (u < u1) {
+    const uint32_t tile = static_cast<uint32_t>(u / steps), first = static_cast<uint32_t>(u - static_cast<uint64_t>(tile) * steps);
+    const uint32_t end = static_cast<uint32_t>(u1 - u < steps - first ? first + (u1 - u) : steps);
+    u += end - first;
+    __syncthreads();  // the last tile's terms and tokens have been read
+    uint32_t group, count;
+    find_tile<M>(p, tile, s_token, nullptr, group, count, bad);
+    float scale;
+    const uint32_t rank = adapter(p, group, scale, bad);
+    Expand<T, Y, RP, M> x2;
+    x2.prepare(p, group, rank, count, s_token, smem_u32(sm) + L::kRing + warp * L::kStages * Expand<T, Y, RP, M>::kStage, L::kStages);
+    x2.start(first + warp, end);
+    if (rank != 0) {
+      float v[kRowsEach][kPer];
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[r][i] = 0.0f;
+      const float* from = p.inner + (static_cast<uint64_t>(tile) * M + warp * kRowsEach) * RP + lane;
+#pragma unroll 2
+      for (uint32_t sp = 0; sp < p.splits; ++sp, from += static_cast<uint64_t>(p.max_tiles) * M * RP)
+#pragma unroll
+        for (int r = 0; r < kRowsEach; ++r)
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            if (i * 32 + lane < rank) v[r][i] += from[r * RP + i * 32];
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r) {
+        const uint32_t row = warp * kRowsEach + r;
+        const float f = split_row<T, RP, kN>(v[r], lane, scale, [&](int k, uint32_t x, uint16_t bits) {
+          reinterpret_cast<uint16_t*>(s_terms)[(k * M + row) * S::kPitch + x] = bits;
+        });
+        if (lane == 0) s_factor[row] = f;
+      }
+    }
+    __syncthreads();
+    x2.run(first + warp, end, s_terms, s_factor);
+  }
+  if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
 }
 
 // Groups the tokens by adapter: counts, offsets, then each token to its group's next place.  The
@@ -482,19 +772,37 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
   if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
 }
 
+uint32_t padded_rank(uint32_t r) { return r <= 16 ? 16u : r <= 32 ? 32u : r <= 64 ? 64u : 128u; }
+
 struct Layout {
-  uint64_t tiles, order, total;
-  uint32_t max_tiles;
+  uint64_t tiles, order, inner, total;
+  uint32_t max_tiles, splits;
 };
 
+// tile_rows 16: the tiles of lora_kernel, which keeps t to itself.
 Layout layout(const hqb_lora_set* s, uint32_t tokens, uint32_t tile_rows) {
   Layout l{};
   // every group may end in a partly filled tile
   const uint64_t groups = static_cast<uint64_t>(s->adapters) + 1;
   l.max_tiles = static_cast<uint32_t>(tokens / tile_rows + (groups < tokens ? groups : tokens));
+  // column ranges: two CTAs an SM at about the usual tiles, 256 columns a range at least
+  const uint32_t usual = tokens / tile_rows + 1;
+  uint32_t splits = usual < 296 ? 296 / usual : 1;
+  const uint64_t most = (s->cols + 255) / 256;
+  splits = splits > most ? static_cast<uint32_t>(most) : splits;
+  const uint32_t few = groups >= 512 ? 1u : static_cast<uint32_t>(512 / groups);
+  splits = splits > few ? few : splits;
+  l.splits = splits > 16 ? 16 : splits;
   l.tiles = 512;
   l.order = l.tiles + round_up(static_cast<uint64_t>(l.max_tiles) * sizeof(LoraTile), 256);
-  l.total = l.order + round_up(static_cast<uint64_t>(tokens) * 4, 256);
+  l.inner = l.order + round_up(static_cast<uint64_t>(tokens) * 4, 256);
+  l.total = l.inner;
+  if (tile_rows != 16) {
+    // splits * max_tiles at most: splits * (tokens / tile_rows) <= 296 where splits > 1, and splits *
+    // groups <= max(512, groups).  Room for that, so that what a call needs never shrinks with its tokens.
+    const uint64_t cut = 296 + (groups > 512 ? groups : 512), tiles = cut > l.max_tiles ? cut : l.max_tiles;
+    l.total += round_up(tiles * tile_rows * padded_rank(s->max_rank) * 4, 256);
+  }
   return l;
 }
 
@@ -505,44 +813,70 @@ bool set_ok(const hqb_lora_set* s) {
   return s->dtype == HQB_F16 || s->dtype == HQB_BF16;
 }
 
-template <typename T, typename Y, int RP, int M, bool VEC>
-cudaError_t launch_lora(const LoraParams& p, uint32_t tiles, cudaStream_t st) {
-  static DeviceOnce once;
-  constexpr uint32_t smem = kLoraSmem<T, Y, RP, M>;
-  const void* f = reinterpret_cast<const void*>(lora_kernel<T, Y, RP, M, VEC>);
-  const cudaError_t e = allow_dynamic_smem(once, f, smem);
+// One launch with up to `smem` bytes, as a cluster of `cluster` CTAs, and as a programmatic dependent
+// of the kernel before it where `after` (that kernel is this call's own).
+template <typename K>
+cudaError_t launch(K kernel, DeviceOnce& once, uint32_t grid, uint32_t smem, uint32_t cluster, bool after, const LoraParams& p,
+                   cudaStream_t st) {
+  const cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles * kCluster);
+  cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2]{};
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = kCluster;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = cluster;
+    at[cfg.numAttrs].val.clusterDim.y = 1;
+    at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (after) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = p.planned ? 2 : 1;  // a planned call follows its own plan kernel
-  return cudaLaunchKernelEx(&cfg, lora_kernel<T, Y, RP, M, VEC>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T, typename Y, int RP, bool VEC>
+cudaError_t launch_tile(const LoraParams& p, uint32_t tiles, cudaStream_t st) {
+  static DeviceOnce once;
+  return launch(lora_kernel<T, Y, RP, VEC>, once, tiles * kCluster, LoraSmem<T, Y, RP>::kBytes, kCluster, p.planned != 0, p, st);
+}
+
+template <typename T, typename Y, int RP>
+cudaError_t launch_rank(const LoraParams& p, uint32_t tiles, int sms, cudaStream_t st) {
+  if (!p.planned) return launch_tile<T, Y, RP, true>(p, tiles, st);
+  static DeviceOnce once_shrink, once_expand;
+  constexpr int M = kTileRows<RP, sizeof(Y)>;
+  const cudaError_t e = launch(lora_shrink_kernel<T, RP, M>, once_shrink, tiles * p.splits, kShrinkSmem<RP, M>, 1, true, p, st);
+  if (e != cudaSuccess) return e;
+  return launch(lora_expand_kernel<T, Y, RP>, once_expand, static_cast<uint32_t>(sms), ExpandSmem<T, Y, RP>::kBytes, 1, true, p, st);
 }
 
 template <typename T, typename Y>
-cudaError_t launch_rank(const LoraParams& p, bool vec, uint32_t tiles, cudaStream_t st) {
-  if (!vec) return launch_lora<T, Y, 128, 16, false>(p, tiles, st);
-  const uint32_t r = p.s.max_rank;
-  if (p.tile_rows == 16) {
-    if (r <= 16) return launch_lora<T, Y, 16, 16, true>(p, tiles, st);
-    if (r <= 32) return launch_lora<T, Y, 32, 16, true>(p, tiles, st);
-    if (r <= 64) return launch_lora<T, Y, 64, 16, true>(p, tiles, st);
-    return launch_lora<T, Y, 128, 16, true>(p, tiles, st);
+cudaError_t launch_lora(const LoraParams& p, bool vec, uint32_t tiles, int sms, cudaStream_t st) {
+  if (!vec) return launch_tile<T, Y, 128, false>(p, tiles, st);
+  switch (padded_rank(p.s.max_rank)) {
+    case 16: return launch_rank<T, Y, 16>(p, tiles, sms, st);
+    case 32: return launch_rank<T, Y, 32>(p, tiles, sms, st);
+    case 64: return launch_rank<T, Y, 64>(p, tiles, sms, st);
+    default: return launch_rank<T, Y, 128>(p, tiles, sms, st);
   }
-  if (r <= 16) return launch_lora<T, Y, 16, 64, true>(p, tiles, st);
-  if (r <= 32) return launch_lora<T, Y, 32, 64, true>(p, tiles, st);
-  if (r <= 64) return launch_lora<T, Y, 64, 64, true>(p, tiles, st);
-  return launch_lora<T, Y, 128, 64, true>(p, tiles, st);
+}
+
+uint32_t planned_rows(const hqb_lora_set* s, bool vec, bool wide_y) {
+  if (!vec) return 16;
+  switch (padded_rank(s->max_rank)) {
+    case 16: return wide_y ? kTileRows<16, 4> : kTileRows<16, 2>;
+    case 32: return wide_y ? kTileRows<32, 4> : kTileRows<32, 2>;
+    case 64: return wide_y ? kTileRows<64, 4> : kTileRows<64, 2>;
+    default: return wide_y ? kTileRows<128, 4> : kTileRows<128, 2>;
+  }
 }
 
 }  // namespace
@@ -555,7 +889,14 @@ extern "C" {
 HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* s, uint32_t tokens, int device) {
   (void)device;
   if (!set_ok(s) || tokens > 0x7FFFFFFFu) return 0;
-  return tokens <= kDirectTokens ? 256 : layout(s, tokens, 16).total;
+  if (tokens <= kDirectTokens) return 256;
+  // the call's kernels depend on its alignment and output type too: room for any
+  uint64_t most = layout(s, tokens, 16).total;
+  for (const bool wide_y : {false, true}) {
+    const uint64_t n = layout(s, tokens, planned_rows(s, true, wide_y)).total;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, const int32_t* ids, uint32_t tokens,
@@ -592,7 +933,7 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
   p.tokens = tokens;
   p.planned = tokens > kDirectTokens ? 1u : 0u;
   p.in_place = base == y ? 1u : 0u;
-  p.tile_rows = vec && p.planned ? 64u : 16u;
+  p.tile_rows = p.planned ? planned_rows(s, vec, y_dtype == HQB_F32) : 16u;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.error = reinterpret_cast<int*>(ws);
   cudaStream_t st = as_stream(stream);
@@ -602,8 +943,11 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
     p.tile_count = reinterpret_cast<uint32_t*>(ws + 256);
     p.tiles = reinterpret_cast<LoraTile*>(ws + l.tiles);
     p.order = reinterpret_cast<uint32_t*>(ws + l.order);
+    p.inner = reinterpret_cast<float*>(ws + l.inner);
+    p.max_tiles = l.max_tiles;
+    p.splits = l.splits;
     tiles = l.max_tiles;
-    if (tiles > 0x7FFFFFFFu / kCluster) return HQB_ERR_UNSUPPORTED;
+    if (tiles > 0x7FFFFFFFu / 16) return HQB_ERR_UNSUPPORTED;
     static DeviceOnce once;
     const cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(lora_plan_kernel), (kMaxAdapters + 1) * 4);
     if (e != cudaSuccess) return e;
@@ -611,10 +955,16 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
     const cudaError_t e2 = cudaGetLastError();
     if (e2 != cudaSuccess) return e2;
   }
+  int device = 0;
+  const cudaError_t e3 = cudaGetDevice(&device);
+  if (e3 != cudaSuccess) return e3;
+  const int sms = device_sm_count(device);
+  if (sms <= 0) return cudaErrorInvalidDevice;
   if (s->dtype == HQB_F16)
-    return y_dtype == HQB_F32 ? launch_rank<__half, float>(p, vec, tiles, st) : launch_rank<__half, __half>(p, vec, tiles, st);
-  return y_dtype == HQB_F32 ? launch_rank<__nv_bfloat16, float>(p, vec, tiles, st)
-                            : launch_rank<__nv_bfloat16, __nv_bfloat16>(p, vec, tiles, st);
+    return y_dtype == HQB_F32 ? launch_lora<__half, float>(p, vec, tiles, sms, st)
+                              : launch_lora<__half, __half>(p, vec, tiles, sms, st);
+  return y_dtype == HQB_F32 ? launch_lora<__nv_bfloat16, float>(p, vec, tiles, sms, st)
+                            : launch_lora<__nv_bfloat16, __nv_bfloat16>(p, vec, tiles, sms, st);
 }
 
 }  // extern "C"

@@ -58,10 +58,25 @@ struct Elem<__nv_bfloat16> {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t fill) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fill) : "memory");
 }
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, uint32_t fill) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(fill) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Waits for all but the last n groups, n a (uniform) run-time value up to 5.
+__device__ __forceinline__ void cp_async_wait_dynamic(uint32_t n) {
+  switch (n) {
+    case 1: cp_async_wait<1>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 3: cp_async_wait<3>(); break;
+    case 4: cp_async_wait<4>(); break;
+    case 5: cp_async_wait<5>(); break;
+    default: cp_async_wait<0>(); break;
+  }
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t a, uint32_t (&r)[4]) {
