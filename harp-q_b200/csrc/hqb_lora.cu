@@ -18,6 +18,11 @@ namespace {
 constexpr uint32_t kCluster = 8;         // CTAs that share a tile: the portable cluster size
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kDirectTokens = 256;  // up to here every cluster finds its own tile
+// A planned call keeps to lora_kernel up to this many tokens * padded rank.  B200, us, lora_kernel /
+// shrink + expand, FP16 or BF16, 8 adapters: rank 16, 4096 x 4096: 1024 tokens 18.4 / 24.0, 2048 tokens
+// 28.7 / 27.5; rank 24, 1024 x 8192: 777 tokens 18.0 / 27.2; rank 64, 11008 x 4096: 300 tokens 16.8 /
+// 24.1, 777 tokens 41.5 / 32.8.
+constexpr uint64_t kClusterWork = 32768;
 constexpr uint32_t kMaxAdapters = 16383;
 
 struct LoraTile {
@@ -850,7 +855,7 @@ cudaError_t launch_tile(const LoraParams& p, uint32_t tiles, cudaStream_t st) {
 
 template <typename T, typename Y, int RP>
 cudaError_t launch_rank(const LoraParams& p, uint32_t tiles, int sms, cudaStream_t st) {
-  if (!p.planned) return launch_tile<T, Y, RP, true>(p, tiles, st);
+  if (p.tile_rows == 16) return launch_tile<T, Y, RP, true>(p, tiles, st);
   static DeviceOnce once_shrink, once_expand;
   constexpr int M = kTileRows<RP, sizeof(Y)>;
   const cudaError_t e = launch(lora_shrink_kernel<T, RP, M>, once_shrink, tiles * p.splits, kShrinkSmem<RP, M>, 1, true, p, st);
@@ -869,8 +874,8 @@ cudaError_t launch_lora(const LoraParams& p, bool vec, uint32_t tiles, int sms, 
   }
 }
 
-uint32_t planned_rows(const hqb_lora_set* s, bool vec, bool wide_y) {
-  if (!vec) return 16;
+uint32_t planned_rows(const hqb_lora_set* s, uint32_t tokens, bool vec, bool wide_y) {
+  if (!vec || static_cast<uint64_t>(tokens) * padded_rank(s->max_rank) <= kClusterWork) return 16;
   switch (padded_rank(s->max_rank)) {
     case 16: return wide_y ? kTileRows<16, 4> : kTileRows<16, 2>;
     case 32: return wide_y ? kTileRows<32, 4> : kTileRows<32, 2>;
@@ -893,7 +898,7 @@ HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* s, uint32_t tokens
   // the call's kernels depend on its alignment and output type too: room for any
   uint64_t most = layout(s, tokens, 16).total;
   for (const bool wide_y : {false, true}) {
-    const uint64_t n = layout(s, tokens, planned_rows(s, true, wide_y)).total;
+    const uint64_t n = layout(s, tokens, planned_rows(s, tokens, true, wide_y)).total;
     most = n > most ? n : most;
   }
   return most;
@@ -933,7 +938,7 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
   p.tokens = tokens;
   p.planned = tokens > kDirectTokens ? 1u : 0u;
   p.in_place = base == y ? 1u : 0u;
-  p.tile_rows = p.planned ? planned_rows(s, vec, y_dtype == HQB_F32) : 16u;
+  p.tile_rows = p.planned ? planned_rows(s, tokens, vec, y_dtype == HQB_F32) : 16u;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.error = reinterpret_cast<int*>(ws);
   cudaStream_t st = as_stream(stream);
