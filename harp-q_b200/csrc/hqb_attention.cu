@@ -11,27 +11,27 @@
 namespace hqb {
 namespace {
 
-constexpr uint32_t kRowsThreads = 128;
-constexpr uint32_t kRowsWarps = kRowsThreads / 32;
 constexpr uint32_t kKeyBlock = 64;
 constexpr uint32_t kChunk = 16;  // keys a warp takes at once
 constexpr uint32_t kStages = 3;  // chunks of a warp's ring
 
-template <int DP>
+template <int DP, int kRowsWarps>
 constexpr uint32_t kRowsSmem = kRowsWarps * kStages * 2 * kChunk * DP * 2;
 
 // Mathematics: the softmax over the keys in one pass.  A warp keeps, per row, the running
 // maximum m of t = scale*log2(e) * q.k, the sum l of 2^(t - m) and the sums O of 2^(t - m) v;
 // a larger maximum m' rescales l and O by 2^(m - m').  Warps, and CTAs, that saw different keys
 // are joined the same way.
-// Split: the four warps of a CTA take the segment's 16-key chunks in turn, each with its own
+// Split: the warps of a CTA take the segment's 16-key chunks in turn, each with its own
 // ring of asynchronous copies, so the loop has no CTA barrier and keeps 2 chunks (16 KB at 128
 // dimensions) a warp in flight; the warps are joined once per segment.  Rows: the group's heads
 // of all nodes share the keys, so a key is read once per 16 rows.
+// Warps: four, two CTAs an SM, so that one CTA's ends of segments lie under the other's copies; eight
+// where items are not cut (up to 512 keys: every copy is then in flight at once).
 // Bound by HBM at 16 rows: 32 MMAs a chunk are about 310 cycles of one of the four tensor pipes
 // a chunk against 1400 cycles an SM needs to fetch four chunks.
-template <typename T, int DP, bool VEC>
-__global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __grid_constant__ AttnParams p) {
+template <typename T, int DP, bool VEC, int kRowsWarps>
+__global__ void __launch_bounds__(kRowsWarps * 32) attention_rows_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t sm[];
   constexpr uint32_t kRowBytes = DP * 2, kTileBytes = kChunk * kRowBytes, kStageBytes = 2 * kTileBytes;
   constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
     // join the warps: sums in shared memory over the (drained) rings, [warp][16][DP + 2]
     __syncthreads();
     constexpr uint32_t kPitch = DP + 2;
-    static_assert(kRowsWarps * 16 * kPitch * 4 <= kRowsSmem<DP>, "the join area fits the rings");
+    static_assert(kRowsWarps * 16 * kPitch * 4 <= kRowsSmem<DP, kRowsWarps>, "the join area fits the rings");
     float* joint = reinterpret_cast<float*>(sm);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
     }
     __syncthreads();
     {
-      const uint32_t row = threadIdx.x >> 3, part = threadIdx.x & 7;  // 8 threads a row
+      constexpr uint32_t kEach = kRowsWarps * 2;  // threads a row
+      const uint32_t row = threadIdx.x / kEach, part = threadIdx.x % kEach;
       float mm = -INFINITY, ll = 0.0f, f[kRowsWarps];
 #pragma unroll
       for (uint32_t x = 0; x < kRowsWarps; ++x) mm = fmaxf(mm, joint[(x * 16 + row) * kPitch + DP]);
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(const __gr
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
         T* out = static_cast<T*>(p.a.out) + (q.start + nd) * p.a.out_token_stride + h * p.a.out_head_stride;
         float* keep = part_sums(p, blockIdx.x, w.b0 == 0 ? 1u : 0u) + row * 4;
-        for (uint32_t d = part * 2; d < DP; d += 16) {
+        for (uint32_t d = part * 2; d < DP; d += kEach * 2) {
           float2 o = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (uint32_t x = 0; x < kRowsWarps; ++x) {
@@ -498,14 +499,22 @@ Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem,
   return s;
 }
 
+template <typename T, int DP, bool VEC, int kRowsWarps>
+cudaError_t launch_warps(const AttnParams& p, cudaStream_t st) {
+  static DeviceOnce once;
+  constexpr uint32_t smem = kRowsSmem<DP, kRowsWarps>;
+  const cudaError_t e =
+      allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_rows_kernel<T, DP, VEC, kRowsWarps>), smem);
+  if (e != cudaSuccess) return e;
+  attention_rows_kernel<T, DP, VEC, kRowsWarps><<<p.grid, kRowsWarps * 32, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T, int DP, bool VEC>
 cudaError_t launch_rows(const AttnParams& p, cudaStream_t st) {
-  static DeviceOnce once;
-  const cudaError_t e =
-      allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_rows_kernel<T, DP, VEC>), kRowsSmem<DP>);
-  if (e != cudaSuccess) return e;
-  attention_rows_kernel<T, DP, VEC><<<p.grid, kRowsThreads, kRowsSmem<DP>, st>>>(p);
-  return cudaGetLastError();
+  if constexpr (DP <= 128)
+    if (p.whole) return launch_warps<T, DP, VEC, 8>(p, st);
+  return launch_warps<T, DP, VEC, 4>(p, st);
 }
 
 template <typename T, bool VEC>

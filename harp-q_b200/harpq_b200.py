@@ -601,20 +601,21 @@ def _raw_stream(stream, index: int) -> int:
     return _stream(stream) or 0
 
 
-def _ints(name: str, t: torch.Tensor, n: int, device) -> int:
-    """Checks an int32 index tensor of n elements and gives its address."""
-    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on {device}, "
+def _ints(name: str, t: torch.Tensor, n: int, device: int) -> int:
+    """Checks an int32 index tensor of n elements on GPU `device` and gives its address."""
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on GPU {device}, "
                          f"got {list(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _table(name: str, t: torch.Tensor, rows: int, device) -> int:
+def _table(name: str, t: torch.Tensor, rows: int, device: int) -> int:
     """Checks an int32 matrix of `rows` rows and gives its columns."""
-    if t.dim() != 2 or t.shape[0] != rows:
-        raise ValueError(f"{name} must have {rows} rows, got {list(t.shape)}")
-    _ints(name, t, t.numel(), device)
-    return t.shape[1]
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows, got {list(shape)}")
+    _ints(name, t, rows * shape[1], device)
+    return shape[1]
 
 
 class PagePlan:
@@ -649,7 +650,7 @@ class PagePlan:
         new tokens pages and slots, writing new columns into it; parents [at least the step's
         tokens] gives tree positions and masks.  held and free_head are the counts before the
         step (a previous plan's, not this one's buffers)."""
-        n, device = self.batch, self.device
+        n, device = self.batch, self._index
         starts, requests, positions, slots, held_out, head_out, flags, mask = self._out
         ctx = _ints("context_lens", context_lens, n, device)
         new = _ints("new_lens", new_lens, n, device)
@@ -705,13 +706,13 @@ class PagedCache:
         """Writes rows of k and v [tokens, heads, dim] (FP16, BF16 or FP32) into the cache's slots
         [count]: row rows[i], or i, goes to slots[i]; negative ones are skipped.  flags collects
         HQB_DEVERR_* bits."""
-        shape, strides, device = k.shape, k.stride(), self.device
+        shape, strides, device = k.shape, k.stride(), self._index
         if len(shape) != 3 or shape[1] != self.heads or shape[2] != self.dim or v.shape != shape:
             raise ValueError(f"k and v must be [tokens, {self.heads}, {self.dim}]")
         kind = _ROW_DTYPES.get(k.dtype)
         if kind is None or v.dtype is not k.dtype:
             raise TypeError("k and v must share a type: float16, bfloat16 or float32")
-        if v.stride() != strides or (strides[2] != 1 and self.dim > 1) or k.device != device or v.device != device:
+        if v.stride() != strides or (strides[2] != 1 and self.dim > 1) or k.get_device() != device or v.get_device() != device:
             raise ValueError("k and v must share strides (adjacent elements within a head) and the cache's device")
         n = slots.numel()
         to = _ints("slots", slots, n, device)
@@ -748,20 +749,22 @@ class TreeAttention:
         if need == 0:
             raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
         self.ws = Workspace(need, cache.device)
-        self._ws = self.ws.ptr()
+        self._ws, self._ws_bytes = self.ws.ptr(), self.ws.nbytes
         self._args = ctypes.create_string_buffer(_ATTENTION.size)
         self._at = ctypes.addressof(self._args)
         self._call = lib().hqb_tree_attention
 
-    def _rows(self, name: str, t: torch.Tensor, tokens: int, heads: int) -> tuple:
-        c, shape, strides = self.cache, t.shape, t.stride()
-        if len(shape) != 3 or shape[0] != tokens or shape[1] != heads or shape[2] != c.dim:
-            raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}], got {list(shape)}")
-        if t.dtype is not c.dtype or t.device != c.device:
-            raise TypeError(f"{name} must have the cache's type and device")
-        if strides[2] != 1 and c.dim > 1:
-            raise ValueError(f"{name}: a head's elements must be adjacent")
-        return strides
+    def _refuse(self, tokens: int, q, k, v, out) -> None:
+        """Says which of the row tensors does not fit."""
+        c = self.cache
+        for name, t, heads in (("q", q, self.q_heads), ("k", k, c.heads), ("v", v, c.heads), ("out", out, self.q_heads)):
+            if tuple(t.shape) != (tokens, heads, c.dim):
+                raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}], got {list(t.shape)}")
+            if t.dtype is not c.dtype or t.get_device() != c._index:
+                raise TypeError(f"{name} must have the cache's type and device")
+            if t.stride(2) != 1 and c.dim > 1:
+                raise ValueError(f"{name}: a head's elements must be adjacent")
+        raise ValueError("k and v must share strides")
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tables: torch.Tensor,
                  context_lens: torch.Tensor, starts: torch.Tensor, mask: torch.Tensor | None = None,
@@ -773,15 +776,18 @@ class TreeAttention:
         [tokens, words]: bit j of a node's row shows it node j of its request (None: the nodes
         up to itself).  scale None: dim ** -0.5.  lse [tokens, q_heads] FP32 gets the logarithm of
         the sum of weights."""
-        c, device = self.cache, self.cache.device
+        c = self.cache
+        device, dim, dtype = c._index, c.dim, c.dtype
         tokens, requests = q.shape[0], context_lens.numel()
         if out is None:
-            out = torch.empty(tokens, self.q_heads, c.dim, dtype=c.dtype, device=device)
-        qs = self._rows("q", q, tokens, self.q_heads)
-        ks = self._rows("k", k, tokens, c.heads)
-        if self._rows("v", v, tokens, c.heads) != ks:
-            raise ValueError("k and v must share strides")
-        os = self._rows("out", out, tokens, self.q_heads)
+            out = torch.empty(tokens, self.q_heads, dim, dtype=dtype, device=c.device)
+        rows, news = (tokens, self.q_heads, dim), (tokens, c.heads, dim)
+        qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+        if (q.shape != rows or out.shape != rows or k.shape != news or v.shape != news or q.dtype is not dtype
+                or k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or ks != vs
+                or q.get_device() != device or k.get_device() != device or v.get_device() != device
+                or out.get_device() != device or (dim > 1 and not qs[2] == ks[2] == os[2] == 1)):
+            self._refuse(tokens, q, k, v, out)
         if requests > self.requests or tokens > self.tokens:
             raise ValueError(f"built for {self.requests} requests and {self.tokens} tokens, got {requests} and {tokens}")
         columns = _table("tables", tables, requests, device)
@@ -795,14 +801,14 @@ class TreeAttention:
             bits = mask.data_ptr()
         sums = 0
         if lse is not None:
-            if (lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape[0] != tokens or lse.shape[1] != self.q_heads
-                    or not lse.is_contiguous() or lse.device != device):
+            if (lse.dtype is not torch.float32 or lse.shape != rows[:2] or not lse.is_contiguous()
+                    or lse.get_device() != device):
                 raise ValueError(f"lse must be a contiguous float32 [{tokens}, {self.q_heads}] tensor")
             sums = lse.data_ptr()
         _ATTENTION.pack_into(self._args, 0, requests, tokens, self.max_new, self.max_context, self.q_heads, columns, words,
-                             c.dim ** -0.5 if scale is None else scale, first, ctx, tables.data_ptr(), bits, q.data_ptr(),
+                             dim ** -0.5 if scale is None else scale, first, ctx, tables.data_ptr(), bits, q.data_ptr(),
                              k.data_ptr(), v.data_ptr(), out.data_ptr(), sums, qs[0], qs[1], ks[0], ks[1], os[0], os[1])
-        status = self._call(c._at, self._at, self._ws, self.ws.nbytes, _raw_stream(stream, c._index))
+        status = self._call(c._at, self._at, self._ws, self._ws_bytes, _raw_stream(stream, device))
         if status:
             check(status, "hqb_tree_attention")
         return out
@@ -829,7 +835,7 @@ class LoraSet:
         if not 1 <= self.max_rank <= MAX_RANK:
             raise ValueError(f"max_rank must be 1..{MAX_RANK}")
         if ranks is not None:
-            _ints("ranks", ranks, self.adapters, a.device)
+            _ints("ranks", ranks, self.adapters, _device_index(a.device))
         if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (self.adapters,)
                                    or not scales.is_contiguous() or scales.device != a.device):
             raise ValueError(f"scales must be a contiguous float32 [{self.adapters}] tensor")
@@ -858,7 +864,7 @@ class LoraSet:
 
     def _out(self, name: str, t: torch.Tensor, tokens: int, kind) -> int:
         shape, strides = t.shape, t.stride()
-        if len(shape) != 2 or shape[0] != tokens or shape[1] != self.rows or t.dtype is not kind or t.device != self.device:
+        if shape != (tokens, self.rows) or t.dtype is not kind or t.get_device() != self._index:
             raise ValueError(f"{name} must be [{tokens}, {self.rows}] {kind} on {self.device}")
         if (strides[1] != 1 and self.rows > 1) or (strides[0] < self.rows and tokens > 1):
             raise ValueError(f"{name}: a row's elements must be adjacent, and rows must not overlap")
@@ -871,7 +877,7 @@ class LoraSet:
         x [tokens, cols]; base [tokens, rows] (None: zeros) and the result share a type, the
         set's or FP32.  out=base adds in place, e.g. to the output of a projection's gemv()."""
         shape, strides = x.shape, x.stride()
-        if len(shape) != 2 or shape[1] != self.cols or x.dtype is not self.dtype or x.device != self.device:
+        if len(shape) != 2 or shape[1] != self.cols or x.dtype is not self.dtype or x.get_device() != self._index:
             raise ValueError(f"x must be [tokens, {self.cols}] {self.dtype} on {self.device}")
         tokens = shape[0]
         if (strides[1] != 1 and self.cols > 1) or (strides[0] < self.cols and tokens > 1):
@@ -882,7 +888,7 @@ class LoraSet:
         kind = out.dtype
         if kind is not self.dtype and kind is not torch.float32:
             raise TypeError("the result must have the set's type or float32")
-        which = _ints("ids", ids, tokens, self.device)
+        which = _ints("ids", ids, tokens, self._index)
         y_stride, base_stride, base_at = self._out("out", out, tokens, kind), 0, 0
         if base is not None:
             base_stride, base_at = self._out("base", base, tokens, kind), base.data_ptr()
