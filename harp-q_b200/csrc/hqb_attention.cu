@@ -369,6 +369,7 @@ template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
   __shared__ __align__(16) T turned[kJoinRows][HQB_MAX_HEAD_DIM + 8];
   const uint32_t first = blockIdx.x;
+  griddep_launch_dependents();
   griddep_wait();
   const Split q = p.splits[first];
   if (q.last == first) return;
@@ -506,8 +507,7 @@ cudaError_t launch_warps(const AttnParams& p, cudaStream_t st) {
   const cudaError_t e =
       allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_rows_kernel<T, DP, VEC, kRowsWarps>), smem);
   if (e != cudaSuccess) return e;
-  attention_rows_kernel<T, DP, VEC, kRowsWarps><<<p.grid, kRowsWarps * 32, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(attention_rows_kernel<T, DP, VEC, kRowsWarps>, dim3(p.grid), kRowsWarps * 32, smem, 1, st, p);
 }
 
 template <typename T, int DP, bool VEC>
@@ -528,17 +528,8 @@ template <typename T>
 cudaError_t launch_attention(const AttnParams& p, bool vec, bool tmem, cudaStream_t st) {
   cudaError_t e = tmem ? launch_attention_tmem<T>(p, st) : vec ? launch_dim<T, true>(p, st) : launch_dim<T, false>(p, st);
   if (e != cudaSuccess || p.whole) return e;
-  cudaLaunchConfig_t cfg{};
   const uint32_t rows = p.rows < p.a.max_new * p.group ? p.rows : p.a.max_new * p.group;
-  cfg.gridDim = dim3(p.grid, (rows + kJoinRows - 1) / kJoinRows);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T>, p);
+  return launch_dependent(attention_join_kernel<T>, dim3(p.grid, (rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, 1, st, p);
 }
 
 }  // namespace

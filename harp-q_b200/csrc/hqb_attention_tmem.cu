@@ -685,8 +685,7 @@ cudaError_t launch(const AttnParams& p, const Maps& maps, cudaStream_t st) {
   static_assert(smem <= 232448, "one CTA's shared memory");
   const cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_tmem_kernel<T, DP>), smem);
   if (e != cudaSuccess) return e;
-  attention_tmem_kernel<T, DP><<<p.grid, kTmemThreads, smem, st>>>(p, maps);
-  return cudaGetLastError();
+  return launch_dependent(attention_tmem_kernel<T, DP>, dim3(p.grid), kTmemThreads, smem, 1, st, p, maps);
 }
 
 }  // namespace

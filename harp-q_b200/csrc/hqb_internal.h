@@ -41,6 +41,29 @@ inline cudaError_t allow_dynamic_smem(DeviceOnce& done, const void* kernel, uint
   return e;
 }
 
+// Launches a kernel as a programmatic dependent of the one before it in the stream: its CTAs may
+// start while that one ends.  Only for kernels that run griddepcontrol.wait before their first
+// access to global memory (in at least one thread of a grid that would otherwise end early).
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t smem, uint32_t cluster,
+                             cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // The int8-limb GEMV on the reference's raw layout (hqb_raw_i8.cu): 128x128 tiles,
 // group 128, prefix 1..4, batch one, FP32 x / y.  HQB_ERR_UNSUPPORTED (nothing
 // enqueued) when the geometry, alignment or shared-memory size rules it out.

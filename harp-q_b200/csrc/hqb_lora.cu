@@ -443,6 +443,7 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const uint32_t cta = cluster_rank(), tile = blockIdx.x / kCluster;
   uint32_t bad = 0, group, count;
+  griddep_launch_dependents();
   griddep_wait();
   if (!find_tile<M>(p, tile, s_token, s_info, group, count, bad)) return;
   float scale;
@@ -682,6 +683,7 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_cons
   T* s_terms = reinterpret_cast<T*>(sm + L::kTermsAt);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t bad = 0;
+  griddep_launch_dependents();
   griddep_wait();
   const uint32_t steps = static_cast<uint32_t>((p.s.rows + 31) / 32);
   const uint64_t units = static_cast<uint64_t>(*p.tile_count) * steps;
@@ -736,6 +738,7 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, groups = p.s.adapters + 1;
   uint32_t bad = 0;
   griddep_launch_dependents();
+  griddep_wait();
   for (uint32_t i = tid; i < groups; i += 1024) count[i] = 0;
   __syncthreads();
   for (uint32_t t = tid; t < p.tokens; t += 1024) atomicAdd(&count[group_of(p, t, bad)], 1u);
@@ -818,39 +821,18 @@ bool set_ok(const hqb_lora_set* s) {
   return s->dtype == HQB_F16 || s->dtype == HQB_BF16;
 }
 
-// One launch with up to `smem` bytes, as a cluster of `cluster` CTAs, and as a programmatic dependent
-// of the kernel before it where `after` (that kernel is this call's own).
+// One launch with `smem` bytes, as clusters of `cluster` CTAs.
 template <typename K>
-cudaError_t launch(K kernel, DeviceOnce& once, uint32_t grid, uint32_t smem, uint32_t cluster, bool after, const LoraParams& p,
+cudaError_t launch(K kernel, DeviceOnce& once, uint32_t grid, uint32_t smem, uint32_t cluster, const LoraParams& p,
                    cudaStream_t st) {
   const cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(kernel), smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2]{};
-  if (cluster > 1) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[cfg.numAttrs].val.clusterDim.x = cluster;
-    at[cfg.numAttrs].val.clusterDim.y = 1;
-    at[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (after) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  cfg.attrs = at;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return e != cudaSuccess ? e : launch_dependent(kernel, dim3(grid), kThreads, smem, cluster, st, p);
 }
 
 template <typename T, typename Y, int RP, bool VEC>
 cudaError_t launch_tile(const LoraParams& p, uint32_t tiles, cudaStream_t st) {
   static DeviceOnce once;
-  return launch(lora_kernel<T, Y, RP, VEC>, once, tiles * kCluster, LoraSmem<T, Y, RP>::kBytes, kCluster, p.planned != 0, p, st);
+  return launch(lora_kernel<T, Y, RP, VEC>, once, tiles * kCluster, LoraSmem<T, Y, RP>::kBytes, kCluster, p, st);
 }
 
 template <typename T, typename Y, int RP>
@@ -858,9 +840,9 @@ cudaError_t launch_rank(const LoraParams& p, uint32_t tiles, int sms, cudaStream
   if (p.tile_rows == 16) return launch_tile<T, Y, RP, true>(p, tiles, st);
   static DeviceOnce once_shrink, once_expand;
   constexpr int M = kTileRows<RP, sizeof(Y)>;
-  const cudaError_t e = launch(lora_shrink_kernel<T, RP, M>, once_shrink, tiles * p.splits, kShrinkSmem<RP, M>, 1, true, p, st);
+  const cudaError_t e = launch(lora_shrink_kernel<T, RP, M>, once_shrink, tiles * p.splits, kShrinkSmem<RP, M>, 1, p, st);
   if (e != cudaSuccess) return e;
-  return launch(lora_expand_kernel<T, Y, RP>, once_expand, static_cast<uint32_t>(sms), ExpandSmem<T, Y, RP>::kBytes, 1, true, p, st);
+  return launch(lora_expand_kernel<T, Y, RP>, once_expand, static_cast<uint32_t>(sms), ExpandSmem<T, Y, RP>::kBytes, 1, p, st);
 }
 
 template <typename T, typename Y>
@@ -954,11 +936,9 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
     tiles = l.max_tiles;
     if (tiles > 0x7FFFFFFFu / 16) return HQB_ERR_UNSUPPORTED;
     static DeviceOnce once;
-    const cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(lora_plan_kernel), (kMaxAdapters + 1) * 4);
+    cudaError_t e = allow_dynamic_smem(once, reinterpret_cast<const void*>(lora_plan_kernel), (kMaxAdapters + 1) * 4);
+    if (e == cudaSuccess) e = launch_dependent(lora_plan_kernel, dim3(1), 1024, (s->adapters + 1) * 4, 1, st, p);
     if (e != cudaSuccess) return e;
-    lora_plan_kernel<<<1, 1024, (s->adapters + 1) * 4, st>>>(p);
-    const cudaError_t e2 = cudaGetLastError();
-    if (e2 != cudaSuccess) return e2;
   }
   int device = 0;
   const cudaError_t e3 = cudaGetDevice(&device);

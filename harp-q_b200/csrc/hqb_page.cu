@@ -48,6 +48,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
   __shared__ uint64_t red[kPlanThreads / 32];
   __shared__ uint32_t s_start[kPlanThreads + 1], s_ctx[kPlanThreads], s_held[kPlanThreads], s_fresh[kPlanThreads];
   const uint32_t tid = threadIdx.x;
+  griddep_launch_dependents();
+  griddep_wait();
   const uint32_t t0 = min(a.token_capacity, blockIdx.x * per_cta), t1 = min(a.token_capacity, t0 + per_cta);
   const bool scribe = blockIdx.x == 0, paged = a.tables != nullptr;
   uint32_t bad = 0;
@@ -233,6 +235,8 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const __grid_constant
   const uint32_t pieces = p.dim / W, row_pieces = pieces * p.heads;
   const uint64_t total = static_cast<uint64_t>(p.count) * row_pieces;
   uint32_t bad = 0;
+  griddep_launch_dependents();
+  griddep_wait();
   for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
     const uint32_t entry = static_cast<uint32_t>(i / row_pieces);
     const uint32_t j = static_cast<uint32_t>(i - static_cast<uint64_t>(entry) * row_pieces);
@@ -289,9 +293,7 @@ cudaError_t launch_append(const AppendParams& p, bool wide, cudaStream_t st) {
   const uint64_t total = static_cast<uint64_t>(p.count) * p.heads * (wide ? p.dim / 8 : p.dim);
   const uint64_t blocks = (total + 255) / 256;
   const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
-  if (wide) cache_append_kernel<S, T, 8><<<grid, 256, 0, st>>>(p);
-  else cache_append_kernel<S, T, 1><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(wide ? cache_append_kernel<S, T, 8> : cache_append_kernel<S, T, 1>, dim3(grid), 256, 0, 1, st, p);
 }
 
 }  // namespace
@@ -332,8 +334,7 @@ HQB_API int hqb_page_plan(const hqb_page_plan_args* a, void* stream) {
   uint32_t grid = (a->token_capacity + kPlanThreads - 1) / kPlanThreads;
   grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
   const uint32_t per_cta = (a->token_capacity + grid - 1) / grid;
-  page_plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(*a, per_cta);
-  return cudaGetLastError();
+  return launch_dependent(page_plan_kernel, dim3(grid), kPlanThreads, 0, 1, as_stream(stream), *a, per_cta);
 }
 
 HQB_API int hqb_cache_append(const hqb_paged_cache* c, const void* k, const void* v, int dtype, uint64_t token_stride,
