@@ -682,9 +682,10 @@ class PagePlan:
 class PagedCache:
     """A paged cache over two device tensors k, v [pages, page_size, heads, dim] (FP16 or BF16;
     any strides with adjacent elements within a head, the same for both: a cache that stores
-    heads before tokens is passed as its transpose(1, 2))."""
+    heads before tokens is passed as its transpose(1, 2)).  flags [1] int32 collects the
+    HQB_DEVERR_* bits of append() (made here when not given)."""
 
-    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, flags: torch.Tensor | None = None):
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
             raise ValueError("k and v must be [pages, page_size, heads, dim] tensors of one shape, layout, type and device")
         if k.dtype not in _SERVING_DTYPES:
@@ -694,9 +695,9 @@ class PagedCache:
         self.k, self.v = k, v
         self.num_pages, self.page_size, self.heads, self.dim = k.shape
         self.dtype, self.device = k.dtype, k.device
-        self.flags = torch.zeros(1, dtype=torch.int32, device=k.device)
         self.c = PagedCacheC(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), _SERVING_DTYPES[k.dtype],
                              self.heads, self.dim, self.page_size, self.num_pages, 0)
+        self.flags = torch.zeros(1, dtype=torch.int32, device=k.device) if flags is None else flags
         self._at, self._flags = ctypes.addressof(self.c), self.flags.data_ptr()
         self._index = _device_index(self.device)
         self._call = lib().hqb_cache_append
@@ -704,8 +705,8 @@ class PagedCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor | None = None,
                stream=None) -> None:
         """Writes rows of k and v [tokens, heads, dim] (FP16, BF16 or FP32) into the cache's slots
-        [count]: row rows[i], or i, goes to slots[i]; negative ones are skipped.  flags collects
-        HQB_DEVERR_* bits."""
+        [count]: row rows[i], or i, goes to slots[i]; negative ones are skipped, and so are ones out
+        of range (see flags)."""
         shape, strides, device = k.shape, k.stride(), self._index
         if len(shape) != 3 or shape[1] != self.heads or shape[2] != self.dim or v.shape != shape:
             raise ValueError(f"k and v must be [tokens, {self.heads}, {self.dim}]")
@@ -731,9 +732,11 @@ class PagedCache:
 class TreeAttention:
     """Attention of drafted trees over a paged cache (hqb_tree_attention) for steps of up to
     `requests` requests, `tokens` tokens in all, max_new nodes and about max_context cached
-    tokens a request; holds the call's workspace, so calls that overlap need one each."""
+    tokens a request; holds the call's workspace (or takes one: workspace(bytes) gives it), so
+    calls that overlap need one each."""
 
-    def __init__(self, cache: PagedCache, q_heads: int, requests: int, tokens: int, max_new: int, max_context: int):
+    def __init__(self, cache: PagedCache, q_heads: int, requests: int, tokens: int, max_new: int, max_context: int,
+                 workspace=None):
         if q_heads < 1 or q_heads % cache.heads != 0:
             raise ValueError("q_heads must be a multiple of the cache's heads")
         if not 1 <= max_new <= MAX_NODES:
@@ -748,7 +751,7 @@ class TreeAttention:
         need = lib().hqb_tree_attention_workspace_bytes(cache._at, ctypes.addressof(args), cache._index)
         if need == 0:
             raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
-        self.ws = Workspace(need, cache.device)
+        self.ws = Workspace(need, cache.device) if workspace is None else workspace(need)
         self._ws, self._ws_bytes = self.ws.ptr(), self.ws.nbytes
         self._args = ctypes.create_string_buffer(_ATTENTION.size)
         self._at = ctypes.addressof(self._args)
@@ -818,7 +821,7 @@ class LoraSet:
     """Low-rank adapters stacked in two device tensors: a [adapters, max_rank, cols] and b
     [adapters, rows, max_rank] (FP16 or BF16), with ranks [adapters] int32 (None: max_rank each)
     and scales [adapters] FP32 (None: 1).  Workspaces are kept per stream; the constructing
-    stream's is made at once, for up to max_tokens tokens."""
+    stream's is made at once, for up to max_tokens tokens (0: when it is first needed)."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, ranks: torch.Tensor | None = None,
                  scales: torch.Tensor | None = None, max_tokens: int = 8192):
@@ -846,13 +849,17 @@ class LoraSet:
         self._at, self._index = ctypes.addressof(self.c), _device_index(a.device)
         self._call = lib().hqb_lora
         self._ws: dict = {}
-        self.workspace(max_tokens, _raw_stream(None, self._index))
+        if max_tokens > 0:
+            self.workspace(max_tokens, _raw_stream(None, self._index))
+
+    def workspace_bytes(self, tokens: int) -> int:
+        return lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
 
     def workspace(self, tokens: int, stream: int) -> Workspace:
         """The stream's workspace, grown to what `tokens` tokens need."""
         ws = self._ws.get(stream)
         if ws is None or tokens > ws.tokens:
-            need = lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
+            need = self.workspace_bytes(tokens)
             if stream == _raw_stream(None, self._index):
                 ws = Workspace(need, self.device)
             else:  # allocated on the stream that uses it: the allocator then reuses it in that order

@@ -1,4 +1,5 @@
-"""PyTorch operator over the C ABI: ``torch.ops.harpq_b200.gemv``.
+"""PyTorch operators over the C ABI: ``torch.ops.harpq_b200.gemv`` and the serving operators
+``cache_append``, ``tree_attention`` and ``lora`` (at the end of this file).
 
 The reference lists a PyTorch custom-op wrapper over its native GEMV as planned work
 (docs/RESEARCH_PLAN.md:106-107); it has no implementation to mirror.  This module
@@ -86,3 +87,79 @@ def gemv(x: torch.Tensor, planes: List[torch.Tensor], rows: int, cols: int, pref
 def _gemv_fake(x, planes, rows, cols, prefix, bias=None, out_dtype=torch.float16):
     torch._check(x.dim() == 2 and x.shape[1] == cols, lambda: f"x must be [batch, {cols}]")
     return x.new_empty((x.shape[0], rows), dtype=out_dtype)
+
+
+# ---- serving operators -------------------------------------------------------------------
+#
+#   cache_append(k_cache, v_cache, k, v, slots, rows)          writes into the caches
+#   tree_attention(q, k, v, k_cache, v_cache, tables, context_lens, starts, mask, max_new,
+#                  max_context, scale)                         -> [tokens, q_heads, dim]
+#   lora(x, a, b, ids, ranks, scales, base, out_dtype)         -> [tokens, rows]
+#
+# The same calls and the same bits as PagedCache.append, TreeAttention and LoraSet.apply, whose
+# arguments they share, without a handle to keep.  Workspaces are cached per stream and grown.
+
+_SERVING_WORKSPACES: dict = {}
+
+
+def _serving_workspace(kind: str, device: torch.device, stream: int, need: int) -> "hqb.Workspace":
+    key = (kind, device.index, stream)
+    ws = _SERVING_WORKSPACES.get(key)
+    if ws is None or ws.nbytes < need:
+        ws = _SERVING_WORKSPACES[key] = hqb.Workspace(need, device)
+    return ws
+
+
+def _serving_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, stream: int) -> "hqb.PagedCache":
+    return hqb.PagedCache(k_cache, v_cache, _serving_workspace("cache", k_cache.device, stream, 256).buf.view(torch.int32)[:1])
+
+
+@torch.library.custom_op("harpq_b200::cache_append", mutates_args=("k_cache", "v_cache"), device_types="cuda")
+def cache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
+                 rows: Optional[torch.Tensor] = None) -> None:
+    """k_cache, v_cache[slots[i]] = k, v[rows[i]] (rows None: row i); negative slots and rows are skipped."""
+    stream = torch.cuda.current_stream(k.device).cuda_stream
+    _serving_cache(k_cache, v_cache, stream).append(k, v, slots, rows=rows)
+
+
+@cache_append.register_fake
+def _cache_append_fake(k_cache, v_cache, k, v, slots, rows=None):
+    torch._check(k.dim() == 3 and k.shape == v.shape, lambda: "k and v must be [tokens, heads, dim]")
+    torch._check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, lambda: "caches must be [pages, page_size, heads, dim]")
+
+
+@torch.library.custom_op("harpq_b200::tree_attention", mutates_args=(), device_types="cuda")
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   tables: torch.Tensor, context_lens: torch.Tensor, starts: torch.Tensor,
+                   mask: Optional[torch.Tensor], max_new: int, max_context: int,
+                   scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of each request's drafted nodes over its cached context and the nodes its mask shows."""
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    attend = hqb.TreeAttention(_serving_cache(k_cache, v_cache, stream), q.shape[1], context_lens.numel(), q.shape[0], max_new,
+                               max_context, workspace=lambda need: _serving_workspace("attention", q.device, stream, need))
+    return attend(q, k, v, tables, context_lens, starts, mask, scale=scale)
+
+
+@tree_attention.register_fake
+def _tree_attention_fake(q, k, v, k_cache, v_cache, tables, context_lens, starts, mask, max_new, max_context, scale=None):
+    torch._check(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and q.shape[0] == k.shape[0],
+                 lambda: "q, k and v must be [tokens, heads, dim]")
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("harpq_b200::lora", mutates_args=(), device_types="cuda")
+def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, ranks: Optional[torch.Tensor] = None,
+         scales: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
+         out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """base + scales[i] * b[i] (a[i] x) per token, i = ids[token] (negative: base alone)."""
+    adapters = hqb.LoraSet(a, b, ranks, scales, max_tokens=0)
+    stream = torch.cuda.current_stream(x.device).cuda_stream
+    ws = _serving_workspace("lora", x.device, stream, adapters.workspace_bytes(x.shape[0]))
+    return adapters.apply(x, ids, base=base, y_dtype=out_dtype, workspace=ws)
+
+
+@lora.register_fake
+def _lora_fake(x, a, b, ids, ranks=None, scales=None, base=None, out_dtype=None):
+    torch._check(x.dim() == 2 and a.dim() == 3 and x.shape[1] == a.shape[2], lambda: "x must be [tokens, cols]")
+    kind = out_dtype or (base.dtype if base is not None else x.dtype)
+    return x.new_empty((x.shape[0], b.shape[1]), dtype=kind)

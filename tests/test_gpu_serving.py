@@ -718,3 +718,87 @@ def test_lora_beside_a_plane_matrix():
     want, tol = lora_reference(x, a, b, ranks, scales, ids, y.clone(), F32)
     hqb.LoraSet(a, b, ranks, scales).apply(x, ids, base=y, out=y)
     assert bool(((y.double() - want).abs() <= tol).all())
+
+
+# ---- refusals of the binding, the PyTorch operators, the example ---------------------------------
+
+
+def test_binding_refusals():
+    k = torch.zeros(4, 16, 2, 64, dtype=F16, device="cuda")
+    cache = hqb.PagedCache(k, k.clone())
+    for bad in ((k, k.bfloat16()), (k, k[:2]), (k, k.transpose(1, 2)), (k[..., ::2], k[..., ::2]), (k[0], k[0])):
+        with pytest.raises(ValueError):
+            hqb.PagedCache(*bad)
+    with pytest.raises(TypeError):
+        hqb.PagedCache(k.float(), k.float())
+    rows, slots = torch.zeros(3, 2, 64, dtype=F16, device="cuda"), ints([0, 1, 2])
+    for bad in ((rows[:2], rows[:2], slots), (rows, rows[:2], slots), (rows[:, :1], rows[:, :1], slots), (rows, rows, slots.long()),
+                (rows, rows, slots.cpu()), (rows, rows.transpose(0, 1).contiguous().transpose(0, 1), slots)):
+        with pytest.raises(ValueError):
+            cache.append(*bad)
+    with pytest.raises(TypeError):
+        cache.append(rows.double(), rows.double(), slots)
+    for bad in (dict(q_heads=3), dict(max_new=0), dict(max_new=257), dict(requests=0), dict(tokens=0)):
+        with pytest.raises(ValueError):
+            hqb.TreeAttention(cache, **{**dict(q_heads=4, requests=1, tokens=3, max_new=3, max_context=10), **bad})
+    attend = hqb.TreeAttention(cache, 4, 1, 3, 3, 10)
+    q, tables, one, starts = torch.zeros(3, 4, 64, dtype=F16, device="cuda"), ints([[0]]), ints([3]), ints([0, 3])
+    good = dict(q=q, k=rows, v=rows, tables=tables, context_lens=one, starts=starts)
+    attend(**good)
+    for bad in (dict(q=q[:, :2]), dict(k=rows[:2]), dict(tables=ints([0])), dict(starts=ints([0])), dict(mask=ints([[1]])),
+                dict(context_lens=one.long()), dict(lse=torch.zeros(3, 4, device="cuda").half()), dict(out=q[:2])):
+        with pytest.raises((ValueError, TypeError)):
+            attend(**{**good, **bad})
+    with pytest.raises(TypeError):
+        attend(**{**good, "q": q.bfloat16()})
+    with pytest.raises(ValueError):
+        attend(torch.zeros(4, 4, 64, dtype=F16, device="cuda"), *[torch.zeros(4, 2, 64, dtype=F16, device="cuda")] * 2, tables, one, starts)
+    a, b = torch.zeros(2, 8, 64, dtype=F16, device="cuda"), torch.zeros(2, 32, 8, dtype=F16, device="cuda")
+    for bad in ((a, b[:1]), (a, b.transpose(1, 2)), (a[:, :, ::2], b), (torch.zeros(2, 129, 4, device="cuda").half(), torch.zeros(2, 4, 129, device="cuda").half())):
+        with pytest.raises(ValueError):
+            hqb.LoraSet(*bad)
+    with pytest.raises(TypeError):
+        hqb.LoraSet(a, b.bfloat16())
+    with pytest.raises(ValueError):
+        hqb.LoraSet(a, b, ranks=ints([1]))
+    s, x, ids = hqb.LoraSet(a, b), torch.zeros(3, 64, dtype=F16, device="cuda"), ints([0, 1, -1])
+    for bad in (dict(x=x[:, :32]), dict(x=x.float()), dict(ids=ids[:2]), dict(base=x), dict(out=torch.zeros(3, 32, device="cuda").bfloat16())):
+        with pytest.raises((ValueError, TypeError)):
+            s.apply(**{**dict(x=x, ids=ids), **bad})
+    plan = hqb.PagePlan(2, 4, 16, 8)
+    for bad in (dict(context_lens=ints([1])), dict(new_lens=ints([1, 2]).long()), dict(tables=ints([[0], [1]])), dict(parents=ints([-1, 0, -1, 0]))):
+        with pytest.raises(ValueError):
+            plan.build(**{**dict(context_lens=ints([1, 2]), new_lens=ints([2, 2])), **bad})
+
+
+def test_torch_operators_match_the_binding():
+    import harpq_b200_ops  # noqa: F401
+
+    ops = torch.ops.harpq_b200
+    s = make_attention(21, [40, 300], [5, 9], 8, 2, 64, 16, F16)
+    out, _ = check_attention(s)
+    again = ops.tree_attention(s["q"], s["k"], s["v"], s["kc"], s["vc"], s["tables"], ints(s["ctx"]), ints(s["starts"]), s["mask"],
+                               s["most"], 300, None)
+    assert torch.equal(out, again)
+    slots = torch.arange(14, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    kc, vc = s["kc"].clone(), s["vc"].clone()
+    hqb.PagedCache(kc, vc).append(s["k"], s["v"], slots)
+    ops.cache_append(s["kc"], s["vc"], s["k"], s["v"], slots)
+    assert torch.equal(kc, s["kc"]) and torch.equal(vc, s["vc"])
+    for tokens in (9, 600):
+        x, a, b, ranks, scales, ids, base = make_lora(22, tokens, 128, 64, 3, 16, BF16, BF16)
+        y = hqb.LoraSet(a, b, ranks, scales).apply(x, ids, base=base)
+        assert torch.equal(y, ops.lora(x, a, b, ids, ranks, scales, base))
+
+
+@pytest.mark.parametrize("requests", [1, 3])
+def test_drafted_trees_decode_as_plain_decoding(requests):
+    """The example: page plan, adapters, tree attention and cache append around quantized projections."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+    import draft_tree_decode
+
+    same, rate = draft_tree_decode.main(requests, 20)
+    assert same and rate >= 1.0
