@@ -17,7 +17,7 @@ namespace {
 
 constexpr uint32_t kCluster = 8;         // CTAs that share a tile: the portable cluster size
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kDirectTokens = 256;  // up to here every cluster finds its own tile
+constexpr uint32_t kDirectTokens = kThreads;  // up to here every cluster finds its own tile
 // A planned call keeps to lora_kernel up to this many tokens * padded rank.  B200, us, lora_kernel /
 // shrink + expand, FP16 or BF16, 8 adapters: rank 16, 4096 x 4096: 1024 tokens 18.4 / 24.0, 2048 tokens
 // 28.7 / 27.5; rank 24, 1024 x 8192: 777 tokens 18.0 / 27.2; rank 64, 11008 x 4096: 300 tokens 16.8 /
@@ -49,6 +49,7 @@ struct LoraParams {
   uint32_t tile_rows;
   uint32_t max_tiles;
   uint32_t splits;    // column ranges of the first product
+  uint32_t stages;    // of lora_kernel's rings
   float* inner;       // [splits][max_tiles][tile_rows][padded rank]
 };
 
@@ -365,27 +366,47 @@ __device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, in
     count = t.count;
     for (uint32_t i = tid; i < M; i += kThreads) s_token[i] = i < count ? static_cast<int32_t>(p.order[t.first + i]) : -1;
   } else {
-    // the cluster of a token that has a multiple of M tokens of its adapter before it takes
-    // that token and the adapter's next M - 1
-    group = group_of(p, tile, bad);
-    const bool same = tid < p.tokens && group_of(p, tid, bad) == group;
-    const uint32_t votes = ballot(same);
-    if (lane == 0) s_info[warp] = votes;
+    // a token with a multiple of M tokens of its adapter before it begins a tile of that token and the
+    // adapter's next M - 1; cluster i takes the i-th tile, in the order of their first tokens
+    const bool mine = tid < p.tokens;
+    const uint32_t own = mine ? group_of(p, tid, bad) : 0xFFFFu;
+    if (bad != 0 && tile == 0) atomicOr(p.error, static_cast<int>(bad));
+    // groups fit 16 bits (kMaxAdapters): two a word
+    reinterpret_cast<uint16_t*>(s_info + 64)[tid] = static_cast<uint16_t>(own);
     for (uint32_t i = tid; i < M; i += kThreads) s_token[i] = -1;
     __syncthreads();
-    uint32_t before = 0, mine = 0, all = 0;
+    uint32_t pairs = 0;
+    const uint32_t twice = own * 0x10001u;
+    for (uint32_t s = 0; s < warp * 16 && warp * 32 < p.tokens; s += 4) {  // the earlier warps' tokens, 8 at a time
+      const uint4 v = *reinterpret_cast<const uint4*>(&s_info[64 + s]);
+      pairs += __vseteq2(v.x, twice) + __vseteq2(v.y, twice) + __vseteq2(v.z, twice) + __vseteq2(v.w, twice);
+    }
+    for (uint32_t s = 0; s < 16 && warp * 32 + s * 2 < p.tokens; ++s) {  // this warp's, up to the thread's own
+      const uint32_t same = __vseteq2(s_info[64 + warp * 16 + s], twice);
+      pairs += 2 * s + 1 < lane ? same : 2 * s < lane ? same & 1u : 0u;
+    }
+    const uint32_t before = (pairs & 0xFFFFu) + (pairs >> 16);
+    const bool first = mine && before % M == 0 && !(own == p.s.adapters && p.in_place);
+    const uint32_t votes = ballot(first);
+    if (lane == 0) s_info[warp] = __popc(votes);
+    __syncthreads();
+    uint32_t index = __popc(votes & ((1u << lane) - 1u)), all = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kThreads / 32; ++w) {
-      const uint32_t v = s_info[w], n = __popc(v);
-      all += n;
-      if (w < (tile >> 5)) before += n;
-      if (w == (tile >> 5)) before += __popc(v & ((1u << (tile & 31)) - 1u));
-      if (w < warp) mine += n;
+      if (w < warp) index += s_info[w];
+      all += s_info[w];
     }
-    if (before % M != 0) return false;
-    mine += __popc(votes & ((1u << lane) - 1u));
-    if (same && mine >= before && mine < before + M) s_token[mine - before] = static_cast<int32_t>(tid);
-    count = min(static_cast<uint32_t>(M), all - before);
+    if (tile >= all) return false;
+    if (first && index == tile) {
+      s_info[32] = own;
+      s_info[33] = before;
+    }
+    __syncthreads();
+    group = s_info[32];
+    const uint32_t place = before - s_info[33];
+    const bool member = own == group && before >= s_info[33] && place < M;
+    if (member) s_token[place] = static_cast<int32_t>(tid);
+    count = __syncthreads_count(member);
   }
   __syncthreads();
   return true;
@@ -405,16 +426,21 @@ constexpr uint32_t kSliceWarps = 8;  // warps along the columns in lora_kernel
 
 template <typename T, typename Y, int RP>
 struct LoraSmem {
-  static constexpr uint32_t kToken = 256, kFactor = kToken + 64, kTermsAt = kFactor + 64;
+  static constexpr uint32_t kToken = 256 + kDirectTokens * 2, kFactor = kToken + 64, kTermsAt = kFactor + 64;
   static constexpr uint32_t kSum = kTermsAt + kTerms<T, Y> * 16 * LoraShape<RP>::kPitch * 2;
   static constexpr uint32_t kPart = kSum + 16 * RP * 4;
   static constexpr uint32_t kRing = kPart + kSliceWarps * 16 * RP * 4;
   // as many stages as leave room for two CTAs an SM, else as fit one
   static constexpr uint32_t kTwo = kRing < 110 * 1024 ? (110 * 1024 - kRing) / (8 * Expand<T, Y, RP, 16>::kStage) : 0;
   static constexpr uint32_t kOne = (227 * 1024 - kRing) / (8 * Expand<T, Y, RP, 16>::kStage);
-  static constexpr uint32_t kStages = kTwo > 6 ? 6 : kTwo >= 2 ? kTwo : kOne >= 2 ? 2 : 1;
+  static constexpr uint32_t kMost = kTwo > 6 ? 6 : kTwo >= 2 ? kTwo : kOne >= 2 ? 2 : 1;
   static_assert(kOne >= 1, "a stage fits");
-  static constexpr uint32_t kBytes = kRing + 8 * kStages * Expand<T, Y, RP, 16>::kStage;
+  // no more than a warp has steps: what is not needed lets more CTAs share an SM
+  static uint32_t stages(uint64_t rows) {
+    const uint64_t steps = (rows + 32 * 8 * kCluster - 1) / (32 * 8 * kCluster);
+    return steps < kMost ? static_cast<uint32_t>(steps) : kMost;
+  }
+  static uint32_t bytes(uint32_t stages) { return kRing + 8 * stages * Expand<T, Y, RP, 16>::kStage; }
 };
 
 // Mathematics: t = A x (FP32 sums of exact 16-bit products), y = base + scale B t.
@@ -434,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
   constexpr int kN = kTerms<T, Y>;
   constexpr uint32_t M = 16;
   extern __shared__ __align__(128) uint8_t sm[];
-  uint32_t* s_info = reinterpret_cast<uint32_t*>(sm);             // 64 words
+  uint32_t* s_info = reinterpret_cast<uint32_t*>(sm);             // 64 words, the tokens' groups
   int32_t* s_token = reinterpret_cast<int32_t*>(sm + L::kToken);  // [M], -1: no row
   float* s_factor = reinterpret_cast<float*>(sm + L::kFactor);    // [M]
   T* s_terms = reinterpret_cast<T*>(sm + L::kTermsAt);            // [kN][M][kPitch]
@@ -455,7 +481,7 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
   const uint32_t n_steps = static_cast<uint32_t>((rows + 31) / 32);
   const uint32_t n0 = static_cast<uint64_t>(n_steps) * cta / kCluster, n1 = static_cast<uint64_t>(n_steps) * (cta + 1) / kCluster;
   Expand<T, Y, RP, M> x2;
-  x2.prepare(p, group, rank, count, s_token, smem_u32(sm) + L::kRing + warp * L::kStages * Expand<T, Y, RP, M>::kStage, L::kStages);
+  x2.prepare(p, group, rank, count, s_token, smem_u32(sm) + L::kRing + warp * p.stages * Expand<T, Y, RP, M>::kStage, p.stages);
   if (VEC) x2.start(n0 + warp, n1);
 
   if (rank != 0) {
@@ -830,9 +856,14 @@ cudaError_t launch(K kernel, DeviceOnce& once, uint32_t grid, uint32_t smem, uin
 }
 
 template <typename T, typename Y, int RP, bool VEC>
-cudaError_t launch_tile(const LoraParams& p, uint32_t tiles, cudaStream_t st) {
+cudaError_t launch_tile(LoraParams p, uint32_t tiles, cudaStream_t st) {
+  using L = LoraSmem<T, Y, RP>;
   static DeviceOnce once;
-  return launch(lora_kernel<T, Y, RP, VEC>, once, tiles * kCluster, LoraSmem<T, Y, RP>::kBytes, kCluster, p, st);
+  p.stages = L::stages(p.s.rows);
+  const cudaError_t e =
+      allow_dynamic_smem(once, reinterpret_cast<const void*>(lora_kernel<T, Y, RP, VEC>), L::bytes(L::kMost));
+  if (e != cudaSuccess) return e;
+  return launch_dependent(lora_kernel<T, Y, RP, VEC>, dim3(tiles * kCluster), kThreads, L::bytes(p.stages), kCluster, st, p);
 }
 
 template <typename T, typename Y, int RP>
@@ -924,7 +955,9 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.error = reinterpret_cast<int*>(ws);
   cudaStream_t st = as_stream(stream);
-  uint32_t tiles = tokens;
+  // tiles at most: every group may end in a partly filled one
+  const uint32_t groups = s->adapters + 1, full = tokens / 16 + groups;
+  uint32_t tiles = tokens < full ? tokens : full;
   if (p.planned) {
     const Layout l = layout(s, tokens, p.tile_rows);
     p.tile_count = reinterpret_cast<uint32_t*>(ws + 256);
