@@ -371,21 +371,29 @@ __device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, in
     const bool mine = tid < p.tokens;
     const uint32_t own = mine ? group_of(p, tid, bad) : 0xFFFFu;
     if (bad != 0 && tile == 0) atomicOr(p.error, static_cast<int>(bad));
-    // groups fit 16 bits (kMaxAdapters): two a word
-    reinterpret_cast<uint16_t*>(s_info + 64)[tid] = static_cast<uint16_t>(own);
+    // tokens of the same group among the earlier ones, by the votes on each bit of the group (15 at
+    // most: kMaxAdapters): a warp's peers are the AND of its votes, each taken as the own bit is
+    const uint32_t bits = 32 - __clz(p.s.adapters);
+    uint32_t* s_votes = s_info + 64;  // [warp][16], the last its live tokens
+    const uint32_t live = ballot(mine);
+    uint32_t peers = live;
+    for (uint32_t i = 0; i < bits; ++i) {
+      const uint32_t v = ballot(own >> i & 1u);
+      peers &= own >> i & 1u ? v : ~v;
+      if (lane == 0) s_votes[warp * 16 + i] = v;
+    }
+    if (lane == 0) s_votes[warp * 16 + 15] = live;
     for (uint32_t i = tid; i < M; i += kThreads) s_token[i] = -1;
     __syncthreads();
-    uint32_t pairs = 0;
-    const uint32_t twice = own * 0x10001u;
-    for (uint32_t s = 0; s < warp * 16 && warp * 32 < p.tokens; s += 4) {  // the earlier warps' tokens, 8 at a time
-      const uint4 v = *reinterpret_cast<const uint4*>(&s_info[64 + s]);
-      pairs += __vseteq2(v.x, twice) + __vseteq2(v.y, twice) + __vseteq2(v.z, twice) + __vseteq2(v.w, twice);
+    uint32_t before = __popc(peers & ((1u << lane) - 1u));
+    for (uint32_t w = 0; w < warp && warp * 32 < p.tokens; ++w) {
+      uint32_t m = s_votes[w * 16 + 15];
+      for (uint32_t i = 0; i < bits; ++i) {
+        const uint32_t v = s_votes[w * 16 + i];
+        m &= own >> i & 1u ? v : ~v;
+      }
+      before += __popc(m);
     }
-    for (uint32_t s = 0; s < 16 && warp * 32 + s * 2 < p.tokens; ++s) {  // this warp's, up to the thread's own
-      const uint32_t same = __vseteq2(s_info[64 + warp * 16 + s], twice);
-      pairs += 2 * s + 1 < lane ? same : 2 * s < lane ? same & 1u : 0u;
-    }
-    const uint32_t before = (pairs & 0xFFFFu) + (pairs >> 16);
     const bool first = mine && before % M == 0 && !(own == p.s.adapters && p.in_place);
     const uint32_t votes = ballot(first);
     if (lane == 0) s_info[warp] = __popc(votes);
@@ -426,7 +434,7 @@ constexpr uint32_t kSliceWarps = 8;  // warps along the columns in lora_kernel
 
 template <typename T, typename Y, int RP>
 struct LoraSmem {
-  static constexpr uint32_t kToken = 256 + kDirectTokens * 2, kFactor = kToken + 64, kTermsAt = kFactor + 64;
+  static constexpr uint32_t kToken = 256 + kThreads / 32 * 64, kFactor = kToken + 64, kTermsAt = kFactor + 64;
   static constexpr uint32_t kSum = kTermsAt + kTerms<T, Y> * 16 * LoraShape<RP>::kPitch * 2;
   static constexpr uint32_t kPart = kSum + 16 * RP * 4;
   static constexpr uint32_t kRing = kPart + kSliceWarps * 16 * RP * 4;
@@ -460,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
   constexpr int kN = kTerms<T, Y>;
   constexpr uint32_t M = 16;
   extern __shared__ __align__(128) uint8_t sm[];
-  uint32_t* s_info = reinterpret_cast<uint32_t*>(sm);             // 64 words, the tokens' groups
+  uint32_t* s_info = reinterpret_cast<uint32_t*>(sm);             // 64 words, the votes
   int32_t* s_token = reinterpret_cast<int32_t*>(sm + L::kToken);  // [M], -1: no row
   float* s_factor = reinterpret_cast<float*>(sm + L::kFactor);    // [M]
   T* s_terms = reinterpret_cast<T*>(sm + L::kTermsAt);            // [kN][M][kPitch]
