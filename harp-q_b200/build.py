@@ -2,7 +2,9 @@
 
 Sources are compiled with nvcc for ``-gencode arch=compute_100a,code=sm_100a`` and
 linked with the static CUDA runtime (its symbols hidden) plus cuBLAS for the
-materialize-then-SGEMM oracle entry point.  The native test program
+materialize-then-SGEMM oracle entry point.  The serving operators' CPython module
+(csrc/hqb_bind.cpp, over torch's C++ headers) is built beside it as
+harp-q_b200/lib/harpq_b200_bind.so.  The native test program
 (tests/native/api_test.cu) is linked against the library as
 harp-q_b200/lib/hqb_api_test.  Rebuilds only what is out of date.
 """
@@ -23,6 +25,8 @@ LIB_DIR = PKG / "lib"
 OBJ_DIR = LIB_DIR / "obj"
 LIB = LIB_DIR / "libharpq_b200.so"
 API_TEST = LIB_DIR / "hqb_api_test"
+BIND = LIB_DIR / "harpq_b200_bind.so"
+CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["hqb_plane.cu", "hqb_bulk.cu", "hqb_raw.cu", "hqb_raw_i8.cu", "hqb_step.cu", "hqb_prefill.cu", "harpq_native.cu", "hqb_static_scratch.cu",
@@ -58,6 +62,23 @@ def _compile(cmd: list[str], obj: Path) -> None:
     os.utime(obj, (t0, t0))
 
 
+def _build_bind() -> None:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(NVCC).resolve().parent.parent
+    torch_lib = Path(torch.__file__).parent / "lib"
+    tmp = BIND.with_name(BIND.name + ".tmp")
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-I", str(REPO / "include"), "-I", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
+          *[a for d in cpp_extension.include_paths() for a in ("-isystem", d)], str(CSRC / "hqb_bind.cpp"), "-o", str(tmp),
+          "-L", str(LIB_DIR), "-lharpq_b200", "-L", str(torch_lib), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+          "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, BIND)
+
+
 def build(force: bool = False, ptxas_verbose: bool = False) -> Path:
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     headers = _headers()
@@ -78,6 +99,8 @@ def build(force: bool = False, ptxas_verbose: bool = False) -> Path:
         _run([NVCC, *ARCH, "-shared", "-cudart", "static", "-Xlinker", "--exclude-libs,ALL",
               *map(str, objs), "-o", str(tmp), "-lcublas"])
         os.replace(tmp, LIB)
+    if force or _stale(BIND, [CSRC / "hqb_bind.cpp", LIB, REPO / "include" / "harpq_b200.h"]):
+        _build_bind()
     test_src = REPO / "tests" / "native" / "api_test.cu"
     if test_src.exists() and (force or _stale(API_TEST, [test_src, LIB, *headers])):
         _run([NVCC, *CFLAGS, str(test_src), "-o", str(API_TEST), "-L", str(LIB_DIR), "-lharpq_b200",

@@ -13,7 +13,7 @@ this module without the built library, or calling it without a CUDA device, rais
 from __future__ import annotations
 
 import ctypes
-import struct
+import importlib.util
 from pathlib import Path
 from typing import Sequence
 
@@ -21,6 +21,7 @@ import torch
 
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "lib" / "libharpq_b200.so"
+BIND_PATH = PKG / "lib" / "harpq_b200_bind.so"
 
 F32, F16, BF16 = 0, 1, 2  # BF16: serving operators only
 FLAG_PDL, FLAG_SIMT, FLAG_RING, FLAG_TCGEN05, FLAG_STREAMK, FLAG_ROWBLOCK = 1, 2, 4, 8, 16, 32
@@ -187,6 +188,22 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+_bind_module = None
+
+
+def bind():
+    """The CPython module of the serving operators' calls (csrc/hqb_bind.cpp)."""
+    global _bind_module
+    if _bind_module is None:
+        lib()
+        if not BIND_PATH.exists():
+            raise ImportError(f"{BIND_PATH} is missing: build it with __graft_entry__.build()")
+        spec = importlib.util.spec_from_file_location("harpq_b200_bind", str(BIND_PATH))
+        _bind_module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_bind_module)
+    return _bind_module
 
 
 def check(status: int, what: str) -> None:
@@ -584,38 +601,32 @@ class RawMatrix:
 
 _SERVING_DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
 _ROW_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-# A step's host time is mostly this module's own, so the calls below read each attribute once,
-# pack their argument structures in one go and ask for the raw stream.
-_PAGE_PLAN = struct.Struct("@8I15P")
-_ATTENTION = struct.Struct("@7If9P6Q")
-assert _PAGE_PLAN.size == ctypes.sizeof(PagePlanC) and _ATTENTION.size == ctypes.sizeof(AttentionC)
+# The calls below go through bind(), which checks the tensors and fills the argument structure in
+# one step and answers _UNFIT where an argument does not fit; the methods here then say which.
+_UNFIT = -1
 
 
 def _device_index(device: torch.device) -> int:
     return torch.cuda.current_device() if device.index is None else device.index
 
 
-def _raw_stream(stream, index: int) -> int:
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(index)
-    return _stream(stream) or 0
+def _raw_stream(stream) -> int | None:
+    """A stream argument as the number that bind() takes; None: the device's current one."""
+    return None if stream is None else _stream(stream) or 0
 
 
-def _ints(name: str, t: torch.Tensor, n: int, device: int) -> int:
-    """Checks an int32 index tensor of n elements on GPU `device` and gives its address."""
+def _ints(name: str, t: torch.Tensor, n: int, device: int) -> None:
+    """Refuses what is no contiguous int32 tensor of n elements on GPU `device`."""
     if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous() or t.get_device() != device:
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on GPU {device}, "
                          f"got {list(t.shape)} {t.dtype} on {t.device}")
-    return t.data_ptr()
 
 
-def _table(name: str, t: torch.Tensor, rows: int, device: int) -> int:
-    """Checks an int32 matrix of `rows` rows and gives its columns."""
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != rows:
-        raise ValueError(f"{name} must have {rows} rows, got {list(shape)}")
-    _ints(name, t, rows * shape[1], device)
-    return shape[1]
+def _table(name: str, t: torch.Tensor, rows: int, device: int) -> None:
+    """Refuses what is no int32 matrix of `rows` rows."""
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows, got {list(t.shape)}")
+    _ints(name, t, t.numel(), device)
 
 
 class PagePlan:
@@ -638,10 +649,12 @@ class PagePlan:
         self.mask = mask.view(tokens, self.words) if self.words else None
         self.device = self.starts.device
         self._index = _device_index(self.device)
-        self._out = [t.data_ptr() for t in parts]
-        self._args = ctypes.create_string_buffer(_PAGE_PLAN.size)
+        at = [t.data_ptr() for t in parts]
+        self._args = PagePlanC(requests=requests, page_size=page_size, num_pages=num_pages, token_capacity=tokens,
+                               starts=at[0], token_request=at[1], positions=at[2], flags=at[6])
         self._at = ctypes.addressof(self._args)
-        self._call = lib().hqb_page_plan
+        self._outputs = (at[3], at[4], at[5], at[7], self.words)
+        self._call = bind().page_plan
 
     def build(self, context_lens: torch.Tensor, new_lens: torch.Tensor, held: torch.Tensor | None = None,
               tables: torch.Tensor | None = None, free_pages: torch.Tensor | None = None,
@@ -650,33 +663,30 @@ class PagePlan:
         new tokens pages and slots, writing new columns into it; parents [at least the step's
         tokens] gives tree positions and masks.  held and free_head are the counts before the
         step (a previous plan's, not this one's buffers)."""
+        status = self._call(self._at, self._index, _raw_stream(stream), context_lens, new_lens, held, tables, free_pages,
+                            free_head, parents, *self._outputs)
+        if status:
+            if status == _UNFIT:
+                self._refuse(context_lens, new_lens, held, tables, free_pages, free_head, parents)
+            check(status, "hqb_page_plan")
+        return self
+
+    def _refuse(self, context_lens, new_lens, held, tables, free_pages, free_head, parents) -> None:
         n, device = self.batch, self._index
-        starts, requests, positions, slots, held_out, head_out, flags, mask = self._out
-        ctx = _ints("context_lens", context_lens, n, device)
-        new = _ints("new_lens", new_lens, n, device)
-        have = 0 if held is None else _ints("held", held, n, device)
-        stride = free = rows = pool = head = tree = words = 0
+        _ints("context_lens", context_lens, n, device)
+        _ints("new_lens", new_lens, n, device)
+        if held is not None:
+            _ints("held", held, n, device)
         if tables is not None:
             if free_pages is None or free_head is None:
                 raise ValueError("tables need free_pages and free_head")
-            stride, rows, free = _table("tables", tables, n, device), tables.data_ptr(), free_pages.numel()
-            pool = _ints("free_pages", free_pages, free, device)
-            head = _ints("free_head", free_head, 1, device)
-        else:
-            slots = held_out = head_out = 0
+            _table("tables", tables, n, device)
+            _ints("free_pages", free_pages, free_pages.numel(), device)
+            _ints("free_head", free_head, 1, device)
         if parents is not None:
             if not self.words:
                 raise ValueError("parents need a plan with max_new > 0")
-            tree, words = _ints("parents", parents, parents.numel(), device), self.words
-        else:
-            mask = 0
-        _PAGE_PLAN.pack_into(self._args, 0, n, self.page_size, self.num_pages, stride, self.tokens, free, words, 0, ctx,
-                             new, have, pool, head, tree, rows, starts, requests, positions, slots, held_out, head_out,
-                             mask, flags)
-        status = self._call(self._at, _raw_stream(stream, self._index))
-        if status:
-            check(status, "hqb_page_plan")
-        return self
+            _ints("parents", parents, parents.numel(), device)
 
 
 class PagedCache:
@@ -700,33 +710,31 @@ class PagedCache:
         self.flags = torch.zeros(1, dtype=torch.int32, device=k.device) if flags is None else flags
         self._at, self._flags = ctypes.addressof(self.c), self.flags.data_ptr()
         self._index = _device_index(self.device)
-        self._call = lib().hqb_cache_append
+        self._call = bind().cache_append
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor | None = None,
                stream=None) -> None:
         """Writes rows of k and v [tokens, heads, dim] (FP16, BF16 or FP32) into the cache's slots
         [count]: row rows[i], or i, goes to slots[i]; negative ones are skipped, and so are ones out
         of range (see flags)."""
-        shape, strides, device = k.shape, k.stride(), self._index
-        if len(shape) != 3 or shape[1] != self.heads or shape[2] != self.dim or v.shape != shape:
-            raise ValueError(f"k and v must be [tokens, {self.heads}, {self.dim}]")
-        kind = _ROW_DTYPES.get(k.dtype)
-        if kind is None or v.dtype is not k.dtype:
-            raise TypeError("k and v must share a type: float16, bfloat16 or float32")
-        if v.stride() != strides or (strides[2] != 1 and self.dim > 1) or k.get_device() != device or v.get_device() != device:
-            raise ValueError("k and v must share strides (adjacent elements within a head) and the cache's device")
-        n = slots.numel()
-        to = _ints("slots", slots, n, device)
-        if rows is not None:
-            pick = _ints("rows", rows, n, device)
-        else:
-            pick = 0
-            if n > shape[0]:
-                raise ValueError("more slots than rows")
-        status = self._call(self._at, k.data_ptr(), v.data_ptr(), kind, strides[0], strides[1], shape[0], pick, to, n,
-                            self._flags, _raw_stream(stream, self._index))
+        status = self._call(self._at, self._index, _raw_stream(stream), k, v, slots, rows, self._flags)
         if status:
+            if status == _UNFIT:
+                self._refuse(k, v, slots, rows)
             check(status, "hqb_cache_append")
+
+    def _refuse(self, k, v, slots, rows) -> None:
+        if k.dim() != 3 or k.shape[1] != self.heads or k.shape[2] != self.dim or v.shape != k.shape:
+            raise ValueError(f"k and v must be [tokens, {self.heads}, {self.dim}]")
+        if k.dtype not in _ROW_DTYPES or v.dtype is not k.dtype:
+            raise TypeError("k and v must share a type: float16, bfloat16 or float32")
+        if (v.stride() != k.stride() or (k.stride(2) != 1 and self.dim > 1) or k.get_device() != self._index
+                or v.get_device() != self._index):
+            raise ValueError("k and v must share strides (adjacent elements within a head) and the cache's device")
+        _ints("slots", slots, slots.numel(), self._index)
+        if rows is not None:
+            _ints("rows", rows, slots.numel(), self._index)
+        raise ValueError("more slots than rows")
 
 
 class TreeAttention:
@@ -747,27 +755,15 @@ class TreeAttention:
             raise ValueError("requests and tokens must be positive")
         self.cache, self.q_heads, self.requests, self.tokens = cache, q_heads, requests, tokens
         self.max_new, self.max_context = max_new, max_context
-        args = AttentionC(requests=requests, tokens=tokens, max_new=max_new, max_context=max_context, q_heads=q_heads)
-        need = lib().hqb_tree_attention_workspace_bytes(cache._at, ctypes.addressof(args), cache._index)
+        self._args = AttentionC(requests=requests, tokens=tokens, max_new=max_new, max_context=max_context, q_heads=q_heads)
+        self._at = ctypes.addressof(self._args)
+        need = lib().hqb_tree_attention_workspace_bytes(cache._at, self._at, cache._index)
         if need == 0:
             raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
         self.ws = Workspace(need, cache.device) if workspace is None else workspace(need)
         self._ws, self._ws_bytes = self.ws.ptr(), self.ws.nbytes
-        self._args = ctypes.create_string_buffer(_ATTENTION.size)
-        self._at = ctypes.addressof(self._args)
-        self._call = lib().hqb_tree_attention
-
-    def _refuse(self, tokens: int, q, k, v, out) -> None:
-        """Says which of the row tensors does not fit."""
-        c = self.cache
-        for name, t, heads in (("q", q, self.q_heads), ("k", k, c.heads), ("v", v, c.heads), ("out", out, self.q_heads)):
-            if tuple(t.shape) != (tokens, heads, c.dim):
-                raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}], got {list(t.shape)}")
-            if t.dtype is not c.dtype or t.get_device() != c._index:
-                raise TypeError(f"{name} must have the cache's type and device")
-            if t.stride(2) != 1 and c.dim > 1:
-                raise ValueError(f"{name}: a head's elements must be adjacent")
-        raise ValueError("k and v must share strides")
+        self._scale = cache.dim ** -0.5
+        self._call = bind().tree_attention
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tables: torch.Tensor,
                  context_lens: torch.Tensor, starts: torch.Tensor, mask: torch.Tensor | None = None,
@@ -780,41 +776,37 @@ class TreeAttention:
         up to itself).  scale None: dim ** -0.5.  lse [tokens, q_heads] FP32 gets the logarithm of
         the sum of weights."""
         c = self.cache
-        device, dim, dtype = c._index, c.dim, c.dtype
-        tokens, requests = q.shape[0], context_lens.numel()
         if out is None:
-            out = torch.empty(tokens, self.q_heads, dim, dtype=dtype, device=c.device)
-        rows, news = (tokens, self.q_heads, dim), (tokens, c.heads, dim)
-        qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-        if (q.shape != rows or out.shape != rows or k.shape != news or v.shape != news or q.dtype is not dtype
-                or k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or ks != vs
-                or q.get_device() != device or k.get_device() != device or v.get_device() != device
-                or out.get_device() != device or (dim > 1 and not qs[2] == ks[2] == os[2] == 1)):
-            self._refuse(tokens, q, k, v, out)
-        if requests > self.requests or tokens > self.tokens:
-            raise ValueError(f"built for {self.requests} requests and {self.tokens} tokens, got {requests} and {tokens}")
-        columns = _table("tables", tables, requests, device)
-        ctx = _ints("context_lens", context_lens, requests, device)
-        first = _ints("starts", starts, requests + 1, device)
-        bits = words = 0
-        if mask is not None:
-            words = _table("mask", mask, mask.shape[0], device)
-            if mask.shape[0] < tokens or words * 32 < self.max_new:
-                raise ValueError(f"mask must be [{tokens}, {-(-self.max_new // 32)}] or larger")
-            bits = mask.data_ptr()
-        sums = 0
-        if lse is not None:
-            if (lse.dtype is not torch.float32 or lse.shape != rows[:2] or not lse.is_contiguous()
-                    or lse.get_device() != device):
-                raise ValueError(f"lse must be a contiguous float32 [{tokens}, {self.q_heads}] tensor")
-            sums = lse.data_ptr()
-        _ATTENTION.pack_into(self._args, 0, requests, tokens, self.max_new, self.max_context, self.q_heads, columns, words,
-                             dim ** -0.5 if scale is None else scale, first, ctx, tables.data_ptr(), bits, q.data_ptr(),
-                             k.data_ptr(), v.data_ptr(), out.data_ptr(), sums, qs[0], qs[1], ks[0], ks[1], os[0], os[1])
-        status = self._call(c._at, self._at, self._ws, self._ws_bytes, _raw_stream(stream, device))
+            out = torch.empty(q.shape[0], self.q_heads, c.dim, dtype=c.dtype, device=c.device)
+        status = self._call(c._at, self._at, self._ws, self._ws_bytes, c._index, _raw_stream(stream), q, k, v, tables,
+                            context_lens, starts, mask, self._scale if scale is None else scale, out, lse)
         if status:
+            if status == _UNFIT:
+                self._refuse(q, k, v, tables, context_lens, starts, mask, out, lse)
             check(status, "hqb_tree_attention")
         return out
+
+    def _refuse(self, q, k, v, tables, context_lens, starts, mask, out, lse) -> None:
+        c, tokens, requests = self.cache, q.shape[0], context_lens.numel()
+        for name, t, heads in (("q", q, self.q_heads), ("k", k, c.heads), ("v", v, c.heads), ("out", out, self.q_heads)):
+            if tuple(t.shape) != (tokens, heads, c.dim):
+                raise ValueError(f"{name} must be [{tokens}, {heads}, {c.dim}], got {list(t.shape)}")
+            if t.dtype is not c.dtype or t.get_device() != c._index:
+                raise TypeError(f"{name} must have the cache's type and device")
+            if t.stride(2) != 1 and c.dim > 1:
+                raise ValueError(f"{name}: a head's elements must be adjacent")
+        if k.stride() != v.stride():
+            raise ValueError("k and v must share strides")
+        if requests > self.requests or tokens > self.tokens:
+            raise ValueError(f"built for {self.requests} requests and {self.tokens} tokens, got {requests} and {tokens}")
+        _table("tables", tables, requests, c._index)
+        _ints("context_lens", context_lens, requests, c._index)
+        _ints("starts", starts, requests + 1, c._index)
+        if mask is not None:
+            _table("mask", mask, mask.shape[0], c._index)
+            if mask.shape[0] < tokens or mask.shape[1] * 32 < self.max_new:
+                raise ValueError(f"mask must be [{tokens}, {-(-self.max_new // 32)}] or larger")
+        raise ValueError(f"lse must be a contiguous float32 [{tokens}, {self.q_heads}] tensor")
 
 
 class LoraSet:
@@ -847,10 +839,10 @@ class LoraSet:
         self.c = LoraSetC(a.data_ptr(), b.data_ptr(), _ptr(ranks), _ptr(scales), self.rows, self.cols, self.adapters,
                           self.max_rank, _SERVING_DTYPES[a.dtype], 0)
         self._at, self._index = ctypes.addressof(self.c), _device_index(a.device)
-        self._call = lib().hqb_lora
+        self._call = bind().lora
         self._ws: dict = {}
         if max_tokens > 0:
-            self.workspace(max_tokens, _raw_stream(None, self._index))
+            self.workspace(max_tokens, torch.cuda.current_stream(a.device).cuda_stream)
 
     def workspace_bytes(self, tokens: int) -> int:
         return lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
@@ -860,7 +852,7 @@ class LoraSet:
         ws = self._ws.get(stream)
         if ws is None or tokens > ws.tokens:
             need = self.workspace_bytes(tokens)
-            if stream == _raw_stream(None, self._index):
+            if stream == torch.cuda.current_stream(self.device).cuda_stream:
                 ws = Workspace(need, self.device)
             else:  # allocated on the stream that uses it: the allocator then reuses it in that order
                 with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
@@ -869,43 +861,39 @@ class LoraSet:
             self._ws[stream] = ws
         return ws
 
-    def _out(self, name: str, t: torch.Tensor, tokens: int, kind) -> int:
-        shape, strides = t.shape, t.stride()
-        if shape != (tokens, self.rows) or t.dtype is not kind or t.get_device() != self._index:
-            raise ValueError(f"{name} must be [{tokens}, {self.rows}] {kind} on {self.device}")
-        if (strides[1] != 1 and self.rows > 1) or (strides[0] < self.rows and tokens > 1):
-            raise ValueError(f"{name}: a row's elements must be adjacent, and rows must not overlap")
-        return strides[0] if tokens > 1 else self.rows  # torch leaves any stride on a single row
-
     def apply(self, x: torch.Tensor, ids: torch.Tensor, base: torch.Tensor | None = None,
               out: torch.Tensor | None = None, y_dtype: torch.dtype | None = None, workspace: Workspace | None = None,
               stream=None) -> torch.Tensor:
         """base + scale_i * b_i (a_i x) per token, i = ids[token] (negative: base alone) (hqb_lora).
         x [tokens, cols]; base [tokens, rows] (None: zeros) and the result share a type, the
         set's or FP32.  out=base adds in place, e.g. to the output of a projection's gemv()."""
-        shape, strides = x.shape, x.stride()
-        if len(shape) != 2 or shape[1] != self.cols or x.dtype is not self.dtype or x.get_device() != self._index:
-            raise ValueError(f"x must be [tokens, {self.cols}] {self.dtype} on {self.device}")
-        tokens = shape[0]
-        if (strides[1] != 1 and self.cols > 1) or (strides[0] < self.cols and tokens > 1):
-            raise ValueError("x: a row's elements must be adjacent, and rows must not overlap")
         if out is None:
             kind = y_dtype or (base.dtype if base is not None else x.dtype)
-            out = torch.empty(tokens, self.rows, dtype=kind, device=self.device)
-        kind = out.dtype
-        if kind is not self.dtype and kind is not torch.float32:
-            raise TypeError("the result must have the set's type or float32")
-        which = _ints("ids", ids, tokens, self._index)
-        y_stride, base_stride, base_at = self._out("out", out, tokens, kind), 0, 0
-        if base is not None:
-            base_stride, base_at = self._out("base", base, tokens, kind), base.data_ptr()
-        s = _raw_stream(stream, self._index)
-        ws = workspace or self.workspace(tokens, s)
-        status = self._call(self._at, x.data_ptr(), strides[0] if tokens > 1 else self.cols, which, tokens, base_at,
-                            base_stride, out.data_ptr(), _ROW_DTYPES[kind], y_stride, ws.ptr(), ws.nbytes, s)
+            out = torch.empty(x.shape[0], self.rows, dtype=kind, device=self.device)
+        s = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else _raw_stream(stream)
+        ws = workspace or self._ws.get(s)
+        if ws is None or (workspace is None and x.shape[0] > ws.tokens):
+            ws = self.workspace(x.shape[0], s)
+        status = self._call(self._at, ws.ptr(), ws.nbytes, self._index, s, x, ids, base, out)
         if status:
+            if status == _UNFIT:
+                self._refuse(x, ids, base, out)
             check(status, "hqb_lora")
         return out
+
+    def _refuse(self, x, ids, base, out) -> None:
+        tokens = x.shape[0]
+        for name, t, cols, kinds in (("x", x, self.cols, (self.dtype,)), ("out", out, self.rows, (self.dtype, torch.float32)),
+                                     ("base", base, self.rows, (out.dtype,))):
+            if t is None:
+                continue
+            if tuple(t.shape) != (tokens, cols) or t.get_device() != self._index:
+                raise ValueError(f"{name} must be [{tokens}, {cols}] on {self.device}, got {list(t.shape)}")
+            if t.dtype not in kinds:
+                raise TypeError(f"{name} must be {' or '.join(map(str, kinds))}, got {t.dtype}")
+            if (t.stride(1) != 1 and cols > 1) or (t.stride(0) < cols and tokens > 1):
+                raise ValueError(f"{name}: a row's elements must be adjacent, and rows must not overlap")
+        _ints("ids", ids, tokens, self._index)
 
 
 # ---- output-row sharding across ranks --------------------------------------------------
