@@ -13,10 +13,13 @@ namespace {
 
 constexpr uint32_t kKeyBlock = 64;
 constexpr uint32_t kChunk = 16;  // keys a warp takes at once
-constexpr uint32_t kStages = 3;  // chunks of a warp's ring
 
+// Chunks of a warp's ring, and a CTA's shared memory: the rings, over which the warps' sums are
+// joined at an item's end.
+template <int kRowsWarps>
+constexpr uint32_t kStagesOf = kRowsWarps == 2 ? 2 : 3;
 template <int DP, int kRowsWarps>
-constexpr uint32_t kRowsSmem = kRowsWarps * kStages * 2 * kChunk * DP * 2;
+constexpr uint32_t kRowsSmem = kRowsWarps * kStagesOf<kRowsWarps> * 2 * kChunk * DP * 2;
 
 // Mathematics: the softmax over the keys in one pass.  A warp keeps, per row, the running
 // maximum m of t = scale*log2(e) * q.k, the sum l of 2^(t - m) and the sums O of 2^(t - m) v;
@@ -26,13 +29,15 @@ constexpr uint32_t kRowsSmem = kRowsWarps * kStages * 2 * kChunk * DP * 2;
 // ring of asynchronous copies, so the loop has no CTA barrier and keeps 2 chunks (16 KB at 128
 // dimensions) a warp in flight; the warps are joined once per segment.  Rows: the group's heads
 // of all nodes share the keys, so a key is read once per 16 rows.
-// Warps: four, two CTAs an SM, so that one CTA's ends of segments lie under the other's copies; eight
-// where items are not cut (up to 512 keys: every copy is then in flight at once).
+// Warps: four, two CTAs an SM, so that one CTA's ends of segments lie under the other's copies.  Where
+// items are not cut (up to 512 keys): eight for few items, every copy then in flight at once; two for
+// more items than SMs, with six CTAs an SM.
 // Bound by HBM at 16 rows: 32 MMAs a chunk are about 310 cycles of one of the four tensor pipes
 // a chunk against 1400 cycles an SM needs to fetch four chunks.
 template <typename T, int DP, bool VEC, int kRowsWarps>
-__global__ void __launch_bounds__(kRowsWarps * 32) attention_rows_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kRowsWarps * 32, kRowsWarps == 2 && DP <= 128 ? 6 : 1) attention_rows_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t sm[];
+  constexpr uint32_t kStages = kStagesOf<kRowsWarps>;
   constexpr uint32_t kRowBytes = DP * 2, kTileBytes = kChunk * kRowBytes, kStageBytes = 2 * kTileBytes;
   constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
   constexpr int kSteps = DP / 16;
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
 }
 
 struct Shape {
-  uint32_t rows, block, max_tiles, dim_pad, grid, whole, tmem;
+  uint32_t rows, block, max_tiles, dim_pad, grid, whole, warps, tmem;
   uint64_t splits_bytes, parts_bytes;
   uint64_t bytes() const { return 256 + round_up(splits_bytes + parts_bytes, 256); }  // with the error word
 };
@@ -491,10 +496,16 @@ Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem,
   s.max_tiles = (a->max_new * group + s.rows - 1) / s.rows;
   s.grid = static_cast<uint32_t>(sms) * (tmem || s.dim_pad == 256 ? 1u : 2u);
   const uint64_t items = static_cast<uint64_t>(a->requests) * c->kv_heads * s.max_tiles;
-  // up to 8 blocks a request: an item is one CTA's work of a few microseconds, and cutting it
-  // would add a second launch
+  // up to 512 keys a request: an item is one CTA's work of a few microseconds, and cutting it would
+  // add a second launch
   s.whole = static_cast<uint64_t>(a->max_context) + a->max_new <= 512 ? 1u : 0u;
-  if (s.whole) s.grid = static_cast<uint32_t>(items < s.grid * 4ull ? (items > 0 ? items : 1) : s.grid * 4ull);
+  s.warps = 4;
+  if (s.whole) {
+    // few items: eight warps each; more than SMs: two, six CTAs an SM
+    s.warps = tmem || s.dim_pad == 256 ? 4u : items <= static_cast<uint64_t>(sms) ? 8u : 2u;
+    const uint64_t slots = tmem ? sms : static_cast<uint64_t>(sms) * (s.warps == 2 ? 6 : 1);
+    s.grid = static_cast<uint32_t>(items < slots ? (items > 0 ? items : 1) : slots);
+  }
   s.splits_bytes = s.whole ? 0 : static_cast<uint64_t>(s.grid) * sizeof(Split);
   s.parts_bytes = s.whole ? 0 : static_cast<uint64_t>(s.grid) * 2 * s.rows * (s.dim_pad + 2) * 4;
   return s;
@@ -512,8 +523,10 @@ cudaError_t launch_warps(const AttnParams& p, cudaStream_t st) {
 
 template <typename T, int DP, bool VEC>
 cudaError_t launch_rows(const AttnParams& p, cudaStream_t st) {
-  if constexpr (DP <= 128)
-    if (p.whole) return launch_warps<T, DP, VEC, 8>(p, st);
+  if constexpr (DP <= 128) {
+    if (p.warps == 2) return launch_warps<T, DP, VEC, 2>(p, st);
+    if (p.warps == 8) return launch_warps<T, DP, VEC, 8>(p, st);
+  }
   return launch_warps<T, DP, VEC, 4>(p, st);
 }
 
@@ -586,6 +599,7 @@ HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_arg
   p.min_blocks = 4;
   p.whole = s.whole;
   p.grid = s.grid;
+  p.warps = s.warps;
   p.vec = vec ? 1u : 0u;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   cudaStream_t st = as_stream(stream);

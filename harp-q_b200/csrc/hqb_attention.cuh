@@ -30,6 +30,7 @@ struct AttnParams {
   uint32_t min_blocks;  // fewest blocks worth a CTA of its own
   uint32_t whole;       // 1: items are not cut (a unit is an item, no partials)
   uint32_t grid;        // CTAs of the attention kernel
+  uint32_t warps;       // of a CTA of the rows kernel
   uint32_t vec;         // 16-byte accesses fit every row
   float scale_log2;     // scale * log2(e)
 };
