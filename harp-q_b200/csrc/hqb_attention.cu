@@ -14,12 +14,10 @@ namespace {
 constexpr uint32_t kKeyBlock = 64;
 constexpr uint32_t kChunk = 16;  // keys a warp takes at once
 
-// Chunks of a warp's ring, and a CTA's shared memory: the rings, over which the warps' sums are
-// joined at an item's end.
-template <int kRowsWarps>
-constexpr uint32_t kStagesOf = kRowsWarps == 2 ? 2 : 3;
-template <int DP, int kRowsWarps>
-constexpr uint32_t kRowsSmem = kRowsWarps * kStagesOf<kRowsWarps> * 2 * kChunk * DP * 2;
+// A CTA's shared memory: the warps' rings of kStages chunks, over which their sums are joined at an
+// item's end.
+template <int DP, int kRowsWarps, int kStages>
+constexpr uint32_t kRowsSmem = kRowsWarps * kStages * 2 * kChunk * DP * 2;
 
 // Mathematics: the softmax over the keys in one pass.  A warp keeps, per row, the running
 // maximum m of t = scale*log2(e) * q.k, the sum l of 2^(t - m) and the sums O of 2^(t - m) v;
@@ -30,14 +28,13 @@ constexpr uint32_t kRowsSmem = kRowsWarps * kStagesOf<kRowsWarps> * 2 * kChunk *
 // dimensions) a warp in flight; the warps are joined once per segment.  Rows: the group's heads
 // of all nodes share the keys, so a key is read once per 16 rows.
 // Warps: four, two CTAs an SM, so that one CTA's ends of segments lie under the other's copies.  Where
-// items are not cut (up to 512 keys): eight for few items, every copy then in flight at once; two for
-// more items than SMs, with six CTAs an SM.
+// items are not cut (up to 512 keys): eight for few items, every copy then in flight at once; four
+// or two for more items than SMs, with twelve warps an SM in CTAs of their own.
 // Bound by HBM at 16 rows: 32 MMAs a chunk are about 310 cycles of one of the four tensor pipes
 // a chunk against 1400 cycles an SM needs to fetch four chunks.
-template <typename T, int DP, bool VEC, int kRowsWarps>
-__global__ void __launch_bounds__(kRowsWarps * 32, kRowsWarps == 2 && DP <= 128 ? 6 : 1) attention_rows_kernel(const __grid_constant__ AttnParams p) {
+template <typename T, int DP, bool VEC, int kRowsWarps, int kStages>
+__global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarps : 1) attention_rows_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t sm[];
-  constexpr uint32_t kStages = kStagesOf<kRowsWarps>;
   constexpr uint32_t kRowBytes = DP * 2, kTileBytes = kChunk * kRowBytes, kStageBytes = 2 * kTileBytes;
   constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
   constexpr int kSteps = DP / 16;
@@ -299,7 +296,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kRowsWarps == 2 && DP <= 128 
     // join the warps: sums in shared memory over the (drained) rings, [warp][16][DP + 2]
     __syncthreads();
     constexpr uint32_t kPitch = DP + 2;
-    static_assert(kRowsWarps * 16 * kPitch * 4 <= kRowsSmem<DP, kRowsWarps>, "the join area fits the rings");
+    static_assert(kRowsWarps * 16 * kPitch * 4 <= kRowsSmem<DP, kRowsWarps, kStages>, "the join area fits the rings");
     float* joint = reinterpret_cast<float*>(sm);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -470,11 +467,18 @@ bool aligned_rows(const hqb_paged_cache* c, const hqb_attention_args* a) {
   return (addresses & 15u) == 0 && (strides & 7u) == 0;
 }
 
+// Items of up to 512 keys are not cut: one CTA's work of a few microseconds, where cutting it would
+// add a second launch.
+bool whole_items(const hqb_attention_args* a) { return static_cast<uint64_t>(a->max_context) + a->max_new <= 512; }
+
 // Whether the tensor-memory kernel can take a shape: heads of up to 128, groups that fit a score
-// tile, more rows than one tile of the rows kernel.
+// tile, more rows than one tile of the rows kernel, or than two where items are not cut.  B200, us,
+// rows / tensor-memory kernel, BF16, 64 heads over 8 of 128: 51 requests of 3 nodes and 1 token 14.7 /
+// 24.6; 40 of 9 and 58 tokens 27.3 / 23.8; 32 of 64 and 400 tokens 194 / 66; 16 requests over 4096
+// tokens: 2 nodes 45 / -, 4 nodes 97 / 53.
 bool tmem_shape(const hqb_paged_cache* c, const hqb_attention_args* a) {
   const uint32_t group = a->q_heads / c->kv_heads;
-  return c->head_dim <= 128 && group <= 128 && a->max_new * group > 16;
+  return c->head_dim <= 128 && group <= 128 && a->max_new * group > (whole_items(a) ? 32u : 16u);
 }
 
 // ... and the call: its masked scores are -inf * scale; a stride of zero (a broadcast input) or
@@ -496,14 +500,13 @@ Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem,
   s.max_tiles = (a->max_new * group + s.rows - 1) / s.rows;
   s.grid = static_cast<uint32_t>(sms) * (tmem || s.dim_pad == 256 ? 1u : 2u);
   const uint64_t items = static_cast<uint64_t>(a->requests) * c->kv_heads * s.max_tiles;
-  // up to 512 keys a request: an item is one CTA's work of a few microseconds, and cutting it would
-  // add a second launch
-  s.whole = static_cast<uint64_t>(a->max_context) + a->max_new <= 512 ? 1u : 0u;
+  s.whole = whole_items(a) ? 1u : 0u;
   s.warps = 4;
   if (s.whole) {
-    // few items: eight warps each; more than SMs: two, six CTAs an SM
-    s.warps = tmem || s.dim_pad == 256 ? 4u : items <= static_cast<uint64_t>(sms) ? 8u : 2u;
-    const uint64_t slots = tmem ? sms : static_cast<uint64_t>(sms) * (s.warps == 2 ? 6 : 1);
+    // few items: eight warps each; more than SMs: four, or two, twelve warps an SM
+    const uint64_t n = static_cast<uint64_t>(sms);
+    s.warps = items <= n ? 8u : items <= 3 * n ? 4u : 2u;
+    const uint64_t slots = n * (tmem || s.dim_pad == 256 || s.warps == 8 ? 1 : 12 / s.warps);
     s.grid = static_cast<uint32_t>(items < slots ? (items > 0 ? items : 1) : slots);
   }
   s.splits_bytes = s.whole ? 0 : static_cast<uint64_t>(s.grid) * sizeof(Split);
@@ -511,23 +514,24 @@ Shape shape_of(const hqb_paged_cache* c, const hqb_attention_args* a, bool tmem,
   return s;
 }
 
-template <typename T, int DP, bool VEC, int kRowsWarps>
+template <typename T, int DP, bool VEC, int kRowsWarps, int kStages>
 cudaError_t launch_warps(const AttnParams& p, cudaStream_t st) {
   static DeviceOnce once;
-  constexpr uint32_t smem = kRowsSmem<DP, kRowsWarps>;
+  constexpr uint32_t smem = kRowsSmem<DP, kRowsWarps, kStages>;
   const cudaError_t e =
-      allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_rows_kernel<T, DP, VEC, kRowsWarps>), smem);
+      allow_dynamic_smem(once, reinterpret_cast<const void*>(attention_rows_kernel<T, DP, VEC, kRowsWarps, kStages>), smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(attention_rows_kernel<T, DP, VEC, kRowsWarps>, dim3(p.grid), kRowsWarps * 32, smem, 1, st, p);
+  return launch_dependent(attention_rows_kernel<T, DP, VEC, kRowsWarps, kStages>, dim3(p.grid), kRowsWarps * 32, smem, 1, st, p);
 }
 
 template <typename T, int DP, bool VEC>
 cudaError_t launch_rows(const AttnParams& p, cudaStream_t st) {
   if constexpr (DP <= 128) {
-    if (p.warps == 2) return launch_warps<T, DP, VEC, 2>(p, st);
-    if (p.warps == 8) return launch_warps<T, DP, VEC, 8>(p, st);
+    if (p.whole && p.warps == 2) return launch_warps<T, DP, VEC, 2, 2>(p, st);
+    if (p.whole && p.warps == 4) return launch_warps<T, DP, VEC, 4, 2>(p, st);
+    if (p.whole) return launch_warps<T, DP, VEC, 8, 3>(p, st);
   }
-  return launch_warps<T, DP, VEC, 4>(p, st);
+  return launch_warps<T, DP, VEC, 4, 3>(p, st);
 }
 
 template <typename T, bool VEC>
