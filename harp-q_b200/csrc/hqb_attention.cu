@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarp
     auto load = [&](uint32_t i, uint32_t stage, uint64_t where) {
       uint32_t key, valid;
       const bool drafted = place(i, key, valid);
+      if (valid == 0) return;  // not read either
       const T* ks = drafted ? kn : kc;
       const T* vs = drafted ? vn : vc;
       const uint32_t base = ring_a + stage * kStageBytes;
