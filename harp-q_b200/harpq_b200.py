@@ -841,6 +841,7 @@ class LoraSet:
         self._at, self._index = ctypes.addressof(self.c), _device_index(a.device)
         self._call = bind().lora
         self._ws: dict = {}
+        self._kept: list = []
         if max_tokens > 0:
             self.workspace(max_tokens, torch.cuda.current_stream(a.device).cuda_stream)
 
@@ -848,9 +849,11 @@ class LoraSet:
         return lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
 
     def workspace(self, tokens: int, stream: int) -> Workspace:
-        """The stream's workspace, grown to what `tokens` tokens need."""
+        """The stream's workspace, grown to what `tokens` tokens need (in powers of two; the smaller
+        ones stay too, since a captured graph may hold them)."""
         ws = self._ws.get(stream)
         if ws is None or tokens > ws.tokens:
+            tokens = 1 << (tokens - 1).bit_length()
             need = self.workspace_bytes(tokens)
             if stream == torch.cuda.current_stream(self.device).cuda_stream:
                 ws = Workspace(need, self.device)
@@ -859,6 +862,7 @@ class LoraSet:
                     ws = Workspace(need, self.device)
             ws.tokens = tokens
             self._ws[stream] = ws
+            self._kept.append(ws)
         return ws
 
     def apply(self, x: torch.Tensor, ids: torch.Tensor, base: torch.Tensor | None = None,

@@ -97,16 +97,18 @@ def _gemv_fake(x, planes, rows, cols, prefix, bias=None, out_dtype=torch.float16
 #   lora(x, a, b, ids, ranks, scales, base, out_dtype)         -> [tokens, rows]
 #
 # The same calls and the same bits as PagedCache.append, TreeAttention and LoraSet.apply, whose
-# arguments they share, without a handle to keep.  Workspaces are cached per stream and grown.
+# arguments they share, without a handle to keep.  Workspaces are cached per stream in sizes of powers
+# of two, none of which is freed: a captured graph may hold it.
 
 _SERVING_WORKSPACES: dict = {}
 
 
 def _serving_workspace(kind: str, device: torch.device, stream: int, need: int) -> "hqb.Workspace":
-    key = (kind, device.index, stream)
+    size = 1 << (need - 1).bit_length()
+    key = (kind, device.index, stream, size)
     ws = _SERVING_WORKSPACES.get(key)
-    if ws is None or ws.nbytes < need:
-        ws = _SERVING_WORKSPACES[key] = hqb.Workspace(need, device)
+    if ws is None:
+        ws = _SERVING_WORKSPACES[key] = hqb.Workspace(size, device)
     return ws
 
 

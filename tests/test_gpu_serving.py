@@ -708,6 +708,34 @@ def test_lora_streams_and_graphs(tokens):
     assert torch.equal(out, base)
 
 
+def test_lora_graph_outlives_a_larger_call():
+    """A captured call keeps its workspace when a later call needs a larger one."""
+    import harpq_b200_ops  # noqa: F401
+
+    x, a, b, ranks, scales, ids, base = make_lora(9, 3000, 512, 256, 4, 32, BF16, BF16)
+    s = hqb.LoraSet(a, b, ranks, scales, max_tokens=300)
+    out, few = torch.empty_like(base[:300]), (x[:300], ids[:300])
+    want = s.apply(*few, base=base[:300])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # as a capture wants it: warmed up on its stream
+        s.apply(*few, base=base[:300], out=out)
+        torch.ops.harpq_b200.lora(x[:300], a, b, ids[:300], ranks, scales, base[:300])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s.apply(*few, base=base[:300], out=out)
+            other = torch.ops.harpq_b200.lora(x[:300], a, b, ids[:300], ranks, scales, base[:300])
+        s.apply(x, ids, base=base)
+        torch.ops.harpq_b200.lora(x, a, b, ids, ranks, scales, base)
+        filler = [torch.full((1 << 20,), -1, dtype=torch.int32, device="cuda") for _ in range(8)]  # takes what was freed
+        out.zero_()
+        graph.replay()
+        filler.append(filler[0].clone())
+    side.synchronize()
+    assert torch.equal(out, want) and torch.equal(other, want)
+    assert all(bool((f == -1).all()) for f in filler)
+
+
 def test_lora_beside_a_plane_matrix():
     """In place on a quantized projection's output, as a decoder layer runs it."""
     from conftest import plane_matrix, random_matrix
