@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarp
       for (int e = 0; e < 2; ++e) {
         const uint32_t row = row0 + g + 8 * e;
         live[e] = row < rows;
-        node[e] = live[e] ? row / p.group : 0u;
+        node[e] = live[e] ? p.by_group.quotient(row) : 0u;
         const uint32_t h = w.head * p.group + (live[e] ? row - node[e] * p.group : 0u);
         src[e] = static_cast<const T*>(p.a.q) + (q.start + node[e]) * p.a.q_token_stride + h * p.a.q_head_stride;
       }
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarp
       const uint32_t at = row0 + row;
       const bool complete = w.complete();
       if (at < rows) {
-        const uint32_t nd = at / p.group, h = w.head * p.group + at - nd * p.group;
+        const uint32_t nd = p.by_group.quotient(at), h = w.head * p.group + at - nd * p.group;
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
         T* out = static_cast<T*>(p.a.out) + (q.start + nd) * p.a.out_token_stride + h * p.a.out_head_stride;
         float* keep = part_sums(p, blockIdx.x, w.b0 == 0 ? 1u : 0u) + row * 4;
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
   const uint32_t rows = q.nodes * p.group, dim = p.c.head_dim;
   if (q.tile * p.rows + row0 >= rows) return;
   auto place = [&](uint32_t r, uint32_t& token, uint32_t& head) {
-    const uint32_t at = q.tile * p.rows + r, node = at / p.group;
+    const uint32_t at = q.tile * p.rows + r, node = p.by_group.quotient(at);
     token = q.start + node;
     head = q.head * p.group + at - node * p.group;
   };
@@ -598,7 +598,10 @@ HQB_API int hqb_tree_attention(const hqb_paged_cache* c, const hqb_attention_arg
   p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256 + s.splits_bytes);
   p.group = a->q_heads / c->kv_heads;
   p.rows = s.rows;
-  p.block = s.block;
+  p.block_shift = s.block == 128 ? 7 : 6;
+  p.by_page = Divisor::of(c->page_size);
+  p.by_group = Divisor::of(p.group);
+  p.by_rows = Divisor::of(p.rows);
   p.max_tiles = s.max_tiles;
   p.dim_pad = s.dim_pad;
   p.min_blocks = 4;

@@ -14,6 +14,20 @@
 
 namespace hqb {
 
+// Quotients by a number that the host knows (Granlund and Montgomery, 1994), for n < 2^31: with
+// s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (n + floor(m n / 2^32)) >> s.  Four
+// instructions; the kernels' single warps that place copies waited for the usual thirty.
+struct Divisor {
+  uint32_t m, s;
+  static Divisor of(uint32_t d) {
+    Divisor v{0, 0};
+    while (v.s < 31 && (1u << v.s) < d) ++v.s;
+    v.m = static_cast<uint32_t>((((1ull << v.s) - d) << 32) / d) + 1;
+    return v;
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (n + __umulhi(m, n)) >> s; }
+};
+
 struct Split;
 
 struct AttnParams {
@@ -24,7 +38,8 @@ struct AttnParams {
   float* parts;         // [cta][2] partial results: see part_sums
   uint32_t group;       // query heads per key head
   uint32_t rows;        // rows of a row tile
-  uint32_t block;       // keys of a block
+  uint32_t block_shift; // log2 of the keys of a block
+  Divisor by_page, by_group, by_rows;
   uint32_t max_tiles;   // row tiles of max_new nodes
   uint32_t dim_pad;     // padded head dimension (columns of a partial row)
   uint32_t min_blocks;  // fewest blocks worth a CTA of its own
@@ -64,9 +79,10 @@ __device__ __forceinline__ Request load_request(const AttnParams& p, uint32_t r,
     bad |= HQB_DEVERR_PAGES;
     q.ctx = static_cast<uint32_t>(room);
   }
-  q.cached_blocks = (q.ctx + p.block - 1) / p.block;
-  q.blocks = q.nodes == 0 ? 0u : q.cached_blocks + (q.nodes + p.block - 1) / p.block;
-  q.tiles = (q.nodes * p.group + p.rows - 1) / p.rows;
+  const uint32_t over = (1u << p.block_shift) - 1;
+  q.cached_blocks = (q.ctx + over) >> p.block_shift;
+  q.blocks = q.nodes == 0 ? 0u : q.cached_blocks + ((q.nodes + over) >> p.block_shift);
+  q.tiles = p.by_rows.quotient(q.nodes * p.group + p.rows - 1);
   return q;
 }
 
@@ -216,7 +232,7 @@ __device__ __forceinline__ float2* part_stats(const AttnParams& p, uint32_t cta,
 // Address of one cached key's row in k or v (elements from the base), its page checked.
 __device__ __forceinline__ uint64_t key_offset(const AttnParams& p, const int32_t* table, uint32_t key, uint32_t head,
                                                uint32_t& bad) {
-  const uint32_t column = key / p.c.page_size, inside = key - column * p.c.page_size;
+  const uint32_t column = p.by_page.quotient(key), inside = key - column * p.c.page_size;
   uint32_t page = static_cast<uint32_t>(__ldg(table + column));
   if (page >= p.c.num_pages) {
     bad |= HQB_DEVERR_PAGES;

@@ -153,10 +153,13 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         // slots (a slot's turns can only be told apart by the warp that waits for each of them): the
         // loading warp, or without maps of the cache the copying warp.  The copying warp hands on
         // the values whose last rows have to be cleared.  Each slot is announced once on kv_full.
-        const bool copier = warp == kCopyWarp, filler = copier == (maps.box_rows == 0);
+        const bool copier = warp == kCopyWarp, mapped = maps.box_rows != 0, filler = copier != mapped;
         constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
         const uint32_t dim = p.c.head_dim;
-        uint32_t issued = 0, seg = 0, fixes = 0;
+        // a lane a box: box `box` of the block, columns 64 h ..
+        const uint32_t box_shift = mapped ? 31 - __clz(maps.box_rows) : 0;
+        const uint32_t h = lane >> (7 - box_shift), box = lane & ((kKeys >> box_shift) - 1);
+        uint32_t slot = 0, pass = 0, seg = 0, fixes = 0;
         uint32_t sent_fix = 0, sent_turn = 0;  // filler, a bit a slot: its last copy goes to fix_full, that one's phase
         bool ok = true;
         while (ok && w.left != 0) {
@@ -166,120 +169,129 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           const bool two = rows - row0 > half;
           const int32_t* table = p.a.tables + static_cast<uint64_t>(w.r) * p.a.table_stride;
           uint32_t* broken = bars.broken[seg & 7];
-          auto load = [&](uint32_t b, bool values) {
-            const uint32_t slot = issued % S::kSlots, turn = issued / S::kSlots - 1;
-            const bool reuse = issued >= S::kSlots;
-            ++issued;
-            if (!ok) return;
+          // the lane's box of a block of keys: its page is looked up while the block before is loaded, and
+          // kept for the values
+          struct Place {
+            uint32_t page, inside;
+          };
+          auto locate = [&](uint32_t b) -> Place {
+            const uint32_t key = b * kKeys + (box << box_shift), column = p.by_page.quotient(key);
+            const bool real = b < q.cached_blocks && key < q.ctx && h < DP / 64;
+            return {real ? static_cast<uint32_t>(__ldg(table + column)) : 0u, key - column * p.c.page_size};
+          };
+          Place ahead{}, keys{}, before{};  // of the next block of keys, of the last one and of the one before it
+          if (!copier && mapped) ahead = locate(w.b0);
+          auto drafted = [&](uint32_t dst, uint64_t* bar, uint32_t first, bool values) {
+            if (lane == 0) mbar_expect_tx(bar, S::kTile);
+            __syncwarp();
+            if (lane < DP / 64)
+              tma_load_3d(dst + lane * S::kHalf, values ? &maps.v : &maps.k, bar, lane * 64, w.head, q.start + first);
+          };
+          // K0 V0 K1 V1 ... for two score tiles over the same keys, K0 K1 V0 K2 V1 ... Vn-2 Vn-1 for two
+          // streams of blocks.  (Instructions are fetched from as far as L2, so the loops here are kept
+          // short, and divisions out of them: with four a copy the loading warp took 1900 cycles each, and
+          // everything waited for it.)
+          for (uint32_t x = 0; x < 2 * n; ++x) {
+            const bool last = x == 2 * n - 1;
+            const bool values = two ? (x & 1) != 0 : last || (x != 0 && (x & 1) == 0);
+            const uint32_t b = w.b0 + (two ? x / 2 : last ? n - 1 : values ? x / 2 - 1 : (x + 1) / 2);
             const bool cached = b < q.cached_blocks;
             const uint32_t first = (cached ? b : b - q.cached_blocks) * kKeys;
             const uint32_t valid = min(kKeys, (cached ? q.ctx : q.nodes) - first);
             const bool fix = values && (!cached || valid < kKeys);  // rows to clear
             uint8_t* const at = sm + S::kRing + slot * S::kTile;
             const uint32_t dst = smem_u32(at);
-            if (filler && reuse) ok = wait_all(&bars.kv_empty[slot], turn);
-            if (!ok) return;
-            if (cached && maps.box_rows == 0) {
-              if (!filler) return;
-              const T* src = static_cast<const T*>(values ? p.c.v : p.c.k);
-              for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
-                const uint64_t where = r0 + lane < valid ? key_offset(p, table, first + r0 + lane, w.head, bad) : 0;
-#pragma unroll 4
-                for (uint32_t x = 0; x < kPieces; ++x) {
-                  const uint32_t i = x * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
-                  const uint64_t row = __shfl_sync(0xffffffffu, where, j);
-                  const bool copy = r < valid && c * 8 < dim;
-                  cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
-                             copy ? 16u : 0u);
-                }
-              }
-              cp_async_commit();
-              cp_async_wait<0>();
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
-              return;
-            }
             if (filler) {
+              if (pass > 0 && !(ok = wait_all(&bars.kv_empty[slot], pass - 1))) break;
               uint64_t* bar = fix ? &bars.fix_full[slot] : &bars.kv_full[slot];
-              sent_fix = fix ? sent_fix | 1u << slot : sent_fix & ~(1u << slot);
-              if (fix) sent_turn ^= 1u << slot;
-              if (cached) {
-                // a lane a box; boxes past the end of the context are left out (scores of what lies there
-                // are hidden, values are cleared)
-                const uint32_t boxes = kKeys / maps.box_rows, real = (valid + maps.box_rows - 1) / maps.box_rows;
-                const uint32_t box = lane % boxes, h = lane / boxes;
-                if (lane == 0) mbar_expect_tx(bar, real * maps.box_rows * DP * 2);
-                __syncwarp();
-                if (h < DP / 64 && box < real) {
-                  const uint32_t key = first + box * maps.box_rows, column = key / p.c.page_size;
-                  uint32_t page = static_cast<uint32_t>(__ldg(table + column));
-                  if (page >= p.c.num_pages) {
-                    bad |= HQB_DEVERR_PAGES;
-                    page = 0;
-                  }
-                  tma_load_4d(dst + h * S::kHalf + box * maps.box_rows * 128, values ? &maps.cv : &maps.ck, bar, h * 64, w.head,
-                              key - column * p.c.page_size, page);
+              if (!copier || !cached) {
+                sent_fix = fix ? sent_fix | 1u << slot : sent_fix & ~(1u << slot);
+                if (fix) sent_turn ^= 1u << slot;
+              }
+              if (!copier && !values) {
+                before = keys;
+                keys = ahead;
+                if (keys.page >= p.c.num_pages) {
+                  bad |= HQB_DEVERR_PAGES;
+                  keys.page = 0;
                 }
+                if (b + 1 < w.b1) ahead = locate(b + 1);
+              }
+              if (!cached) {
+                drafted(dst, bar, first, values);
+              } else if (!copier) {
+                const Place here = two || last || !values ? keys : before;
+                // boxes past the end of the context are left out (scores of what lies there are hidden, values
+                // are cleared)
+                const uint32_t real = (valid + maps.box_rows - 1) >> box_shift;
+                if (lane == 0) mbar_expect_tx(bar, (real << box_shift) * (DP * 2));
+                __syncwarp();
+                if (h < DP / 64 && box < real)
+                  tma_load_4d(dst + h * S::kHalf + (box << box_shift) * 128, values ? &maps.cv : &maps.ck, bar, h * 64, w.head,
+                              here.inside, here.page);
               } else {
-                if (lane == 0) mbar_expect_tx(bar, S::kTile);
-                __syncwarp();
-                if (lane < DP / 64)
-                  tma_load_3d(dst + lane * S::kHalf, values ? &maps.v : &maps.k, bar, lane * 64, w.head, q.start + first);
+                const T* src = static_cast<const T*>(values ? p.c.v : p.c.k);
+                for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
+                  const uint64_t where = r0 + lane < valid ? key_offset(p, table, first + r0 + lane, w.head, bad) : 0;
+#pragma unroll 4
+                  for (uint32_t y = 0; y < kPieces; ++y) {
+                    const uint32_t i = y * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
+                    const uint64_t row = __shfl_sync(0xffffffffu, where, j);
+                    const bool copy = r < valid && c * 8 < dim;
+                    cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
+                               copy ? 16u : 0u);
+                  }
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_proxy_async_smem();
+                arrive_warp(&bars.kv_full[slot]);
               }
             }
-            if (!copier || !fix) return;
-            ok = wait_all(&bars.fix_full[slot], fixes >> slot);
-            if (!ok) return;
-            fixes ^= 1u << slot;
-            // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
-            // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
-            // node get at the end
-            auto piece = [&](uint32_t i) {
-              const uint32_t r = i / kPieces, c = i % kPieces;
-              return reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-            };
-            // (the sums' MMAs stop after the 16 keys that hold the last one)
-            for (uint32_t i = valid * kPieces + lane; i < ((valid + 15) & ~15u) * kPieces; i += 32) *piece(i) = make_uint4(0, 0, 0, 0);
-            for (uint32_t i0 = lane; !cached && i0 < valid * kPieces; i0 += 32 * 8) {
-              uint4 v[8];
+            // (what a copying warp without maps brought of the cache has no rows left to clear)
+            if (copier && fix && (mapped || !cached)) {
+              if (!(ok = wait_all(&bars.fix_full[slot], fixes >> slot))) break;
+              fixes ^= 1u << slot;
+              // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
+              // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
+              // node get at the end
+              auto piece = [&](uint32_t i) {
+                const uint32_t r = i / kPieces, c = i % kPieces;
+                return reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+              };
+              // (the sums' MMAs stop after the 16 keys that hold the last one)
+              for (uint32_t i = valid * kPieces + lane; i < ((valid + 15) & ~15u) * kPieces; i += 32) *piece(i) = make_uint4(0, 0, 0, 0);
+              for (uint32_t i0 = lane; !cached && i0 < valid * kPieces; i0 += 32 * 8) {
+                uint4 v[8];
 #pragma unroll
-              for (uint32_t k = 0; k < 8; ++k)
-                v[k] = i0 + k * 32 < valid * kPieces ? *piece(i0 + k * 32) : make_uint4(0, 0, 0, 0);
+                for (uint32_t k = 0; k < 8; ++k)
+                  v[k] = i0 + k * 32 < valid * kPieces ? *piece(i0 + k * 32) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-              for (uint32_t k = 0; k < 8; ++k) {
-                constexpr uint32_t kMask = Elem<T>::kExpMask;
-                uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-                bool found = false;
+                for (uint32_t k = 0; k < 8; ++k) {
+                  constexpr uint32_t kMask = Elem<T>::kExpMask;
+                  uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                  bool found = false;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if ((u[e] & kMask) == kMask) u[e] &= 0xFFFF0000u, found = true;
-                  if ((u[e] >> 16 & kMask) == kMask) u[e] &= 0x0000FFFFu, found = true;
-                }
-                if (found) {
-                  const uint32_t node = first + (i0 + k * 32) / kPieces;
-                  atomicOr(&broken[node >> 5], 1u << (node & 31));
-                  *piece(i0 + k * 32) = make_uint4(u[0], u[1], u[2], u[3]);
+                  for (int e = 0; e < 4; ++e) {
+                    if ((u[e] & kMask) == kMask) u[e] &= 0xFFFF0000u, found = true;
+                    if ((u[e] >> 16 & kMask) == kMask) u[e] &= 0x0000FFFFu, found = true;
+                  }
+                  if (found) {
+                    const uint32_t node = first + (i0 + k * 32) / kPieces;
+                    atomicOr(&broken[node >> 5], 1u << (node & 31));
+                    *piece(i0 + k * 32) = make_uint4(u[0], u[1], u[2], u[3]);
+                  }
                 }
               }
+              fence_proxy_async_smem();
+              arrive_warp(&bars.kv_full[slot]);
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
-          };
-          // K0 V0 K1 V1 ... for two score tiles over the same keys, K0 K1 V0 K2 V1 ... Vn-2 Vn-1 for two
-          // streams of blocks.  The queries go after the first keys, once the last segment's have been
-          // read.  Only the loading warp may wait for q_empty: a warp that the MMAs do not wait for in
-          // every segment could find it two phases on.  (One call of load: instructions are fetched from
-          // as far as L2, so the loops here are kept short.)
-          for (uint32_t x = 0; ok && x < 2 * n; ++x) {
-            const bool last = x == 2 * n - 1;
-            const bool values = two ? (x & 1) != 0 : last || (x != 0 && (x & 1) == 0);
-            const uint32_t i = two ? x / 2 : last ? n - 1 : values ? x / 2 - 1 : (x + 1) / 2;
-            load(w.b0 + i, values);
+            if (++slot == S::kSlots) slot = 0, ++pass;
             if (x != 0 || copier) continue;
-            if (seg > 0) ok = ok && wait_all(&bars.q_empty, seg - 1);
-            if (!ok) break;
+            // The queries go after the first keys, once the last segment's have been read.  Only the loading
+            // warp may wait for q_empty: a warp that the MMAs do not wait for in every segment could find it
+            // two phases on.
+            if (seg > 0 && !(ok = wait_all(&bars.q_empty, seg - 1))) break;
             uint64_t* q_full = &bars.q_full[seg & 1];
             // past here the epilogue of segment seg - 3 is over: the flags of segment seg - 4 are free
             if (lane < 8) bars.broken[(seg + 4) & 7][lane] = 0;
@@ -290,9 +302,9 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             }
             __syncwarp();
             if (lane < tiles * (DP / 64)) {
-              const uint32_t t = lane / (DP / 64), h = lane % (DP / 64);
-              tma_load_3d(smem_u32(sm + t * S::kTile + h * S::kHalf), &maps.q, q_full, h * 64, w.head * p.group,
-                          q.start + (row0 + t * half) / p.group);
+              const uint32_t t = lane / (DP / 64), c = lane % (DP / 64);
+              tma_load_3d(smem_u32(sm + t * S::kTile + c * S::kHalf), &maps.q, q_full, c * 64, w.head * p.group,
+                          q.start + p.by_group.quotient(row0 + t * half));
             }
           }
           ++seg;
@@ -305,11 +317,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             mbar_arrive(&bars.q_full[seg & 1]);
           }
         }
-        if (!ok && filler && maps.box_rows != 0) {  // copies in flight end before the CTA does
-          for (uint32_t i = issued > S::kSlots ? issued - S::kSlots : 0; i < issued; ++i) {
-            const uint32_t slot = i % S::kSlots;
-            if (sent_fix >> slot & 1u) mbar_wait(&bars.fix_full[slot], (sent_turn >> slot & 1u) ^ 1u, p.error);
-            else mbar_wait(&bars.kv_full[slot], i / S::kSlots & 1u, p.error);
+        if (!ok && filler) {  // copies in flight end before the CTA does
+          for (uint32_t i = 0; i < S::kSlots; ++i) {
+            if (i >= slot && pass == 0) break;
+            if (sent_fix >> i & 1u) mbar_wait(&bars.fix_full[i], (sent_turn >> i & 1u) ^ 1u, p.error);
+            else mbar_wait(&bars.kv_full[i], (i < slot ? pass : pass - 1) & 1u, p.error);
           }
         }
         if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
@@ -446,7 +458,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         const bool two = g->two != 0;
         const uint32_t row = row0 + (two ? s * half : 0u) + lrow;
         const bool live = lrow < half && row < rows;
-        const uint32_t node = live ? row / p.group : 0u;
+        const uint32_t node = live ? p.by_group.quotient(row) : 0u;
         const uint32_t mine = two ? n : (n + 1 - s) / 2;
         float m = -INFINITY, l = 0.0f;
         for (uint32_t i = 0; i < mine; ++i) {
