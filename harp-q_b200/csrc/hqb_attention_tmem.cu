@@ -12,9 +12,11 @@ namespace {
 
 constexpr uint32_t kKeys = 128;      // keys of a block
 constexpr uint32_t kRows = 128;      // tensor-memory lanes: rows of one score tile
-constexpr uint32_t kCopyWarp = 9;  // plain copies and the values' last rows; warp 8: tensor-map copies
+constexpr uint32_t kKeysWarp = 8;    // tensor-map copies of keys and queries
+constexpr uint32_t kCopyWarp = 9;    // plain copies, and the values' last rows
 constexpr uint32_t kMmaWarp = 10;
-constexpr uint32_t kTmemThreads = 384;  // warps 0-7 softmax, 8-10 as above, 11 idle
+constexpr uint32_t kValuesWarp = 11; // tensor-map copies of values
+constexpr uint32_t kTmemThreads = 384;  // warps 0-7 softmax
 constexpr float kSlack = 8.0f;       // log2 of how far the maximum may grow before sums are rescaled
 
 // One segment as the MMA and softmax warps see it, written by the loading warp.
@@ -26,7 +28,7 @@ struct Segment {
 };
 
 struct Bars {
-  uint64_t kv_full[8], kv_empty[8], fix_full[8];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], fix_full[4];
   uint64_t q_full[2], q_empty, s_full[2], p_full[2][2], o_full[2], o_free, joint, drain;
   uint32_t tmem, abort;
   uint32_t broken[8][8];  // by segment: drafted nodes with an infinity or NaN among their values
@@ -37,9 +39,10 @@ template <int DP>
 struct TmemShape {
   static constexpr uint32_t kHalf = kRows * 128;  // 128 rows of 64 columns
   static constexpr uint32_t kTile = kRows * DP * 2;  // a score tile's queries; a block of keys or of values
-  static constexpr uint32_t kSlots = DP == 128 ? 5 : 8;
-  static constexpr uint32_t kRing = 2 * kTile;
-  static constexpr uint32_t kBars = kRing + kSlots * kTile;
+  // blocks of keys and of values in flight (values are held for longer)
+  static constexpr uint32_t kKeySlots = DP == 128 ? 2 : 4, kValueSlots = DP == 128 ? 3 : 4;
+  static constexpr uint32_t kKeyRing = 2 * kTile, kValueRing = kKeyRing + kKeySlots * kTile;
+  static constexpr uint32_t kBars = kValueRing + kValueSlots * kTile;
   static constexpr uint32_t kStats = kBars + (sizeof(Bars) + 15) / 16 * 16;
   static constexpr uint32_t kBytes = kStats + 256 * 8;
 };
@@ -90,9 +93,11 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   }
   if (tid < 64) bars.broken[tid >> 3][tid & 7] = 0;
   if (tid == 0) {
-    for (uint32_t i = 0; i < S::kSlots; ++i) {
-      mbar_init(&bars.kv_full[i], 1);
-      mbar_init(&bars.kv_empty[i], 1);
+    for (uint32_t i = 0; i < 4; ++i) {
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
       mbar_init(&bars.fix_full[i], 1);
     }
     mbar_init(&bars.q_empty, 1);
@@ -146,200 +151,266 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
     if (warp != kMmaWarp) {
       Walk w;
       const bool work = w.begin(p, blockIdx.x, bad);
-      if (tid == 11 * 32 && !p.whole) note_split(p, w, blockIdx.x, work, bad);  // the otherwise idle warp
       if (!work) w.left = 0;
-      if (warp < kMmaWarp) {
-        // ---- both walk the slots in the order in which the MMAs take them.  One of them fills all
-        // slots (a slot's turns can only be told apart by the warp that waits for each of them): the
-        // loading warp, or without maps of the cache the copying warp.  The copying warp hands on
-        // the values whose last rows have to be cleared.  Each slot is announced once on kv_full.
-        const bool copier = warp == kCopyWarp, mapped = maps.box_rows != 0, filler = copier != mapped;
-        constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
-        const uint32_t dim = p.c.head_dim;
+      const uint32_t dim = p.c.head_dim;
+      // Keys and values have a ring of blocks each; block i of a segment takes the ring's next slot, whose
+      // turns are told apart by the one warp that fills it in every turn: the keys' warp and the values'
+      // warp, or without maps of the cache the copying warp both.  A block is announced once on k_full
+      // or v_full.
+      const bool mapped = maps.box_rows != 0;
+      struct Ring {
+        uint32_t slots, slot, turn;
+        __device__ __forceinline__ void next() {
+          if (++slot == slots) slot = 0, ++turn;
+        }
+      } keys{S::kKeySlots, 0, 0}, values{S::kValueSlots, 0, 0};
+      uint32_t seg = 0;
+      uint32_t fixed = 0, fix_turn = 0;  // a bit a slot of values: its last copy went to fix_full, that one's next phase
+      bool ok = true;
+      // one of the segment's blocks: where its keys begin, among the cached ones or the nodes, and how many
+      struct Block {
+        bool cached, fix;  // fix: has values to clear
+        uint32_t first, valid;
+      };
+      auto block = [&](uint32_t b) -> Block {
+        const bool cached = b < w.q.cached_blocks;
+        const uint32_t first = (cached ? b : b - w.q.cached_blocks) * kKeys;
+        const uint32_t valid = min(kKeys, (cached ? w.q.ctx : w.q.nodes) - first);
+        return {cached, !cached || valid < kKeys, first, valid};
+      };
+      auto drafted = [&](uint32_t dst, const CUtensorMap* map, uint64_t* bar, uint32_t first) {
+        if (lane == 0) mbar_expect_tx(bar, S::kTile);
+        __syncwarp();
+        if (lane < DP / 64) tma_load_3d(dst + lane * S::kHalf, map, bar, lane * 64, w.head, w.q.start + first);
+      };
+      if (warp != kCopyWarp) {
+        // ---- keys and queries, or values, by tensor-map copies.  (Instructions are fetched from as far as
+        // L2, so the loop is kept short and divisions out of it; one warp for both took 1900 cycles a copy,
+        // and everything waited for it.)
+        const bool is_values = warp == kValuesWarp;
+        const CUtensorMap* const cache_map = is_values ? &maps.cv : &maps.ck;
+        const CUtensorMap* const step_map = is_values ? &maps.v : &maps.k;
+        uint64_t* const empty = is_values ? bars.v_empty : bars.k_empty;
+        uint64_t* const full = is_values ? bars.v_full : bars.k_full;
+        Ring ring = is_values ? values : keys;
+        const uint32_t ring_at = smem_u32(sm) + (is_values ? S::kValueRing : S::kKeyRing);
         // a lane a box: box `box` of the block, columns 64 h ..
         const uint32_t box_shift = mapped ? 31 - __clz(maps.box_rows) : 0;
         const uint32_t h = lane >> (7 - box_shift), box = lane & ((kKeys >> box_shift) - 1);
-        uint32_t slot = 0, pass = 0, seg = 0, fixes = 0;
-        uint32_t sent_fix = 0, sent_turn = 0;  // filler, a bit a slot: its last copy goes to fix_full, that one's phase
-        bool ok = true;
+        const uint32_t lane_at = h * S::kHalf + (box << box_shift) * 128;
         while (ok && w.left != 0) {
           w.open(p);
-          const Request q = w.q;
-          const uint32_t rows = q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
+          const uint32_t rows = w.q.nodes * p.group, row0 = w.tile * p.rows, n = w.b1 - w.b0;
           const bool two = rows - row0 > half;
           const int32_t* table = p.a.tables + static_cast<uint64_t>(w.r) * p.a.table_stride;
-          uint32_t* broken = bars.broken[seg & 7];
-          // the lane's box of a block of keys: its page is looked up while the block before is loaded, and
-          // kept for the values
-          struct Place {
-            uint32_t page, inside;
-          };
-          auto locate = [&](uint32_t b) -> Place {
+          // the page of the lane's box, looked up while the block before is loaded
+          uint32_t page = 0, inside = 0;
+          auto locate = [&](uint32_t b) {
             const uint32_t key = b * kKeys + (box << box_shift), column = p.by_page.quotient(key);
-            const bool real = b < q.cached_blocks && key < q.ctx && h < DP / 64;
-            return {real ? static_cast<uint32_t>(__ldg(table + column)) : 0u, key - column * p.c.page_size};
+            const bool real = b < w.q.cached_blocks && key < w.q.ctx && h < DP / 64;
+            page = real ? static_cast<uint32_t>(__ldg(table + column)) : 0u;
+            inside = key - column * p.c.page_size;
           };
-          Place ahead{}, keys{}, before{};  // of the next block of keys, of the last one and of the one before it
-          if (!copier && mapped) ahead = locate(w.b0);
-          auto drafted = [&](uint32_t dst, uint64_t* bar, uint32_t first, bool values) {
-            if (lane == 0) mbar_expect_tx(bar, S::kTile);
-            __syncwarp();
-            if (lane < DP / 64)
-              tma_load_3d(dst + lane * S::kHalf, values ? &maps.v : &maps.k, bar, lane * 64, w.head, q.start + first);
-          };
-          // K0 V0 K1 V1 ... for two score tiles over the same keys, K0 K1 V0 K2 V1 ... Vn-2 Vn-1 for two
-          // streams of blocks.  (Instructions are fetched from as far as L2, so the loops here are kept
-          // short, and divisions out of them: with four a copy the loading warp took 1900 cycles each, and
-          // everything waited for it.)
-          for (uint32_t x = 0; x < 2 * n; ++x) {
-            const bool last = x == 2 * n - 1;
-            const bool values = two ? (x & 1) != 0 : last || (x != 0 && (x & 1) == 0);
-            const uint32_t b = w.b0 + (two ? x / 2 : last ? n - 1 : values ? x / 2 - 1 : (x + 1) / 2);
-            const bool cached = b < q.cached_blocks;
-            const uint32_t first = (cached ? b : b - q.cached_blocks) * kKeys;
-            const uint32_t valid = min(kKeys, (cached ? q.ctx : q.nodes) - first);
-            const bool fix = values && (!cached || valid < kKeys);  // rows to clear
-            uint8_t* const at = sm + S::kRing + slot * S::kTile;
-            const uint32_t dst = smem_u32(at);
-            if (filler) {
-              if (pass > 0 && !(ok = wait_all(&bars.kv_empty[slot], pass - 1))) break;
-              uint64_t* bar = fix ? &bars.fix_full[slot] : &bars.kv_full[slot];
-              if (!copier || !cached) {
-                sent_fix = fix ? sent_fix | 1u << slot : sent_fix & ~(1u << slot);
-                if (fix) sent_turn ^= 1u << slot;
-              }
-              if (!copier && !values) {
-                before = keys;
-                keys = ahead;
-                if (keys.page >= p.c.num_pages) {
-                  bad |= HQB_DEVERR_PAGES;
-                  keys.page = 0;
+          if (mapped) locate(w.b0);
+          for (uint32_t b = w.b0; b < w.b1; ++b) {
+            if (mapped) {
+              const Block x = block(b);
+              const uint32_t slot = ring.slot, dst = ring_at + slot * S::kTile;
+              if (ring.turn > 0 && !(ok = wait_all(&empty[slot], ring.turn - 1))) break;
+              uint64_t* bar = &full[slot];
+              if (is_values) {
+                fixed &= ~(1u << slot);
+                if (x.fix) {
+                  bar = &bars.fix_full[slot];
+                  fixed |= 1u << slot;
+                  fix_turn ^= 1u << slot;
                 }
-                if (b + 1 < w.b1) ahead = locate(b + 1);
               }
-              if (!cached) {
-                drafted(dst, bar, first, values);
-              } else if (!copier) {
-                const Place here = two || last || !values ? keys : before;
-                // boxes past the end of the context are left out (scores of what lies there are hidden, values
-                // are cleared)
-                const uint32_t real = (valid + maps.box_rows - 1) >> box_shift;
+              ring.next();
+              if (x.cached) {
+                if (page >= p.c.num_pages) {
+                  bad |= HQB_DEVERR_PAGES;
+                  page = 0;
+                }
+                // boxes past the end of the context are left out (scores of what lies there are hidden,
+                // values are cleared)
+                const uint32_t real = (x.valid + maps.box_rows - 1) >> box_shift;
                 if (lane == 0) mbar_expect_tx(bar, (real << box_shift) * (DP * 2));
                 __syncwarp();
-                if (h < DP / 64 && box < real)
-                  tma_load_4d(dst + h * S::kHalf + (box << box_shift) * 128, values ? &maps.cv : &maps.ck, bar, h * 64, w.head,
-                              here.inside, here.page);
+                if (h < DP / 64 && box < real) tma_load_4d(dst + lane_at, cache_map, bar, h * 64, w.head, inside, page);
               } else {
-                const T* src = static_cast<const T*>(values ? p.c.v : p.c.k);
-                for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
-                  const uint64_t where = r0 + lane < valid ? key_offset(p, table, first + r0 + lane, w.head, bad) : 0;
-#pragma unroll 4
-                  for (uint32_t y = 0; y < kPieces; ++y) {
-                    const uint32_t i = y * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
-                    const uint64_t row = __shfl_sync(0xffffffffu, where, j);
-                    const bool copy = r < valid && c * 8 < dim;
-                    cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
-                               copy ? 16u : 0u);
-                  }
-                }
-                cp_async_commit();
-                cp_async_wait<0>();
-                fence_proxy_async_smem();
-                arrive_warp(&bars.kv_full[slot]);
+                drafted(dst, step_map, bar, x.first);
               }
+              if (b + 1 < w.b1) locate(b + 1);
             }
-            // (what a copying warp without maps brought of the cache has no rows left to clear)
-            if (copier && fix && (mapped || !cached)) {
-              if (!(ok = wait_all(&bars.fix_full[slot], fixes >> slot))) break;
-              fixes ^= 1u << slot;
-              // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
-              // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
-              // node get at the end
-              auto piece = [&](uint32_t i) {
-                const uint32_t r = i / kPieces, c = i % kPieces;
-                return reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-              };
-              // (the sums' MMAs stop after the 16 keys that hold the last one)
-              for (uint32_t i = valid * kPieces + lane; i < ((valid + 15) & ~15u) * kPieces; i += 32) *piece(i) = make_uint4(0, 0, 0, 0);
-              for (uint32_t i0 = lane; !cached && i0 < valid * kPieces; i0 += 32 * 8) {
-                uint4 v[8];
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k)
-                  v[k] = i0 + k * 32 < valid * kPieces ? *piece(i0 + k * 32) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                  constexpr uint32_t kMask = Elem<T>::kExpMask;
-                  uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-                  bool found = false;
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    if ((u[e] & kMask) == kMask) u[e] &= 0xFFFF0000u, found = true;
-                    if ((u[e] >> 16 & kMask) == kMask) u[e] &= 0x0000FFFFu, found = true;
-                  }
-                  if (found) {
-                    const uint32_t node = first + (i0 + k * 32) / kPieces;
-                    atomicOr(&broken[node >> 5], 1u << (node & 31));
-                    *piece(i0 + k * 32) = make_uint4(u[0], u[1], u[2], u[3]);
-                  }
-                }
-              }
-              fence_proxy_async_smem();
-              arrive_warp(&bars.kv_full[slot]);
-            }
-            if (++slot == S::kSlots) slot = 0, ++pass;
-            if (x != 0 || copier) continue;
-            // The queries go after the first keys, once the last segment's have been read.  Only the loading
-            // warp may wait for q_empty: a warp that the MMAs do not wait for in every segment could find it
-            // two phases on.
+            if (b != w.b0 || is_values) continue;
+            // The queries go after the first keys, once the last segment's have been read.  Only the keys' warp
+            // may wait for q_empty: a warp that the MMAs do not wait for in every segment could find it two
+            // phases on.
             if (seg > 0 && !(ok = wait_all(&bars.q_empty, seg - 1))) break;
             uint64_t* q_full = &bars.q_full[seg & 1];
             // past here the epilogue of segment seg - 3 is over: the flags of segment seg - 4 are free
             if (lane < 8) bars.broken[(seg + 4) & 7][lane] = 0;
             const uint32_t tiles = two ? 2u : 1u;
             if (lane == 0) {
-              bars.segments[seg & 3] = Segment{q, w.head, row0, w.b0, n, two ? 1u : 0u, 0u};
+              bars.segments[seg & 3] = Segment{w.q, w.head, row0, w.b0, n, two ? 1u : 0u, 0u};
               mbar_expect_tx(q_full, tiles * half * DP * 2);
             }
             __syncwarp();
             if (lane < tiles * (DP / 64)) {
               const uint32_t t = lane / (DP / 64), c = lane % (DP / 64);
               tma_load_3d(smem_u32(sm + t * S::kTile + c * S::kHalf), &maps.q, q_full, c * 64, w.head * p.group,
-                          q.start + p.by_group.quotient(row0 + t * half));
+                          w.q.start + p.by_group.quotient(row0 + t * half));
             }
           }
           ++seg;
           w.advance(p, bad);
         }
-        if (ok && !copier) {  // the end: with the last queries read, so that no announcement is overtaken
+        if (ok && !is_values) {  // the end: with the last queries read, so that no announcement is overtaken
           if (seg > 0) ok = wait_all(&bars.q_empty, seg - 1);
           if (ok && lane == 0) {
             bars.segments[seg & 3].n = 0;
             mbar_arrive(&bars.q_full[seg & 1]);
           }
         }
-        if (!ok && filler) {  // copies in flight end before the CTA does
-          for (uint32_t i = 0; i < S::kSlots; ++i) {
-            if (i >= slot && pass == 0) break;
-            if (sent_fix >> i & 1u) mbar_wait(&bars.fix_full[i], (sent_turn >> i & 1u) ^ 1u, p.error);
-            else mbar_wait(&bars.kv_full[i], (i < slot ? pass : pass - 1) & 1u, p.error);
+        if (is_values) values = ring;
+        else keys = ring;
+      } else {
+        // ---- rows of values past the end and drafted nodes' infinities; without maps of the cache all blocks
+        if (lane == 0 && !p.whole) note_split(p, w, blockIdx.x, work, bad);
+        __syncwarp();
+        constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
+        uint32_t waited = 0;  // a bit a slot: the next phase of fix_full
+        while (ok && w.left != 0) {
+          w.open(p);
+          const uint32_t n = w.b1 - w.b0;
+          const int32_t* table = p.a.tables + static_cast<uint64_t>(w.r) * p.a.table_stride;
+          uint32_t* broken = bars.broken[seg & 7];
+          // a block by plain copies; drafted ones by the step's maps
+          auto fill = [&](uint32_t b, bool is_values) -> bool {
+            const Block x = block(b);
+            Ring& ring = is_values ? values : keys;
+            const uint32_t slot = ring.slot;
+            const uint32_t dst = smem_u32(sm) + (is_values ? S::kValueRing : S::kKeyRing) + slot * S::kTile;
+            if (ring.turn > 0 && !wait_all(&(is_values ? bars.v_empty : bars.k_empty)[slot], ring.turn - 1)) return false;
+            uint64_t* bar = &(is_values ? bars.v_full : bars.k_full)[slot];
+            if (is_values) fixed &= ~(1u << slot);
+            if (!x.cached) {
+              if (is_values) {
+                bar = &bars.fix_full[slot];
+                fixed |= 1u << slot;
+                fix_turn ^= 1u << slot;
+              } else {
+                keys.next();
+              }
+              drafted(dst, is_values ? &maps.v : &maps.k, bar, x.first);
+              return true;
+            }
+            const T* src = static_cast<const T*>(is_values ? p.c.v : p.c.k);
+            for (uint32_t r0 = 0; r0 < kKeys; r0 += 32) {
+              const uint64_t where = r0 + lane < x.valid ? key_offset(p, table, x.first + r0 + lane, w.head, bad) : 0;
+#pragma unroll 4
+              for (uint32_t y = 0; y < kPieces; ++y) {
+                const uint32_t i = y * 32 + lane, j = i / kPieces, c = i % kPieces, r = r0 + j;
+                const uint64_t row = __shfl_sync(0xffffffffu, where, j);
+                const bool copy = r < x.valid && c * 8 < dim;
+                cp_async16(dst + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (copy ? row + c * 8 : 0),
+                           copy ? 16u : 0u);  // (zeros past the end: nothing is left to clear)
+              }
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            arrive_warp(bar);
+            ring.next();
+            return true;
+          };
+          // a weight of zero must cancel a hidden row of values whatever it holds: rows past the end
+          // become zeros, and so do infinities and NaN of drafted nodes, which the rows that see the
+          // node get at the end
+          auto clear = [&](const Block& x) -> bool {
+            const uint32_t slot = values.slot;
+            if (!wait_all(&bars.fix_full[slot], waited >> slot)) return false;
+            waited ^= 1u << slot;
+            uint8_t* const at = sm + S::kValueRing + slot * S::kTile;
+            auto piece = [&](uint32_t i) {
+              const uint32_t r = i / kPieces, c = i % kPieces;
+              return reinterpret_cast<uint4*>(at + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            };
+            // (the sums' MMAs stop after the 16 keys that hold the last one)
+            for (uint32_t i = x.valid * kPieces + lane; i < ((x.valid + 15) & ~15u) * kPieces; i += 32)
+              *piece(i) = make_uint4(0, 0, 0, 0);
+            for (uint32_t i0 = lane; !x.cached && i0 < x.valid * kPieces; i0 += 32 * 8) {
+              uint4 v[8];
+#pragma unroll
+              for (uint32_t k = 0; k < 8; ++k)
+                v[k] = i0 + k * 32 < x.valid * kPieces ? *piece(i0 + k * 32) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (uint32_t k = 0; k < 8; ++k) {
+                constexpr uint32_t kMask = Elem<T>::kExpMask;
+                uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                bool found = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if ((u[e] & kMask) == kMask) u[e] &= 0xFFFF0000u, found = true;
+                  if ((u[e] >> 16 & kMask) == kMask) u[e] &= 0x0000FFFFu, found = true;
+                }
+                if (found) {
+                  const uint32_t node = x.first + (i0 + k * 32) / kPieces;
+                  atomicOr(&broken[node >> 5], 1u << (node & 31));
+                  *piece(i0 + k * 32) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+              }
+            }
+            fence_proxy_async_smem();
+            arrive_warp(&bars.v_full[slot]);
+            return true;
+          };
+          // (the MMAs ask for up to two blocks of keys before the values of the first)
+          for (uint32_t i = 0; i < n; ++i) {
+            if (!mapped) {
+              if (i == 0 && !(ok = fill(w.b0, false))) break;
+              if (i + 1 < n && !(ok = fill(w.b0 + i + 1, false))) break;
+              if (!(ok = fill(w.b0 + i, true))) break;
+              if (block(w.b0 + i).cached) continue;
+            }
+            const Block x = block(w.b0 + i);
+            if (x.fix && !(ok = clear(x))) break;
+            values.next();
           }
+          ++seg;
+          w.advance(p, bad);
         }
-        if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
       }
+      if (!ok) {  // copies in flight end before the CTA does
+        auto drain = [&](const Ring& r, uint64_t* full, bool is_values) {
+          for (uint32_t i = 0; i < r.slots; ++i) {
+            if (i >= r.slot && r.turn == 0) break;
+            if (is_values && (fixed >> i & 1u)) mbar_wait(&bars.fix_full[i], (fix_turn >> i & 1u) ^ 1u, p.error);
+            else mbar_wait(&full[i], (i < r.slot ? r.turn : r.turn - 1) & 1u, p.error);
+          }
+        };
+        if (warp == kKeysWarp ? mapped : warp == kCopyWarp && !mapped) drain(keys, bars.k_full, false);
+        if (warp == kValuesWarp ? mapped : warp == kCopyWarp && !mapped) drain(values, bars.v_full, true);
+      }
+      if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
     } else {
       // ---- MMA issuer: the whole warp keeps the schedule, one elected lane issues
       constexpr uint32_t kType = sizeof(T) == 2 && Elem<T>::kExpMask == 0x7F80u ? 1u : 0u;  // BF16 : FP16
       constexpr uint32_t kBase = (1u << 4) | (kType << 7) | (kType << 10) | ((kRows >> 4) << 24);
       constexpr uint32_t kScores = kBase | ((kKeys >> 3) << 17);
       constexpr uint32_t kSums = kBase | (1u << 16) | ((DP >> 3) << 17);  // B (values) MN-major
-      uint32_t slot_at = 0, seg = 0, p_at[2] = {0, 0};
+      uint32_t done = 0, seg = 0, p_at[2] = {0, 0};  // done: blocks of earlier segments
       bool ok = true;
-      auto slot_wait = [&](uint32_t n) { return wait_all(&bars.kv_full[n % S::kSlots], n / S::kSlots); };
-      auto slot_addr = [&](uint32_t n) { return smem_u32(sm + S::kRing + (n % S::kSlots) * S::kTile); };
+      auto k_wait = [&](uint32_t n) { return wait_all(&bars.k_full[n % S::kKeySlots], n / S::kKeySlots); };
+      auto v_wait = [&](uint32_t n) { return wait_all(&bars.v_full[n % S::kValueSlots], n / S::kValueSlots); };
+      auto k_done = [&](uint32_t n) { warp_commit(&bars.k_empty[n % S::kKeySlots]); };
+      auto v_done = [&](uint32_t n) { warp_commit(&bars.v_empty[n % S::kValueSlots]); };
       // descriptors step by their address field (16-byte units)
-      auto scores = [&](uint32_t s, uint32_t tile, uint32_t slot) {
+      auto scores = [&](uint32_t s, uint32_t tile, uint32_t n) {  // block n's
         const uint32_t qd = uniform(umma_sw128_low(smem_u32(sm + tile * S::kTile), 16));
-        const uint32_t kd = uniform(umma_sw128_low(slot_addr(slot), 16)), to = uniform(tmem + s * 128);
+        const uint32_t kd = uniform(umma_sw128_low(smem_u32(sm) + S::kKeyRing + n % S::kKeySlots * S::kTile, 16));
+        const uint32_t to = uniform(tmem + s * 128);
 #pragma unroll
         for (uint32_t k = 0; k < DP / 16; ++k) {
           const uint32_t step = (k >> 2) * (S::kHalf >> 4) + (k & 3) * 2;
@@ -354,8 +425,8 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
         return r;
       };
       // the sums of block i, half of its keys as soon as those weights are there
-      auto sums = [&](const Segment* g, uint32_t s, uint32_t i, uint32_t slot, bool first) -> bool {
-        const uint32_t vd = uniform(umma_sw128_low(slot_addr(slot), S::kHalf));
+      auto sums = [&](const Segment* g, uint32_t s, uint32_t i, bool first) -> bool {
+        const uint32_t vd = uniform(umma_sw128_low(smem_u32(sm) + S::kValueRing + (done + i) % S::kValueSlots * S::kTile, S::kHalf));
         const uint32_t to = uniform(tmem + 256 + s * DP), from = uniform(tmem + s * 128);
         const uint32_t b = g->b0 + i;
         const bool cached = b < g->q.cached_blocks;
@@ -373,59 +444,55 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
       for (const Segment* g; ok && (g = segment(seg)) != nullptr;) {
         const uint32_t n = g->n;
         if (g->two) {
-          // slots: K0 V0 K1 V1 ...
-          if (!(ok = slot_wait(slot_at))) break;
+          if (!(ok = k_wait(done))) break;
           tc_fence_after();
-          scores(0, 0, slot_at);
-          scores(1, 1, slot_at);
-          warp_commit(&bars.kv_empty[slot_at % S::kSlots]);
+          scores(0, 0, done);
+          scores(1, 1, done);
+          k_done(done);
           if (seg > 0 && !(ok = wait_all(&bars.o_free, seg - 1))) break;
           if (n == 1) warp_commit(&bars.q_empty);
-          // (the slots of the next turn are waited for before its weights, so that nothing stands between
+          // (the blocks of the next turn are waited for before its weights, so that nothing stands between
           // weights that are ready and their MMAs)
-          if (!(ok = slot_wait(slot_at + 1) && (n == 1 || slot_wait(slot_at + 2)))) break;
+          if (!(ok = v_wait(done) && (n == 1 || k_wait(done + 1)))) break;
           for (uint32_t i = 0; i < n; ++i) {
-            const uint32_t v = slot_at + 2 * i + 1, k = v + 1;
+            const uint32_t v = done + i, k = v + 1;
             const bool more = i + 1 < n;
-            if (!(ok = sums(g, 0, i, v, i == 0))) break;
+            if (!(ok = sums(g, 0, i, i == 0))) break;
             if (more) scores(0, 0, k);
             else warp_commit(&bars.o_full[0]);
-            if (!(ok = sums(g, 1, i, v, i == 0))) break;
-            warp_commit(&bars.kv_empty[v % S::kSlots]);
+            if (!(ok = sums(g, 1, i, i == 0))) break;
+            v_done(v);
             if (!more) {
               warp_commit(&bars.o_full[1]);
               break;
             }
             scores(1, 1, k);
-            warp_commit(&bars.kv_empty[k % S::kSlots]);
+            k_done(k);
             if (i + 2 == n) warp_commit(&bars.q_empty);
-            if (!(ok = slot_wait(v + 2) && (i + 2 == n || slot_wait(k + 2)))) break;
+            if (!(ok = v_wait(v + 1) && (i + 2 == n || k_wait(k + 1)))) break;
           }
         } else {
-          // slots: K0 K1 V0 K2 V1 K3 ...
-          if (!(ok = slot_wait(slot_at))) break;
+          // even blocks are stream 0's, odd ones stream 1's
+          if (!(ok = k_wait(done))) break;
           tc_fence_after();
-          scores(0, 0, slot_at);
-          warp_commit(&bars.kv_empty[slot_at % S::kSlots]);
-          uint32_t next = slot_at + 1;
+          scores(0, 0, done);
+          k_done(done);
           if (n > 1) {
-            if (!(ok = slot_wait(next))) break;
+            if (!(ok = k_wait(done + 1))) break;
             tc_fence_after();
-            scores(1, 0, next);
-            warp_commit(&bars.kv_empty[next % S::kSlots]);
-            ++next;
+            scores(1, 0, done + 1);
+            k_done(done + 1);
           }
           if (seg > 0 && !(ok = wait_all(&bars.o_free, seg - 1))) break;
           if (n <= 2) warp_commit(&bars.q_empty);
           for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t s = j & 1, v = next++;
+            const uint32_t s = j & 1, v = done + j, k = v + 2;
             const bool more = j + 2 < n;
-            if (!(ok = slot_wait(v) && (!more || slot_wait(next)) && sums(g, s, j, v, j < 2))) break;
-            warp_commit(&bars.kv_empty[v % S::kSlots]);
+            if (!(ok = v_wait(v) && (!more || k_wait(k)) && sums(g, s, j, j < 2))) break;
+            v_done(v);
             if (more) {
-              scores(s, 0, next);
-              warp_commit(&bars.kv_empty[next % S::kSlots]);
-              ++next;
+              scores(s, 0, k);
+              k_done(k);
               if (j + 3 == n) warp_commit(&bars.q_empty);
             }
           }
@@ -434,7 +501,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
             warp_commit(&bars.o_full[1]);
           }
         }
-        slot_at += 2 * n;
+        done += n;
         ++seg;
       }
       if (!ok) {  // MMAs that were issued end before the tensor memory is freed
