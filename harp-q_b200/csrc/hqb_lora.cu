@@ -17,7 +17,11 @@ namespace {
 
 constexpr uint32_t kCluster = 8;         // CTAs that share a tile: the portable cluster size
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kDirectTokens = kThreads;  // up to here every cluster finds its own tile
+// Up to kVoteTokens tokens, or kCountTokens of fewer than kCountGroups adapters, every cluster finds its own
+// tile; above, and where the shrink and expand kernels run, lora_plan_kernel finds them all.  B200, us, own /
+// planned, FP16, rank 16, 4096 x 4096: 300 tokens of 8 adapters 8.8 / 10.8; 600 of 64 17.3 / 17.8, of 128
+// 25.2 / 24.5; 1000 of 64 18.4 / 18.9, of 900 121 / 96.
+constexpr uint32_t kVoteTokens = kThreads, kCountTokens = 4 * kThreads, kCountGroups = 96;
 // A planned call keeps to lora_kernel up to this many tokens * padded rank.  B200, us, lora_kernel /
 // shrink + expand, FP16 or BF16, 8 adapters: rank 16, 4096 x 4096: 1024 tokens 18.4 / 24.0, 2048 tokens
 // 28.7 / 27.5; rank 24, 1024 x 8192: 777 tokens 18.0 / 27.2; rank 64, 11008 x 4096: 300 tokens 16.8 /
@@ -355,9 +359,10 @@ struct Expand {
 
 // The tile of a planned call, or the tile that a cluster finds by itself: an adapter (`adapters`:
 // none), its tokens in s_token (-1 past them) and their count; false: nothing to do.
+// s_info: 64 words and the votes; s_count: a word a group, up to kCountGroups (neither in planned calls).
 template <int M>
-__device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, int32_t* s_token, uint32_t* s_info, uint32_t& group,
-                                          uint32_t& count, uint32_t& bad) {
+__device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, int32_t* s_token, uint32_t* s_info, uint32_t* s_count,
+                                          uint32_t& group, uint32_t& count, uint32_t& bad) {
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (p.planned) {
     if (tile >= *p.tile_count) return false;
@@ -365,6 +370,75 @@ __device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, in
     group = t.group;
     count = t.count;
     for (uint32_t i = tid; i < M; i += kThreads) s_token[i] = i < count ? static_cast<int32_t>(p.order[t.first + i]) : -1;
+  } else if (p.tokens > kVoteTokens) {
+    // tokens counted by group; the groups' tiles lie in the groups' order, their tokens in the tokens' order
+    constexpr uint32_t kEach = kCountTokens / kThreads;
+    uint32_t* s_votes = s_info + 64;  // members by 32 tokens
+    const uint32_t groups = p.s.adapters + 1;
+    if (tid < kCountGroups) s_count[tid] = 0;
+    for (uint32_t i = tid; i < M; i += kThreads) s_token[i] = -1;
+    uint32_t own[kEach];
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t t = k * kThreads + tid;
+      own[k] = t < p.tokens ? group_of(p, t, bad) : groups;
+    }
+    if (bad != 0 && tile == 0) atomicOr(p.error, static_cast<int>(bad));
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t lead = __shfl_sync(0xffffffffu, own[k], 0), same = ballot(own[k] == lead);
+      if (same == 0xffffffffu) {  // a run of one adapter: 32 additions to one word would queue
+        if (lane == 0 && lead < groups) atomicAdd(&s_count[lead], 32u);
+      } else if (own[k] < groups) {
+        atomicAdd(&s_count[own[k]], 1u);
+      }
+    }
+    __syncthreads();
+    const uint32_t tiles = tid >= groups || (tid == p.s.adapters && p.in_place) ? 0u : (s_count[tid] + M - 1) / M;
+    uint32_t inc = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= static_cast<uint32_t>(o)) inc += up;
+    }
+    if (lane == 31) s_info[warp] = inc;
+    __syncthreads();
+    uint32_t at = inc - tiles, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) at += s_info[w];
+      all += s_info[w];
+    }
+    if (tile >= all) return false;
+    if (tile >= at && tile - at < tiles) {
+      s_info[32] = tid;
+      s_info[33] = (tile - at) * M;
+    }
+    __syncthreads();
+    group = s_info[32];
+    const uint32_t first = s_info[33];
+    count = min(static_cast<uint32_t>(M), s_count[group] - first);
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t votes = ballot(own[k] == group);
+      if (lane == 0) s_votes[k * (kThreads / 32) + warp] = __popc(votes);
+    }
+    __syncthreads();
+    const uint32_t mine = s_votes[lane];
+    uint32_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= static_cast<uint32_t>(o)) before += up;
+    }
+    before -= mine;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t votes = ballot(own[k] == group);
+      const uint32_t place = __shfl_sync(0xffffffffu, before, k * (kThreads / 32) + warp) + __popc(votes & ((1u << lane) - 1u));
+      if (own[k] == group && place >= first && place - first < M) s_token[place - first] = static_cast<int32_t>(k * kThreads + tid);
+    }
   } else {
     // a token with a multiple of M tokens of its adapter before it begins a tile of that token and the
     // adapter's next M - 1; cluster i takes the i-th tile, in the order of their first tokens
@@ -443,6 +517,8 @@ struct LoraSmem {
   static constexpr uint32_t kOne = (227 * 1024 - kRing) / (8 * Expand<T, Y, RP, 16>::kStage);
   static constexpr uint32_t kMost = kTwo > 6 ? 6 : kTwo >= 2 ? kTwo : kOne >= 2 ? 2 : 1;
   static_assert(kOne >= 1, "a stage fits");
+  static_assert(kRing - kPart >= kCountGroups * 4 && kCountGroups <= kThreads, "the counts of groups lie over the partial sums");
+  static_assert(kCountTokens == 32 * 32, "a lane for every 32 tokens");
   // no more than a warp has steps: what is not needed lets more CTAs share an SM
   static uint32_t stages(uint64_t rows) {
     const uint64_t steps = (rows + 32 * 8 * kCluster - 1) / (32 * 8 * kCluster);
@@ -479,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
   uint32_t bad = 0, group, count;
   griddep_launch_dependents();
   griddep_wait();
-  if (!find_tile<M>(p, tile, s_token, s_info, group, count, bad)) return;
+  if (!find_tile<M>(p, tile, s_token, s_info, reinterpret_cast<uint32_t*>(s_part), group, count, bad)) return;
   float scale;
   const uint32_t rank = adapter(p, group, scale, bad);
   if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
@@ -626,7 +702,7 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_cons
   uint32_t bad = 0, group, count;
   griddep_launch_dependents();
   griddep_wait();
-  if (!find_tile<M>(p, tile, s_token, nullptr, group, count, bad)) return;
+  if (!find_tile<M>(p, tile, s_token, nullptr, nullptr, group, count, bad)) return;
   float scale;
   const uint32_t rank = adapter(p, group, scale, bad);
   if (rank == 0) return;
@@ -729,7 +805,7 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_cons
     u += end - first;
     __syncthreads();  // the last tile's terms and tokens have been read
     uint32_t group, count;
-    find_tile<M>(p, tile, s_token, nullptr, group, count, bad);
+    find_tile<M>(p, tile, s_token, nullptr, nullptr, group, count, bad);
     float scale;
     const uint32_t rank = adapter(p, group, scale, bad);
     Expand<T, Y, RP, M> x2;
@@ -915,7 +991,7 @@ extern "C" {
 HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* s, uint32_t tokens, int device) {
   (void)device;
   if (!set_ok(s) || tokens > 0x7FFFFFFFu) return 0;
-  if (tokens <= kDirectTokens) return 256;
+  if (tokens <= kVoteTokens) return 256;
   // the call's kernels depend on its alignment and output type too: room for any
   uint64_t most = layout(s, tokens, 16).total;
   for (const bool wide_y : {false, true}) {
@@ -957,9 +1033,9 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
   p.base_stride = base_stride;
   p.y_stride = y_stride;
   p.tokens = tokens;
-  p.planned = tokens > kDirectTokens ? 1u : 0u;
   p.in_place = base == y ? 1u : 0u;
-  p.tile_rows = p.planned ? planned_rows(s, tokens, vec, y_dtype == HQB_F32) : 16u;
+  p.tile_rows = tokens > kVoteTokens ? planned_rows(s, tokens, vec, y_dtype == HQB_F32) : 16u;
+  p.planned = tokens > kVoteTokens && (p.tile_rows != 16 || tokens > kCountTokens || s->adapters >= kCountGroups) ? 1u : 0u;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.error = reinterpret_cast<int*>(ws);
   cudaStream_t st = as_stream(stream);

@@ -615,6 +615,16 @@ def test_lora_unaligned(kind, y_kind, tokens, cols, rows, adapters, rank):
     check_lora(*make_lora(rank, tokens, cols, rows, adapters, rank, kind, y_kind), y_kind)
 
 
+@pytest.mark.parametrize("run", [1, 37, 2000])
+@pytest.mark.parametrize("tokens,adapters", [(255, 40), (1023, 3), (1024, 1), (1024, 95), (1000, 96), (1025, 5), (513, 700)])
+def test_lora_groups_tokens(tokens, adapters, run):
+    """Runs of one adapter and mixed ids, on both sides of the sizes at which tokens are grouped in another way."""
+    x, a, b, ranks, scales, _, base = make_lora(tokens, tokens, 64, 40, adapters, 16, BF16, BF16)
+    g = torch.Generator("cuda").manual_seed(run)
+    ids = torch.randint(-1, adapters, (-(-tokens // run),), generator=g, device="cuda").to(torch.int32)
+    check_lora(x, a, b, ranks, scales, ids.repeat_interleave(run)[:tokens].contiguous(), base, BF16)
+
+
 @pytest.mark.parametrize("tokens", [7, 500])
 def test_lora_defaults_and_no_base(tokens):
     x, a, b, _, _, ids, _ = make_lora(1, tokens, 256, 128, 3, 16, F16, F16, full=True)
