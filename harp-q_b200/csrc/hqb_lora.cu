@@ -169,24 +169,26 @@ struct Expand {
   static constexpr bool kHold = kN == 1 && RP > 16 && M / 16 * S::kGroups <= 8;
 
   const T* b;                  // the lane's first B row of step 0
-  const Y* base[kRowsEach];    // the lane's rows at its first output of step 0; null: no row, no base
+  const Y* base[kRowsEach];    // the lane's rows (i * 8 + g) at its first output of step 0; past the tile's its first
   Y* y[kRowsEach];
   uint64_t rows;
   uint32_t pitch, rank, count, ring, stages, lane;
+  bool based;
 
   __device__ __forceinline__ void prepare(const LoraParams& p, uint32_t group, uint32_t rank_, uint32_t count_,
                                           const int32_t* s_token, uint32_t ring_, uint32_t stages_) {
     lane = threadIdx.x & 31;
     const uint32_t g = lane >> 2, q = lane & 3;
     rows = p.s.rows, pitch = p.s.max_rank, rank = rank_, count = count_, ring = ring_, stages = stages_;
+    based = p.base != nullptr;
     b = static_cast<const T*>(p.s.b) + (static_cast<uint64_t>(min(group, p.s.adapters - 1)) * rows + 8 * (g >> 1) + (g & 1)) * pitch +
         q * (RP == 16 ? 4 : 8);
 #pragma unroll
     for (int i = 0; i < kRowsEach; ++i) {
       const int32_t t = s_token[(i >> 1) * 16 + g + 8 * (i & 1)];
-      const uint64_t row = static_cast<uint64_t>(max(t, 0));
-      base[i] = t < 0 || p.base == nullptr ? nullptr : static_cast<const Y*>(p.base) + row * p.base_stride + q * 8;
-      y[i] = t < 0 ? nullptr : static_cast<Y*>(p.y) + row * p.y_stride + q * 8;
+      const uint64_t row = static_cast<uint64_t>(t < 0 ? s_token[0] : t);
+      base[i] = static_cast<const Y*>(p.base) + row * p.base_stride + q * 8;
+      y[i] = static_cast<Y*>(p.y) + row * p.y_stride + q * 8;
     }
   }
   // copies of step st into stage at `to` (shared address)
@@ -196,28 +198,42 @@ struct Expand {
     const uint32_t left = rows - n0 < 32 ? static_cast<uint32_t>(rows - n0) : 32u;  // outputs of the step
     if (rank != 0) {
       const T* row = b + n0 * pitch;
+      if (left == 32 && rank == RP) {  // all of it: no sizes to choose
 #pragma unroll
-      for (int j = 0; j < 4; ++j, row += 2 * pitch) {
-        const bool inside = 8 * (g >> 1) + 2 * j + (g & 1) < left;
-        if constexpr (RP == 16) {
-          const bool real = inside && q * 4 < rank;
-          cp_async8(to + (j * 32 + lane) * 8, real ? row : b, real ? 8u : 0u);
-        } else {
+        for (int j = 0; j < 4; ++j, row += 2 * pitch) {
+          if constexpr (RP == 16) {
+            cp_async8(to + (j * 32 + lane) * 8, row, 8u);
+          } else {
 #pragma unroll
-          for (int k = 0; k < S::kGroups; ++k) {
-            const bool real = inside && k * 32 + q * 8 < rank;
-            cp_async16(to + ((j * S::kGroups + k) * 32 + lane) * 16, real ? row + k * 32 : b, real ? 16u : 0u);
+            for (int k = 0; k < S::kGroups; ++k) cp_async16(to + ((j * S::kGroups + k) * 32 + lane) * 16, row + k * 32, 16u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j, row += 2 * pitch) {
+          const bool inside = 8 * (g >> 1) + 2 * j + (g & 1) < left;
+          if constexpr (RP == 16) {
+            const bool real = inside && q * 4 < rank;
+            cp_async8(to + (j * 32 + lane) * 8, real ? row : b, real ? 8u : 0u);
+          } else {
+#pragma unroll
+            for (int k = 0; k < S::kGroups; ++k) {
+              const bool real = inside && k * 32 + q * 8 < rank;
+              cp_async16(to + ((j * S::kGroups + k) * 32 + lane) * 16, real ? row + k * 32 : b, real ? 16u : 0u);
+            }
           }
         }
       }
     }
+    if (based && q * 8 < left) {
 #pragma unroll
-    for (int i = 0; i < kRowsEach; ++i)
-      if (base[i] != nullptr && q * 8 < left) {
+      for (int i = 0; i < kRowsEach; ++i) {
+        if (M == 16 && i * 8 + g >= count) break;  // few rows: none is copied in vain
 #pragma unroll
         for (int v = 0; v < kBaseVecs; ++v)
           cp_async16(to + 32 * kBBytes + ((i * kBaseVecs + v) * 32 + lane) * 16, base[i] + n0 + v * 4, 16u);
       }
+    }
   }
   // the first stages - 1 steps of a warp that takes steps first, first + 8, ... below end
   __device__ __forceinline__ void start(uint32_t first, uint32_t end) const {
@@ -314,11 +330,11 @@ struct Expand {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int i = mt * 2 + e;
-          if (y[i] == nullptr || !inside) continue;
+          if (mt * 16 + 8 * e + g >= count || !inside) continue;
           float out[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) out[x] = 0.0f;
-          if (base[i] != nullptr) {
+          if (based) {
             const uint32_t from = at + 32 * kBBytes + i * kBaseVecs * 512 + lane * 16;
             const uint4 v = lds128a(from);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -712,18 +728,30 @@ __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_cons
   const uint32_t chunks = static_cast<uint32_t>((cols + kShrinkCols - 1) / kShrinkCols);
   const uint32_t c0 = static_cast<uint64_t>(chunks) * split / p.splits, c1 = static_cast<uint64_t>(chunks) * (split + 1) / p.splits;
   const uint32_t ring = smem_u32(sm) + 512;
-  auto load = [&](uint32_t chunk, uint32_t stage) {
-    const uint32_t to = ring + stage * kStage;
+  // a thread copies the same piece of every 16th row of x, then of A, of every chunk
+  constexpr uint32_t kCopies = (M + RP) * kPieces / kThreads, kCopyRows = kThreads / kPieces;
+  const uint32_t piece = tid % kPieces, row = tid / kPieces;
+  const T* src[kCopies];
+  uint32_t real = 0;  // a bit a copy
 #pragma unroll
-    for (uint32_t i = tid; i < (M + RP) * kPieces; i += kThreads) {
-      const uint32_t r = i / kPieces, c = i % kPieces;
-      const uint64_t col = static_cast<uint64_t>(chunk) * kShrinkCols + c * 8;
-      const int32_t t = r < M ? s_token[r] : static_cast<int32_t>(r - M);
-      const bool real = col < cols && (r < M ? t >= 0 : t < static_cast<int32_t>(rank));
-      const T* src = r < M ? x + (real ? t * p.x_stride + col : 0) : a + (real ? t * cols + col : 0);
-      cp_async16(to + r * (kShrinkCols * 2) + ((c ^ ((r & 1) << 2)) << 4), src, real ? 16u : 0u);
-    }
+  for (uint32_t i = 0; i < kCopies; ++i) {
+    const uint32_t r = i * kCopyRows + row;
+    const int32_t t = r < M ? s_token[r] : r - M < rank ? static_cast<int32_t>(r - M) : -1;
+    const uint64_t at = static_cast<uint64_t>(max(t, 0));
+    src[i] = (r < M ? x + at * p.x_stride : a + at * cols) + piece * 8;
+    real |= t >= 0 ? 1u << i : 0u;
+  }
+  const uint32_t dst = ring + row * (kShrinkCols * 2) + ((piece ^ ((row & 1) << 2)) << 4);
+  auto load = [&](uint32_t chunk, uint32_t stage) {
+    const uint32_t to = dst + stage * kStage;
+    const uint64_t col = static_cast<uint64_t>(chunk) * kShrinkCols;
+    const uint32_t copies = col + piece * 8 < cols ? real : 0u;
+    const uint64_t off = copies != 0 ? col : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kCopies; ++i)
+      cp_async16(to + i * kCopyRows * (kShrinkCols * 2), src[i] + off, copies >> i & 1u ? 16u : 0u);
   };
+  static_assert((M + RP) * kPieces % kThreads == 0 && kCopyRows % 2 == 0 && kCopies <= 32, "whole copies");
   const uint32_t wm = warp % kWM, wn = warp / kWM;
   float acc[kNT][4];
 #pragma unroll
