@@ -365,11 +365,11 @@ constexpr uint32_t kJoinThreads = 512;
 
 // One CTA per (CTA of the attention, 32 rows): the partial results of the item that begins there
 // and spans later CTAs, in their order, joined by their maxima.  A thread has 4 columns of a row
-// and reads up to 8 partial results at once, a warp 32 neighbouring rows; the outputs are turned in
+// and reads up to 4 partial results at once, a warp 32 neighbouring rows; the outputs are turned in
 // shared memory so that they leave in whole rows (2-byte stores of 32 rows at once took four
 // times as long as all the rest).
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads, 2) attention_join_kernel(const __grid_constant__ AttnParams p) {
   __shared__ __align__(16) T turned[kJoinRows][HQB_MAX_HEAD_DIM + 8];
   const uint32_t first = blockIdx.x;
   griddep_launch_dependents();
@@ -388,11 +388,11 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     for (uint32_t d = threadIdx.x / kJoinRows * 4; d < dim; d += kJoinThreads / kJoinRows * 4) {
       float m = -INFINITY, l = 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (uint32_t c0 = first; c0 <= q.last; c0 += 8) {
-        float2 s[8];
-        float4 v[8];
+      for (uint32_t c0 = first; c0 <= q.last; c0 += 4) {
+        float2 s[4];
+        float4 v[4];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
+        for (uint32_t k = 0; k < 4; ++k) {
           s[k] = make_float2(-INFINITY, 0.0f);
           v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           if (c0 + k <= q.last) {
@@ -403,13 +403,13 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         }
         float top = m;
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
+        for (uint32_t k = 0; k < 4; ++k) top = fmaxf(top, s[k].x);
         const float use = top == -INFINITY ? 0.0f : top, old = fast_exp2(m - use);
         l *= old;
         o.x *= old, o.y *= old, o.z *= old, o.w *= old;
         m = top;
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
+        for (uint32_t k = 0; k < 4; ++k) {
           if (c0 + k > q.last) break;
           const float f = fast_exp2(s[k].x - use);
           l += f * s[k].y;
