@@ -40,7 +40,6 @@ struct AttnParams {
   uint32_t rows;        // rows of a row tile
   uint32_t block_shift; // log2 of the keys of a block
   Divisor by_page, by_group, by_rows;
-  uint32_t max_tiles;   // row tiles of max_new nodes
   uint32_t dim_pad;     // padded head dimension (columns of a partial row)
   uint32_t min_blocks;  // fewest blocks worth a CTA of its own
   uint32_t whole;       // 1: items are not cut (a unit is an item, no partials)

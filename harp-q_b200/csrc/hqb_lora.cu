@@ -25,7 +25,7 @@ constexpr uint32_t kVoteTokens = kThreads, kCountTokens = 4 * kThreads, kCountGr
 // A planned call keeps to lora_kernel up to this many tokens * padded rank.  B200, us, lora_kernel /
 // shrink + expand, FP16 or BF16, 8 adapters: rank 16, 4096 x 4096: 1024 tokens 18.4 / 24.0, 2048 tokens
 // 28.7 / 27.5; rank 24, 1024 x 8192: 777 tokens 18.0 / 27.2; rank 64, 11008 x 4096: 300 tokens 16.8 /
-// 24.1, 777 tokens 41.5 / 32.8.
+// 24.1, 777 tokens 41.5 / 32.8 (before either form's later steps, which gave both about a tenth).
 constexpr uint64_t kClusterWork = 32768;
 constexpr uint32_t kMaxAdapters = 16383;
 
@@ -552,7 +552,10 @@ struct LoraSmem {
 // of B and of the output; their first rows of B and of base are under way from the start.  One
 // launch, no scratch, no atomics.
 // Bound by latency (two trips to memory and two cluster barriers) up to a few adapters, then by the
-// adapters' bytes.
+// adapters' bytes and the waves of clusters.  Measured, B200: one token of rank 16, 4096 x 4096, FP16, 5.5 us;
+// 48 tokens of 16 adapters of rank 32, 12288 x 4096, FP32 result, 12.0 us (1.8 TB/s); 777 tokens of 6 of rank 24,
+// 1024 x 8192, BF16, 15.6 us.  (Three CTAs an SM at ranks up to 32, in 80 registers: 14.4 us the last one,
+// but 13.7 for 12.0 us the one before.)
 template <typename T, typename Y, int RP, bool VEC>
 __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ LoraParams p) {
   using S = LoraShape<RP>;
@@ -705,7 +708,9 @@ constexpr uint32_t kShrinkSmem = 512 + kShrinkStages * (M + RP) * kShrinkCols * 
 // Split: 16 rows by RP / (8 / row tiles) ranks a warp; x and A come in chunks of 64 columns by
 // asynchronous copies, four chunks deep.  A lane reads 16 bytes of a row at a time (both k-halves of
 // two MMAs); piece c of row r lies at c ^ 4(r & 1), which those reads meet without conflicts.
-// Bound by the bytes of x (A comes from L2).
+// Bound by instructions (issue slots 74 % busy before the copies' addresses left the loop, 30.8 us; since
+// then 25.6 us) at 8192 tokens of rank 64 and 4096 columns, BF16; x alone would take 10.2 us from HBM.
+// Tiles of 128 rows, and four warps along the columns of a chunk, were slower.
 template <typename T, int RP, int M>
 __global__ void __launch_bounds__(kThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
   constexpr uint32_t kWM = M / 16, kWN = 8 / kWM;                 // warps along rows, along ranks
@@ -809,7 +814,9 @@ struct ExpandSmem {
 // are dealt to the CTAs (one an SM) in equal contiguous ranges.  At each tile's start the warps sum
 // the tile's t over the column ranges in their order and split it into terms, while the ring's
 // first copies of B and base are under way.
-// Bound by the bytes of base and y.
+// Two warps a scheduler wait for their own instructions more than for HBM: 11008 outputs of 8192 tokens,
+// rank 64, BF16, take 80 us (4.5 TB/s of base and y), of which the bytes need 55.  Rings of more
+// stages, 16 warps and tiles of 128 rows were slower.
 template <typename T, typename Y, int RP>
 __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   using S = LoraShape<RP>;
@@ -869,7 +876,8 @@ __global__ void __launch_bounds__(kThreads) lora_expand_kernel(const __grid_cons
 }
 
 // Groups the tokens by adapter: counts, offsets, then each token to its group's next place.  The
-// order within a group may change between runs; a token's output does not depend on it.
+// order within a group may change between runs; a token's output does not depend on it.  One CTA: bound by
+// latency (two passes over the ids); 8192 tokens 8 us, of which the kernels after it wait for all.
 __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__ LoraParams p) {
   extern __shared__ uint32_t count[];  // [groups], then the groups' next places
   __shared__ uint32_t red[2][32];

@@ -42,7 +42,8 @@ __device__ __forceinline__ uint64_t block_exclusive_sum(uint64_t v, uint64_t* ca
 // round), so the whole plan is one launch without any hand-over between CTAs.  A token finds
 // its request by a binary search of the chunk's starts.  CTA 0 also writes the per-request
 // outputs.  New page columns are written by the first token in them.
-// What bounds it: latency (launch, three dependent loads, scan, search), not bytes.
+// What bounds it: latency (launch, three dependent loads, scan, search, a load per ancestor), not bytes.
+// Measured, B200: 64 requests of one token 3.1 us; 512 trees of up to 64 nodes 7.3 us, in a CUDA graph.
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_constant__ hqb_page_plan_args a,
                                                                  uint32_t per_cta) {
   __shared__ uint64_t red[kPlanThreads / 32];
@@ -229,7 +230,8 @@ struct AppendElem<__nv_bfloat16, __half> {
 // W consecutive elements a thread: 8 (16 bytes written, 16 or 32 read) where sizes, strides and
 // addresses are multiples of that, else 1.  A thread moves the same piece of k and of v, so two
 // independent copies are in flight per thread.  Bound by the copy itself (HBM, or L2 at the few
-// rows of a decode step, where the launch dominates).
+// rows of a decode step, where the launch dominates).  Measured, B200: 8192 picked rows of 8 heads of 128,
+// BF16, 12.5 us over buffers larger than L2 (5.4 TB/s; a plain copy reaches 6.55); 16 rows of 32 heads 1.6 us.
 template <typename S, typename T, int W>
 __global__ void __launch_bounds__(256) cache_append_kernel(const __grid_constant__ AppendParams p) {
   const uint32_t pieces = p.dim / W, row_pieces = pieces * p.heads;
