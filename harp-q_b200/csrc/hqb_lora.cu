@@ -22,10 +22,10 @@ constexpr uint32_t kThreads = 256;
 // planned, FP16, rank 16, 4096 x 4096: 300 tokens of 8 adapters 8.8 / 10.8; 600 of 64 17.3 / 17.8, of 128
 // 25.2 / 24.5; 1000 of 64 18.4 / 18.9, of 900 121 / 96.
 constexpr uint32_t kVoteTokens = kThreads, kCountTokens = 4 * kThreads, kCountGroups = 96;
-// A planned call keeps to lora_kernel up to this many tokens * padded rank.  B200, us, lora_kernel /
-// shrink + expand, FP16 or BF16, 8 adapters: rank 16, 4096 x 4096: 1024 tokens 18.4 / 24.0, 2048 tokens
-// 28.7 / 27.5; rank 24, 1024 x 8192: 777 tokens 18.0 / 27.2; rank 64, 11008 x 4096: 300 tokens 16.8 /
-// 24.1, 777 tokens 41.5 / 32.8 (before either form's later steps, which gave both about a tenth).
+// A call of more than kVoteTokens tokens keeps to lora_kernel up to this many tokens * padded rank.  B200, us,
+// lora_kernel / shrink + expand, 8 adapters: rank 16, 4096 x 4096, FP16: 1024 tokens 17.4 / 25.6, 2048 tokens
+// 26.2 / 23.6; rank 24, 1024 x 8192, BF16: 777 tokens 15.3 / 23.2; rank 64, 11008 x 4096, FP16: 300 tokens
+// 21.6 / 30.8, 777 tokens 42.8 / 36.8; rank 64, 4096 x 4096, BF16: 500 tokens 21.9 / 23.7.
 constexpr uint64_t kClusterWork = 32768;
 constexpr uint32_t kMaxAdapters = 16383;
 
