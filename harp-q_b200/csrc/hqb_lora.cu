@@ -3,6 +3,7 @@
 //                       launch: decode steps, and rows that no 16-byte access fits
 // Calls of many tokens, three launches:
 //   lora_plan_kernel    groups the tokens by adapter into tiles
+//   lora_lay_kernel     rows of B in multiples of 8 ranks (only where max_rank is not one)
 //   lora_shrink_kernel  t = A x
 //   lora_expand_kernel  y = base + scale * B t
 #include <cuda_runtime.h>
@@ -28,6 +29,7 @@ constexpr uint32_t kVoteTokens = kThreads, kCountTokens = 4 * kThreads, kCountGr
 // 21.6 / 30.8, 777 tokens 42.8 / 36.8; rank 64, 4096 x 4096, BF16: 500 tokens 21.9 / 23.7.
 constexpr uint64_t kClusterWork = 32768;
 constexpr uint32_t kMaxAdapters = 16383;
+constexpr uint32_t kLayTokens = 8;  // tokens an adapter from which its rows of B are laid out
 
 struct LoraTile {
   uint32_t group;  // adapter, or `adapters` for tokens without one
@@ -54,6 +56,8 @@ struct LoraParams {
   uint32_t max_tiles;
   uint32_t splits;    // column ranges of the first product
   uint32_t stages;    // of lora_kernel's rings
+  uint32_t pitch;     // elements of a row of b
+  void* laid;         // b in rows of `pitch`, where the call lays it out
   float* inner;       // [splits][max_tiles][tile_rows][padded rank]
 };
 
@@ -179,9 +183,9 @@ struct Expand {
                                           const int32_t* s_token, uint32_t ring_, uint32_t stages_) {
     lane = threadIdx.x & 31;
     const uint32_t g = lane >> 2, q = lane & 3;
-    rows = p.s.rows, pitch = p.s.max_rank, rank = rank_, count = count_, ring = ring_, stages = stages_;
+    rows = p.s.rows, pitch = p.pitch, rank = rank_, count = count_, ring = ring_, stages = stages_;
     based = p.base != nullptr;
-    b = static_cast<const T*>(p.s.b) + (static_cast<uint64_t>(min(group, p.s.adapters - 1)) * rows + 8 * (g >> 1) + (g & 1)) * pitch +
+    b = static_cast<const T*>(p.laid != nullptr ? p.laid : p.s.b) + (static_cast<uint64_t>(min(group, p.s.adapters - 1)) * rows + 8 * (g >> 1) + (g & 1)) * pitch +
         q * (RP == 16 ? 4 : 8);
 #pragma unroll
     for (int i = 0; i < kRowsEach; ++i) {
@@ -926,6 +930,24 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
   if (bad != 0) atomicOr(p.error, static_cast<int>(bad));
 }
 
+// B in rows of a multiple of 8 ranks, zeros after the last: 16-byte copies need such rows, and without them
+// the second product goes element by element.  Bound by the bytes of B, read and written once.
+__global__ void __launch_bounds__(256) lora_lay_kernel(const __grid_constant__ LoraParams p) {
+  const uint32_t pieces = p.pitch / 8;
+  const uint64_t total = static_cast<uint64_t>(p.s.adapters) * p.s.rows * pieces;
+  griddep_launch_dependents();
+  griddep_wait();
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+    const uint64_t row = i / pieces;
+    const uint32_t r = static_cast<uint32_t>(i - row * pieces) * 8;
+    const uint16_t* src = static_cast<const uint16_t*>(p.s.b) + row * p.s.max_rank;
+    uint16_t v[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) v[k] = r + k < p.s.max_rank ? __ldg(src + r + k) : 0;
+    static_cast<uint4*>(p.laid)[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+}
+
 uint32_t padded_rank(uint32_t r) { return r <= 16 ? 16u : r <= 32 ? 32u : r <= 64 ? 64u : 128u; }
 
 struct Layout {
@@ -958,6 +980,14 @@ Layout layout(const hqb_lora_set* s, uint32_t tokens, uint32_t tile_rows) {
     l.total += round_up(tiles * tile_rows * padded_rank(s->max_rank) * 4, 256);
   }
   return l;
+}
+
+// Whether a call lays B out: rows that no 16-byte copy fits, and tokens enough to pay for all adapters.
+bool lays_out(const hqb_lora_set* s, uint32_t tokens) {
+  return (s->max_rank & 7u) != 0 && tokens > kVoteTokens && s->adapters <= tokens / kLayTokens;
+}
+uint64_t laid_bytes(const hqb_lora_set* s) {
+  return round_up(static_cast<uint64_t>(s->adapters) * s->rows * round_up(s->max_rank, 8) * 2, 256);
 }
 
 bool set_ok(const hqb_lora_set* s) {
@@ -1034,7 +1064,7 @@ HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* s, uint32_t tokens
     const uint64_t n = layout(s, tokens, planned_rows(s, tokens, true, wide_y)).total;
     most = n > most ? n : most;
   }
-  return most;
+  return most + (lays_out(s, tokens) ? laid_bytes(s) : 0);
 }
 
 HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, const int32_t* ids, uint32_t tokens,
@@ -1057,8 +1087,9 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(s->a) | reinterpret_cast<uintptr_t>(s->b) |
                               reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(base) |
                               reinterpret_cast<uintptr_t>(y);
-  const uint64_t sizes = s->cols | s->rows | s->max_rank | x_stride | y_stride | (base != nullptr ? base_stride : 0);
-  const bool vec = (addresses & 15u) == 0 && (sizes & 7u) == 0;
+  const uint64_t sizes = s->cols | s->rows | x_stride | y_stride | (base != nullptr ? base_stride : 0);
+  const bool fits = (addresses & 15u) == 0 && (sizes & 7u) == 0, lay = fits && lays_out(s, tokens);
+  const bool vec = fits && (lay || (s->max_rank & 7u) == 0);
   LoraParams p{};
   p.s = *s;
   p.x = x;
@@ -1078,6 +1109,15 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
   // tiles at most: every group may end in a partly filled one
   const uint32_t groups = s->adapters + 1, full = tokens / 16 + groups;
   uint32_t tiles = tokens < full ? tokens : full;
+  p.pitch = s->max_rank;
+  if (lay) {
+    p.pitch = static_cast<uint32_t>(round_up(s->max_rank, 8));
+    p.laid = ws + hqb_lora_workspace_bytes(s, tokens, 0) - laid_bytes(s);
+    const uint64_t blocks = (static_cast<uint64_t>(s->adapters) * s->rows * (p.pitch / 8) + 255) / 256;
+    const cudaError_t e = launch_dependent(lora_lay_kernel, dim3(static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16)),
+                                           256, 0, 1, st, p);
+    if (e != cudaSuccess) return e;
+  }
   if (p.planned) {
     const Layout l = layout(s, tokens, p.tile_rows);
     p.tile_count = reinterpret_cast<uint32_t*>(ws + 256);

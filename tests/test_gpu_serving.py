@@ -625,6 +625,15 @@ def test_lora_groups_tokens(tokens, adapters, run):
     check_lora(x, a, b, ranks, scales, ids.repeat_interleave(run)[:tokens].contiguous(), base, BF16)
 
 
+@pytest.mark.parametrize("tokens,rows,adapters,rank", [
+    (257, 264, 3, 27), (1000, 520, 8, 61), (1100, 512, 100, 5), (3000, 1024, 7, 33), (2500, 256, 2, 121), (300, 64, 37, 1),
+    (300, 64, 38, 1)])
+@pytest.mark.parametrize("kind,y_kind", [(F16, F32), (BF16, BF16)])
+def test_lora_odd_ranks(kind, y_kind, tokens, rows, adapters, rank):
+    """Rows of b that no 16-byte access fits, on both sides of the tokens at which they are laid out."""
+    check_lora(*make_lora(rank, tokens, 256, rows, adapters, rank, kind, y_kind), y_kind)
+
+
 @pytest.mark.parametrize("tokens", [7, 500])
 def test_lora_defaults_and_no_base(tokens):
     x, a, b, _, _, ids, _ = make_lora(1, tokens, 256, 128, 3, 16, F16, F16, full=True)
