@@ -29,7 +29,7 @@ constexpr uint32_t kVoteTokens = kThreads, kCountTokens = 4 * kThreads, kCountGr
 // 21.6 / 30.8, 777 tokens 42.8 / 36.8; rank 64, 4096 x 4096, BF16: 500 tokens 21.9 / 23.7.
 constexpr uint64_t kClusterWork = 32768;
 constexpr uint32_t kMaxAdapters = 16383;
-constexpr uint32_t kLayTokens = 8;  // tokens an adapter from which its rows of B are laid out
+constexpr uint32_t kLayAdapters = 8;  // adapters whose rows of B are laid out for any number of tokens
 
 struct LoraTile {
   uint32_t group;  // adapter, or `adapters` for tokens without one
@@ -57,7 +57,7 @@ struct LoraParams {
   uint32_t splits;    // column ranges of the first product
   uint32_t stages;    // of lora_kernel's rings
   uint32_t pitch;     // elements of a row of b
-  void* laid;         // b in rows of `pitch`, where the call lays it out
+  void* laid;         // lora_lay_kernel: b in rows of `pitch`, which then is the call's b
   float* inner;       // [splits][max_tiles][tile_rows][padded rank]
 };
 
@@ -185,7 +185,7 @@ struct Expand {
     const uint32_t g = lane >> 2, q = lane & 3;
     rows = p.s.rows, pitch = p.pitch, rank = rank_, count = count_, ring = ring_, stages = stages_;
     based = p.base != nullptr;
-    b = static_cast<const T*>(p.laid != nullptr ? p.laid : p.s.b) + (static_cast<uint64_t>(min(group, p.s.adapters - 1)) * rows + 8 * (g >> 1) + (g & 1)) * pitch +
+    b = static_cast<const T*>(p.s.b) + (static_cast<uint64_t>(min(group, p.s.adapters - 1)) * rows + 8 * (g >> 1) + (g & 1)) * pitch +
         q * (RP == 16 ? 4 : 8);
 #pragma unroll
     for (int i = 0; i < kRowsEach; ++i) {
@@ -982,9 +982,11 @@ Layout layout(const hqb_lora_set* s, uint32_t tokens, uint32_t tile_rows) {
   return l;
 }
 
-// Whether a call lays B out: rows that no 16-byte copy fits, and tokens enough to pay for all adapters.
+// Whether a call lays B out: rows that no 16-byte copy fits, and tokens enough to pay for all adapters.  B200, us,
+// laid out / element by element, FP16, rank 27, 4096 x 4096: 1 token of 4 adapters 7.6 / 13.0; 48 of 8 9.4 / 28.5;
+// 256 of 130 45 / 115; 300 of 8 11.0 / 71; 2000 of 200 84 / 545; 1 of 8 at rank 57 and 11008 rows 14.0 / 22.2.
 bool lays_out(const hqb_lora_set* s, uint32_t tokens) {
-  return (s->max_rank & 7u) != 0 && tokens > kVoteTokens && s->adapters <= tokens / kLayTokens;
+  return (s->max_rank & 7u) != 0 && s->adapters <= kLayAdapters + tokens / 2;
 }
 uint64_t laid_bytes(const hqb_lora_set* s) {
   return round_up(static_cast<uint64_t>(s->adapters) * s->rows * round_up(s->max_rank, 8) * 2, 256);
@@ -1057,14 +1059,15 @@ extern "C" {
 HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* s, uint32_t tokens, int device) {
   (void)device;
   if (!set_ok(s) || tokens > 0x7FFFFFFFu) return 0;
-  if (tokens <= kVoteTokens) return 256;
+  const uint64_t laid = lays_out(s, tokens) ? laid_bytes(s) : 0;
+  if (tokens <= kVoteTokens) return 256 + laid;
   // the call's kernels depend on its alignment and output type too: room for any
   uint64_t most = layout(s, tokens, 16).total;
   for (const bool wide_y : {false, true}) {
     const uint64_t n = layout(s, tokens, planned_rows(s, tokens, true, wide_y)).total;
     most = n > most ? n : most;
   }
-  return most + (lays_out(s, tokens) ? laid_bytes(s) : 0);
+  return most + laid;
 }
 
 HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, const int32_t* ids, uint32_t tokens,
@@ -1117,6 +1120,7 @@ HQB_API int hqb_lora(const hqb_lora_set* s, const void* x, uint64_t x_stride, co
     const cudaError_t e = launch_dependent(lora_lay_kernel, dim3(static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16)),
                                            256, 0, 1, st, p);
     if (e != cudaSuccess) return e;
+    p.s.b = p.laid;
   }
   if (p.planned) {
     const Layout l = layout(s, tokens, p.tile_rows);

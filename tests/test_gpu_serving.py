@@ -626,8 +626,8 @@ def test_lora_groups_tokens(tokens, adapters, run):
 
 
 @pytest.mark.parametrize("tokens,rows,adapters,rank", [
-    (257, 264, 3, 27), (1000, 520, 8, 61), (1100, 512, 100, 5), (3000, 1024, 7, 33), (2500, 256, 2, 121), (300, 64, 37, 1),
-    (300, 64, 38, 1)])
+    (257, 264, 3, 27), (1000, 520, 8, 61), (1100, 512, 100, 5), (3000, 1024, 7, 33), (2500, 256, 2, 121), (300, 64, 158, 1),
+    (300, 64, 159, 1), (1, 512, 3, 27), (20, 264, 18, 13), (20, 264, 19, 13), (256, 520, 8, 63)])
 @pytest.mark.parametrize("kind,y_kind", [(F16, F32), (BF16, BF16)])
 def test_lora_odd_ranks(kind, y_kind, tokens, rows, adapters, rank):
     """Rows of b that no 16-byte access fits, on both sides of the tokens at which they are laid out."""
