@@ -925,11 +925,14 @@ def reference_inputs(name, device):
     return prefix, mats, xs
 
 
+NO_REFERENCE = "oracle/_ref/libharpq_ref.so is not built (oracle/build.py builds it from the reference's sources)"
+
+
 def time_reference(name, steps, warmup, device, threads=None, budget_s=None):
     from oracle import refcpu
 
     if not refcpu.available():
-        raise RuntimeError("oracle/_ref/libharpq_ref.so is not built")
+        raise RuntimeError(NO_REFERENCE)
     threads = threads or os.cpu_count() or 1
     prefix, mats, xs = reference_inputs(name, device)
     runners = [(lname, src, m, refcpu.ShardedReference(m, threads)) for lname, src, m in mats]
@@ -1057,7 +1060,10 @@ def main(argv=None) -> int:
     if args.impl == "reference":
         if rank != 0:
             return 0
-        print(json.dumps(run_reference_arm(args, device)), flush=True)
+        from oracle import refcpu
+
+        arm = run_reference_arm(args, device) if refcpu.available() else {"impl": "reference", "unavailable": NO_REFERENCE}
+        print(json.dumps(arm), flush=True)
         return 0
 
     if world > 1:
@@ -1080,8 +1086,13 @@ def main(argv=None) -> int:
             r70 = run_ours(sub, rank, world, device)
             result["supplementary"]["llama70b_mlp_p3_n1"] = {k: r70[k] for k in ("value", "unit", "ms_per_step")}
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
-        cb = time_reference(args.workload, 3, 1, device, budget_s=20.0)
-        result["cpu_baseline"] = {k: cb[k] for k in ("value", "unit", "cores", "kind", "sample")}
+        from oracle import refcpu
+
+        if refcpu.available():
+            cb = time_reference(args.workload, 3, 1, device, budget_s=20.0)
+            result["cpu_baseline"] = {k: cb[k] for k in ("value", "unit", "cores", "kind", "sample")}
+        else:
+            result["cpu_baseline"] = {"unavailable": NO_REFERENCE}
         result["cpu_baseline"]["numpy"] = time_numpy_reference(args.workload, device)
     if world > 1:
         torch.distributed.barrier()
