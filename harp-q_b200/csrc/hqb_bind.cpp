@@ -82,11 +82,15 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   p->parents = nullptr;
   p->mask = nullptr;
-  p->mask_words = 0;
+  p->mask_words = p->parent_count = 0;
   if (a[9] != Py_None) {
     const Tensor* tree = tensor(a[9]);
     p->mask_words = static_cast<uint32_t>(PyLong_AsUnsignedLong(a[14]));
-    if (tree == nullptr || p->mask_words == 0 || !ints(a[9], tree->numel(), device, false, &p->parents)) return status(kUnfit);
+    if (tree == nullptr || p->mask_words == 0 || !ints(a[9], tree->numel(), device, false, &p->parents) ||
+        tree->numel() > INT32_MAX)
+      return status(kUnfit);
+    p->parent_count = static_cast<uint32_t>(tree->numel());
+    if (p->parent_count == 0) p->parents = p->starts;  // none is read: a step without tokens
     p->mask = static_cast<uint32_t*>(PyLong_AsVoidPtr(a[13]));
   }
   return status(hqb_page_plan(p, stream_of(a[2], device)));

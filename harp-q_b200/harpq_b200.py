@@ -91,7 +91,7 @@ class PagedCacheC(ctypes.Structure):
 
 class PagePlanC(ctypes.Structure):
     _fields_ = [*[(n, u32) for n in ("requests", "page_size", "num_pages", "table_stride", "token_capacity",
-                                     "free_count", "mask_words", "reserved")],
+                                     "free_count", "mask_words", "parent_count")],
                 *[(n, vp) for n in ("context_lens", "new_lens", "held", "free_pages", "free_head", "parents", "tables",
                                     "starts", "token_request", "positions", "slots", "held_out", "free_head_out",
                                     "mask", "flags")]]
@@ -660,8 +660,9 @@ class PagePlan:
               tables: torch.Tensor | None = None, free_pages: torch.Tensor | None = None,
               free_head: torch.Tensor | None = None, parents: torch.Tensor | None = None, stream=None) -> "PagePlan":
         """Fills the buffers.  tables [requests, columns] (with free_pages and free_head) also gives the
-        new tokens pages and slots, writing new columns into it; parents [at least the step's
-        tokens] gives tree positions and masks.  held and free_head are the counts before the
+        new tokens pages and slots, writing new columns into it; parents (one a token, in token
+        order; a token past their end counts as a root, with HQB_DEVERR_INDEX) gives tree positions
+        and masks.  held and free_head are the counts before the
         step (a previous plan's, not this one's buffers)."""
         status = self._call(self._at, self._index, _raw_stream(stream), context_lens, new_lens, held, tables, free_pages,
                             free_head, parents, *self._outputs)

@@ -454,8 +454,9 @@ typedef struct hqb_paged_cache {
  *                        (starts[requests]: all of them)
  *   token_request[t]     request of token t          (each optional: NULL leaves it out)
  *   positions[t]         context + index in the request; with parents, context + depth
- *   mask[t][w]           with parents (an earlier node of the same request, or -1): bit j of
- *                        word j/32 set for j = t's node and its ancestors
+ *   mask[t][w]           with parents (parent_count entries in token order: an earlier node of
+ *                        the same request, or -1): bit j of word j/32 set for j = t's node and
+ *                        its ancestors
  * With tables (not NULL), the pages that the new tokens need beyond the held ones are taken
  * from free_pages[*free_head ..) in request order and written into the table rows:
  *   tables[r][c]         page of column c (in place: only new columns are written)
@@ -466,8 +467,8 @@ typedef struct hqb_paged_cache {
  * the tokens without a page get slot -1 and the counts stop there.  HQB_DEVERR_INDEX: a
  * negative length or head (taken as 0), more pages held than a table row has (taken as the
  * row), fewer held than the context fills (the missing ones are taken as new pages), more
- * tokens than token_capacity (left out), a parent that is not earlier (taken as -1) or a node
- * past the mask (its bit is left out). */
+ * tokens than token_capacity (left out), a parent that is not earlier or a token past
+ * parent_count (its parent taken as -1), or a node past the mask (its bit is left out). */
 typedef struct hqb_page_plan_args {
   uint32_t requests;
   uint32_t page_size;
@@ -476,7 +477,7 @@ typedef struct hqb_page_plan_args {
   uint32_t token_capacity;
   uint32_t free_count; /* entries of free_pages */
   uint32_t mask_words; /* words of a mask row; 0 without a mask */
-  uint32_t reserved;
+  uint32_t parent_count; /* entries of parents */
   const int32_t* context_lens;
   const int32_t* new_lens;
   const int32_t* held;
