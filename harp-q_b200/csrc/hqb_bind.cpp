@@ -2,10 +2,12 @@
 //
 // A step's smallest calls take a few microseconds on the GPU, less than checking a dozen tensors
 // through Python attributes.  Each function here checks its tensors, fills the argument structure
-// and calls the C entry point; it returns that call's status, or -1 without calling where an
-// argument does not fit, and the Python method then says which.
+// and calls the C entry point with the tensors' device current (it launches on the current one); it
+// returns that call's status, or -1 without calling where an argument does not fit, and the Python
+// method then says which.
 #include <Python.h>
 
+#include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -49,6 +51,16 @@ void* stream_of(PyObject* o, int device) {
 
 PyObject* status(long s) { return PyLong_FromLong(s); }
 
+// Makes GPU `device` current until the end of the scope: of two GPUs' default streams, both handle 0,
+// a launch takes the current one's.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) : guard_(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))) {}
+
+ private:
+  c10::DeviceGuard guard_;
+};
+
 // page_plan(args address, device, stream, context_lens, new_lens, held, tables, free_pages, free_head,
 //           parents, slots, held_out, free_head_out, mask, words)
 // The structure at args has the plan's sizes and output addresses; the last five are outputs that
@@ -57,6 +69,7 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 15) return status(kUnfit);
   auto* p = static_cast<hqb_page_plan_args*>(PyLong_AsVoidPtr(a[0]));
   const int device = static_cast<int>(PyLong_AsLong(a[1]));
+  const OnDevice on(device);
   const Tensor* table = nullptr;
   const int32_t* rows = nullptr;
   if (!ints(a[3], p->requests, device, false, &p->context_lens) || !ints(a[4], p->requests, device, false, &p->new_lens) ||
@@ -101,6 +114,7 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 8) return status(kUnfit);
   const auto* c = static_cast<const hqb_paged_cache*>(PyLong_AsVoidPtr(a[0]));
   const int device = static_cast<int>(PyLong_AsLong(a[1]));
+  const OnDevice on(device);
   const Tensor *k, *v, *slots = tensor(a[5]);
   if (slots == nullptr || !heads(a[3], -1, c->kv_heads, c->head_dim, -1, device, &k) ||
       !heads(a[4], k->size(0), c->kv_heads, c->head_dim, code(k->scalar_type()), device, &v) || k->strides() != v->strides() ||
@@ -125,6 +139,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto* c = static_cast<const hqb_paged_cache*>(PyLong_AsVoidPtr(a[0]));
   hqb_attention_args p = *static_cast<const hqb_attention_args*>(PyLong_AsVoidPtr(a[1]));
   const int device = static_cast<int>(PyLong_AsLong(a[4]));
+  const OnDevice on(device);
   const Tensor *q, *k, *v, *out, *table = tensor(a[9]), *ctx = tensor(a[10]);
   if (ctx == nullptr || table == nullptr || !heads(a[6], -1, p.q_heads, c->head_dim, c->dtype, device, &q)) return status(kUnfit);
   const int64_t tokens = q->size(0), requests = ctx->numel();
@@ -187,6 +202,7 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 9) return status(kUnfit);
   const auto* s = static_cast<const hqb_lora_set*>(PyLong_AsVoidPtr(a[0]));
   const int device = static_cast<int>(PyLong_AsLong(a[3]));
+  const OnDevice on(device);
   const Tensor *x, *base = nullptr, *out = tensor(a[8]);
   uint64_t x_stride = 0, base_stride = 0, out_stride = 0;
   const int32_t* ids;
