@@ -70,15 +70,16 @@ def gemv(x: torch.Tensor, planes: List[torch.Tensor], rows: int, cols: int, pref
     x = x.contiguous()
     m = _plane_matrix(planes, rows, cols)
     xd = hqb._dtype_code(x)
-    stream = torch.cuda.current_stream(x.device).cuda_stream
-    ws = _workspace(m, x.device, stream, x.shape[0], xd)
-    y = torch.empty(x.shape[0], rows, dtype=out_dtype, device=x.device)
-    if bias is not None:
-        bias = bias.contiguous()
-    status = hqb.lib().hqb_gemv(ctypes.byref(m), prefix, x.data_ptr(), xd, x.shape[0],
-                                None if bias is None else bias.data_ptr(),
-                                hqb.F32 if bias is None else hqb._dtype_code(bias), y.data_ptr(),
-                                hqb._dtype_code(y), ws.ptr(), ws.nbytes, stream)
+    with torch.cuda.device(x.device):  # the library launches on the current device
+        stream = torch.cuda.current_stream(x.device).cuda_stream
+        ws = _workspace(m, x.device, stream, x.shape[0], xd)
+        y = torch.empty(x.shape[0], rows, dtype=out_dtype, device=x.device)
+        if bias is not None:
+            bias = bias.contiguous()
+        status = hqb.lib().hqb_gemv(ctypes.byref(m), prefix, x.data_ptr(), xd, x.shape[0],
+                                    None if bias is None else bias.data_ptr(),
+                                    hqb.F32 if bias is None else hqb._dtype_code(bias), y.data_ptr(),
+                                    hqb._dtype_code(y), ws.ptr(), ws.nbytes, stream)
     hqb.check(status, "hqb_gemv")
     return y
 

@@ -1,4 +1,5 @@
-"""CPU: the serving operators' binding makes its tensors' GPU current around the library's calls.
+"""CPU: the serving operators' binding, and the GEMV operator, make their tensors' GPU current around
+the library's calls.
 
 PyTorch's device switch is replaced by one that records (tests/native/recording_device_guard.cpp),
 in a process of its own; fake tensors stand in for tensors on a second GPU, so nothing is launched."""
@@ -65,3 +66,37 @@ def test_binding_makes_the_tensors_device_current(tmp_path):
                          env={**os.environ, "PYTHONPATH": str(REPO / "harp-q_b200"), "CUDA_VISIBLE_DEVICES": ""})
     assert run.returncode == 0, run.stderr
     assert run.stdout.split("\n")[:-1] == [f"{name} [1, 0]" for name in ("page_plan", "cache_append", "tree_attention", "lora")]
+
+
+def test_gemv_operator_makes_its_inputs_device_current(monkeypatch):
+    import harpq_b200 as hqb
+    import harpq_b200_ops
+
+    inside, seen = [], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            inside.append(self.device)
+
+        def __exit__(self, *_):
+            inside.pop()
+
+    class Library:
+        @staticmethod
+        def hqb_gemv(*_):
+            seen.append(list(inside))
+            return 0
+
+    planes = [torch.zeros(hqb.plane_bytes(hqb.geometry(128, 128)), dtype=torch.uint8)]
+    x, stream = torch.zeros(2, 128, dtype=torch.float16), type("Stream", (), {"cuda_stream": 7})
+    scratch = type("Scratch", (), {"ptr": lambda self: 256, "nbytes": 256})()
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: stream)
+    monkeypatch.setattr(harpq_b200_ops, "_plane_matrix", lambda *_: hqb.PlaneMatrixC())
+    monkeypatch.setattr(harpq_b200_ops, "_workspace", lambda *_: scratch)
+    monkeypatch.setattr(hqb, "lib", lambda: Library)
+    harpq_b200_ops.gemv._init_fn(x, planes, 128, 128, 1)
+    assert seen == [[x.device]]
