@@ -622,6 +622,19 @@ def _ints(name: str, t: torch.Tensor, n: int, device: int) -> None:
                          f"got {list(t.shape)} {t.dtype} on {t.device}")
 
 
+def _on_gpu(name: str, t: torch.Tensor) -> None:
+    """Refuses host memory: its address means nothing to a kernel."""
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a GPU, got {t.device}")
+
+
+def _own_workspace(ws: Workspace, device: int) -> Workspace:
+    """A workspace that a caller brings, refused where it is not on GPU `device`."""
+    if ws.buf.get_device() != device:
+        raise ValueError(f"the workspace must be on GPU {device}, got {ws.buf.device}")
+    return ws
+
+
 def _table(name: str, t: torch.Tensor, rows: int, device: int) -> None:
     """Refuses what is no int32 matrix of `rows` rows."""
     if t.dim() != 2 or t.shape[0] != rows:
@@ -647,6 +660,7 @@ class PagePlan:
         parts = torch.zeros(sum(sizes), dtype=torch.int32, device=device or "cuda").split(sizes)
         self.starts, self.requests, self.positions, self.slots, self.held, self.free_head, self.flags, mask = parts
         self.mask = mask.view(tokens, self.words) if self.words else None
+        _on_gpu("a plan's buffers", self.starts)
         self.device = self.starts.device
         self._index = _device_index(self.device)
         at = [t.data_ptr() for t in parts]
@@ -703,6 +717,9 @@ class PagedCache:
             raise TypeError(f"unsupported dtype {k.dtype}; use float16 or bfloat16")
         if k.stride(3) != 1 and k.shape[3] > 1:
             raise ValueError("a head's elements must be adjacent")
+        _on_gpu("k and v", k)
+        if flags is not None:
+            _ints("flags", flags, 1, _device_index(k.device))
         self.k, self.v = k, v
         self.num_pages, self.page_size, self.heads, self.dim = k.shape
         self.dtype, self.device = k.dtype, k.device
@@ -761,7 +778,7 @@ class TreeAttention:
         need = lib().hqb_tree_attention_workspace_bytes(cache._at, self._at, cache._index)
         if need == 0:
             raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
-        self.ws = Workspace(need, cache.device) if workspace is None else workspace(need)
+        self.ws = Workspace(need, cache.device) if workspace is None else _own_workspace(workspace(need), cache._index)
         self._ws, self._ws_bytes = self.ws.ptr(), self.ws.nbytes
         self._scale = cache.dim ** -0.5
         self._call = bind().tree_attention
@@ -824,6 +841,7 @@ class LoraSet:
             raise TypeError("a and b must share a type: float16 or bfloat16")
         if not a.is_contiguous() or not b.is_contiguous() or a.device != b.device:
             raise ValueError("a and b must be contiguous and on one device")
+        _on_gpu("a and b", a)
         self.adapters, self.max_rank, self.cols = a.shape
         self.rows = b.shape[1]
         if self.adapters < 1 or self.rows < 1 or self.cols < 1:
@@ -876,9 +894,12 @@ class LoraSet:
             kind = y_dtype or (base.dtype if base is not None else x.dtype)
             out = torch.empty(x.shape[0], self.rows, dtype=kind, device=self.device)
         s = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else _raw_stream(stream)
-        ws = workspace or self._ws.get(s)
-        if ws is None or (workspace is None and x.shape[0] > ws.tokens):
-            ws = self.workspace(x.shape[0], s)
+        if workspace is not None:
+            ws = _own_workspace(workspace, self._index)
+        else:
+            ws = self._ws.get(s)
+            if ws is None or x.shape[0] > ws.tokens:
+                ws = self.workspace(x.shape[0], s)
         status = self._call(self._at, ws.ptr(), ws.nbytes, self._index, s, x, ids, base, out)
         if status:
             if status == _UNFIT:

@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import harpq_b200 as hqb  # noqa: E402
-from test_gpu_serving import ints, plan_reference  # noqa: E402
+from test_gpu_serving import BF16, F16, ints, make_lora, plan_reference  # noqa: E402
 
 
 # ---- page plan ----------------------------------------------------------------------------
@@ -35,3 +35,15 @@ def test_plan_of_no_tokens_takes_no_parents():
     plan = hqb.PagePlan(2, 3, 16, 8, max_new=4)
     plan.build(ints([9, 4]), ints([0, 0]), parents=ints([]))
     assert plan.starts.tolist() == [0, 0, 0] and plan.positions.tolist() == [-1] * 3 and plan.flags.item() == 0
+
+
+# ---- memory that callers bring --------------------------------------------------------------
+
+
+def test_workspaces_in_host_memory_are_refused():
+    k = torch.zeros(4, 16, 2, 64, dtype=F16, device="cuda")
+    with pytest.raises(ValueError):
+        hqb.TreeAttention(hqb.PagedCache(k, k), 4, 1, 3, 3, 10, workspace=lambda need: hqb.Workspace(need, "cpu"))
+    x, a, b, ranks, scales, ids, base = make_lora(1, 5, 64, 32, 2, 8, BF16, BF16)
+    with pytest.raises(ValueError):
+        hqb.LoraSet(a, b, ranks, scales).apply(x, ids, base=base, workspace=hqb.Workspace(1 << 20, "cpu"))

@@ -145,3 +145,22 @@ def test_operators_have_no_cpu_fallback():
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.ops.harpq_b200.lora(x, torch.zeros(1, 8, 64, dtype=torch.float16), torch.zeros(1, 4, 8, dtype=torch.float16),
                                   torch.zeros(2, dtype=torch.int32))
+
+
+def test_host_memory_is_refused():
+    """Before any address of it reaches a kernel."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    cache = torch.zeros(4, 16, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        hqb.PagedCache(cache, cache)
+    with pytest.raises(ValueError):
+        hqb.LoraSet(torch.zeros(2, 8, 64, dtype=torch.float16), torch.zeros(2, 32, 8, dtype=torch.float16), max_tokens=0)
+    with pytest.raises(ValueError):
+        hqb.PagePlan(1, 1, 16, 8, device="cpu")
+    with FakeTensorMode():
+        k = torch.empty(4, 16, 2, 64, dtype=torch.float16, device="cuda:0")
+        for flags in (torch.empty(1, dtype=torch.int32), torch.empty(1, device="cuda:0"), torch.empty(0, dtype=torch.int32, device="cuda:0"),
+                      torch.empty(1, dtype=torch.int32, device="cuda:1")):
+            with pytest.raises(ValueError):
+                hqb.PagedCache(k, k, flags)
