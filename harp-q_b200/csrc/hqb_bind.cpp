@@ -219,6 +219,16 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
                          PyLong_AsVoidPtr(a[1]), PyLong_AsUnsignedLongLong(a[2]), stream_of(a[4], device)));
 }
 
+// capture(device, stream) -> hqb_stream_capture's number
+PyObject* capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2) return status(kUnfit);
+  const OnDevice on(static_cast<int>(PyLong_AsLong(a[0])));
+  uint64_t id = 0;
+  const int s = hqb_stream_capture(PyLong_AsVoidPtr(a[1]), &id);
+  if (s != HQB_OK) return PyErr_Format(PyExc_RuntimeError, "hqb_stream_capture: status %d (%s)", s, hqb_status_string(s));
+  return PyLong_FromUnsignedLongLong(id);
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   try {
@@ -240,7 +250,8 @@ PyMethodDef method(const char* name) {
 }
 
 PyMethodDef kMethods[] = {method<page_plan>("page_plan"), method<cache_append>("cache_append"),
-                          method<tree_attention>("tree_attention"), method<lora>("lora"), {nullptr, nullptr, 0, nullptr}};
+                          method<tree_attention>("tree_attention"), method<lora>("lora"), method<capture>("capture"),
+                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "harpq_b200_bind", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -2552,6 +2552,18 @@ HQB_API int hqb_workspace_error(const void* workspace, int* host_flags, void* st
   return cudaStreamSynchronize(as_stream(stream));
 }
 
+HQB_API int hqb_stream_capture(void* stream, uint64_t* capture) {
+  if (capture == nullptr) return HQB_ERR_INVALID;
+  *capture = 0;
+  const cudaStream_t st = as_stream(stream);
+  if (st == nullptr || st == cudaStreamLegacy) return HQB_OK;  // the legacy stream cannot be captured
+  cudaStreamCaptureStatus now = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(st, &now, &id);
+  if (e == cudaSuccess && now == cudaStreamCaptureStatusActive) *capture = id + 1;
+  return e;
+}
+
 HQB_API uint64_t hqb_depth_plan_bytes(uint32_t grid_rows) { return (static_cast<uint64_t>(grid_rows) + 1) * 4; }
 
 HQB_API int hqb_depth_plan(const uint8_t* depth, uint32_t grid_rows, uint32_t grid_cols, uint32_t stage_count,

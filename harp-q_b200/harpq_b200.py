@@ -120,6 +120,7 @@ EXPORTS = {
     "hqb_workspace_bytes": (u64, [ctypes.POINTER(PlaneMatrixC), u32, i32, i32]),
     "hqb_workspace_init": (i32, [vp, u64, vp]),
     "hqb_workspace_error": (i32, [vp, ctypes.POINTER(i32), vp]),
+    "hqb_stream_capture": (i32, [vp, ctypes.POINTER(u64)]),
     "hqb_depth_plan_bytes": (u64, [u32]),
     "hqb_depth_plan": (i32, [vp, u32, u32, u32, vp, vp, vp]),
     "hqb_gemv": (i32, [ctypes.POINTER(PlaneMatrixC), u32, vp, i32, u32, vp, i32, vp, i32, vp, u64, vp]),
@@ -257,10 +258,15 @@ def prepare_x(x: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> 
 
 
 class Workspace:
-    """Caller-owned scratch for GEMV launches (cleared once at allocation)."""
+    """Caller-owned scratch of launches, cleared once at allocation: as much as a GEMV needs (all of
+    it), or the first `clear` bytes (the serving operators: the error word's)."""
 
-    def __init__(self, nbytes: int, device=None, stream=None):
-        self.buf = torch.zeros(max(256, nbytes), dtype=torch.uint8, device=device or "cuda")
+    def __init__(self, nbytes: int, device=None, stream=None, clear: int | None = None):
+        if clear is None:
+            self.buf = torch.zeros(max(256, nbytes), dtype=torch.uint8, device=device or "cuda")
+        else:
+            self.buf = torch.empty(max(256, nbytes), dtype=torch.uint8, device=device or "cuda")
+            self.buf[:clear].zero_()
         self.nbytes = self.buf.numel()
 
     def ptr(self) -> int:
@@ -642,6 +648,44 @@ def _table(name: str, t: torch.Tensor, rows: int, device: int) -> None:
     _ints(name, t, t.numel(), device)
 
 
+class StreamWorkspaces:
+    """The workspaces of calls that bring none: one a stream, grown in powers of two.
+
+    A call under capture gets one that belongs to its capture, from its graph's memory pool, whose
+    error word each replay clears: the graph may be replayed on any stream, beside eager calls and
+    other graphs.  The newest capture's is held here, for its error word; the graph keeps the memory
+    of all of them."""
+
+    def __init__(self, device: torch.device, bytes_of):
+        self.device, self.bytes_of = device, bytes_of  # bytes_of(size): what calls up to `size` need
+        self._index, self._capture = _device_index(device), bind().capture
+        self.eager: dict = {}
+        self.captured: dict = {}
+
+    def take(self, size: int, stream: int) -> Workspace:
+        """A workspace for a call of `size` on a stream."""
+        capture = self._capture(self._index, stream)
+        if capture:
+            last = self.captured.get(stream)
+            if last is None or last[0] != capture or size > last[1].size:
+                last = self.captured[stream] = (capture, self._make(size, stream, None))
+            return last[1]
+        ws = self.eager.get(stream)
+        if ws is None or size > ws.size:
+            ws = self.eager[stream] = self._make(size, stream, ws)
+        return ws
+
+    def _make(self, size: int, stream: int, smaller: Workspace | None) -> Workspace:
+        size = 1 << (size - 1).bit_length()
+        # on the stream that uses it: the allocator then reuses it in that order
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
+            ws = Workspace(self.bytes_of(size), self.device, clear=256)
+            if smaller is not None:
+                ws.buf[:256].copy_(smaller.buf[:256])  # the error word
+        ws.size = size
+        return ws
+
+
 class PagePlan:
     """One decode step's lengths as addresses (hqb_page_plan), in buffers that are kept between
     steps: starts [requests + 1], requests, positions and slots [tokens] (entries past the
@@ -778,7 +822,7 @@ class TreeAttention:
         need = lib().hqb_tree_attention_workspace_bytes(cache._at, self._at, cache._index)
         if need == 0:
             raise ValueError("hqb_tree_attention_workspace_bytes rejected the shape")
-        self.ws = Workspace(need, cache.device) if workspace is None else _own_workspace(workspace(need), cache._index)
+        self.ws = Workspace(need, cache.device, clear=256) if workspace is None else _own_workspace(workspace(need), cache._index)
         self._ws, self._ws_bytes = self.ws.ptr(), self.ws.nbytes
         self._scale = cache.dim ** -0.5
         self._call = bind().tree_attention
@@ -830,8 +874,9 @@ class TreeAttention:
 class LoraSet:
     """Low-rank adapters stacked in two device tensors: a [adapters, max_rank, cols] and b
     [adapters, rows, max_rank] (FP16 or BF16), with ranks [adapters] int32 (None: max_rank each)
-    and scales [adapters] FP32 (None: 1).  Workspaces are kept per stream; the constructing
-    stream's is made at once, for up to max_tokens tokens (0: when it is first needed)."""
+    and scales [adapters] FP32 (None: 1).  Workspaces are kept per stream and capture (see
+    StreamWorkspaces); the constructing stream's is made at once, for up to max_tokens tokens (0:
+    when it is first needed)."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, ranks: torch.Tensor | None = None,
                  scales: torch.Tensor | None = None, max_tokens: int = 8192):
@@ -859,8 +904,8 @@ class LoraSet:
                           self.max_rank, _SERVING_DTYPES[a.dtype], 0)
         self._at, self._index = ctypes.addressof(self.c), _device_index(a.device)
         self._call = bind().lora
-        self._ws: dict = {}
-        self._kept: list = []
+        self._workspaces = StreamWorkspaces(self.device, self.workspace_bytes)
+        self._ws = self._workspaces.eager
         if max_tokens > 0:
             self.workspace(max_tokens, torch.cuda.current_stream(a.device).cuda_stream)
 
@@ -868,21 +913,8 @@ class LoraSet:
         return lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
 
     def workspace(self, tokens: int, stream: int) -> Workspace:
-        """The stream's workspace, grown to what `tokens` tokens need (in powers of two; the smaller
-        ones stay too, since a captured graph may hold them)."""
-        ws = self._ws.get(stream)
-        if ws is None or tokens > ws.tokens:
-            tokens = 1 << (tokens - 1).bit_length()
-            need = self.workspace_bytes(tokens)
-            if stream == torch.cuda.current_stream(self.device).cuda_stream:
-                ws = Workspace(need, self.device)
-            else:  # allocated on the stream that uses it: the allocator then reuses it in that order
-                with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
-                    ws = Workspace(need, self.device)
-            ws.tokens = tokens
-            self._ws[stream] = ws
-            self._kept.append(ws)
-        return ws
+        """The stream's workspace, or under capture the capture's, grown to what `tokens` tokens need."""
+        return self._workspaces.take(tokens, stream)
 
     def apply(self, x: torch.Tensor, ids: torch.Tensor, base: torch.Tensor | None = None,
               out: torch.Tensor | None = None, y_dtype: torch.dtype | None = None, workspace: Workspace | None = None,
@@ -894,12 +926,7 @@ class LoraSet:
             kind = y_dtype or (base.dtype if base is not None else x.dtype)
             out = torch.empty(x.shape[0], self.rows, dtype=kind, device=self.device)
         s = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else _raw_stream(stream)
-        if workspace is not None:
-            ws = _own_workspace(workspace, self._index)
-        else:
-            ws = self._ws.get(s)
-            if ws is None or x.shape[0] > ws.tokens:
-                ws = self.workspace(x.shape[0], s)
+        ws = self._workspaces.take(x.shape[0], s) if workspace is None else _own_workspace(workspace, self._index)
         status = self._call(self._at, ws.ptr(), ws.nbytes, self._index, s, x, ids, base, out)
         if status:
             if status == _UNFIT:

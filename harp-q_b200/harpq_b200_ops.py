@@ -98,19 +98,17 @@ def _gemv_fake(x, planes, rows, cols, prefix, bias=None, out_dtype=torch.float16
 #   lora(x, a, b, ids, ranks, scales, base, out_dtype)         -> [tokens, rows]
 #
 # The same calls and the same bits as PagedCache.append, TreeAttention and LoraSet.apply, whose
-# arguments they share, without a handle to keep.  Workspaces are cached per stream in sizes of powers
-# of two, none of which is freed: a captured graph may hold it.
+# arguments they share, without a handle to keep.  Workspaces are kept per stream and capture
+# (harpq_b200.StreamWorkspaces).
 
 _SERVING_WORKSPACES: dict = {}
 
 
 def _serving_workspace(kind: str, device: torch.device, stream: int, need: int) -> "hqb.Workspace":
-    size = 1 << (need - 1).bit_length()
-    key = (kind, device.index, stream, size)
-    ws = _SERVING_WORKSPACES.get(key)
-    if ws is None:
-        ws = _SERVING_WORKSPACES[key] = hqb.Workspace(size, device)
-    return ws
+    key = (kind, device.index)
+    if key not in _SERVING_WORKSPACES:
+        _SERVING_WORKSPACES[key] = hqb.StreamWorkspaces(device, lambda size: size)
+    return _SERVING_WORKSPACES[key].take(need, stream)
 
 
 def _serving_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, stream: int) -> "hqb.PagedCache":

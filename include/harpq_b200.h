@@ -174,6 +174,10 @@ HQB_API uint64_t hqb_workspace_bytes(const hqb_plane_matrix* m, uint32_t batch, 
 HQB_API int hqb_workspace_init(void* workspace, uint64_t bytes, void* stream);
 /* Copies the workspace error word (HQB_DEVERR_* bits) to *host_flags, synchronously. */
 HQB_API int hqb_workspace_error(const void* workspace, int* host_flags, void* stream);
+/* *capture: a number of the capture under way on the stream (the same for all of one capture's
+ * streams, another for each capture), 0 without one.  What a captured call is given has to last, and
+ * stay untouched by other work, as long as its graph is replayed. */
+HQB_API int hqb_stream_capture(void* stream, uint64_t* capture);
 
 /* ---- mixed depth ------------------------------------------------------------------ */
 
@@ -546,7 +550,8 @@ typedef struct hqb_attention_args {
   uint64_t out_token_stride, out_head_stride;
 } hqb_attention_args;
 /* Scratch bytes of a call (its pointers are not looked at); 0 for arguments that are refused.
- * It starts with the error word (hqb_workspace_error); hqb_workspace_init clears it once. */
+ * It starts with the error word (hqb_workspace_error), which has to start at zero; what the rest
+ * holds does not matter. */
 HQB_API uint64_t hqb_tree_attention_workspace_bytes(const hqb_paged_cache* cache, const hqb_attention_args* args,
                                                     int device);
 HQB_API int hqb_tree_attention(const hqb_paged_cache* cache, const hqb_attention_args* args, void* workspace,

@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import harpq_b200 as hqb  # noqa: E402
-from test_gpu_serving import BF16, F16, ints, make_lora, plan_reference  # noqa: E402
+from test_gpu_serving import BF16, F16, ints, make_attention, make_lora, plan_reference  # noqa: E402
 
 
 # ---- page plan ----------------------------------------------------------------------------
@@ -47,3 +47,75 @@ def test_workspaces_in_host_memory_are_refused():
     x, a, b, ranks, scales, ids, base = make_lora(1, 5, 64, 32, 2, 8, BF16, BF16)
     with pytest.raises(ValueError):
         hqb.LoraSet(a, b, ranks, scales).apply(x, ids, base=base, workspace=hqb.Workspace(1 << 20, "cpu"))
+
+
+def test_captures_have_workspaces_of_their_own():
+    """Two graphs captured on one stream, and eager calls on it, may run at once."""
+    import harpq_b200_ops  # noqa: F401
+
+    many = make_lora(2, 3000, 256, 128, 5, 32, BF16, BF16)
+    a, b, ranks, scales = many[1:5]
+    s = hqb.LoraSet(a, b, ranks, scales, max_tokens=0)
+    sizes = (3000, 1700, 2300)
+    inputs = [(many[0][:n].clone(), many[5][:n].clone(), many[6][:n].clone()) for n in sizes]
+    want = [s.apply(x, ids, base=base).clone() for x, ids, base in inputs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs, places = [], [], []
+    for x, ids, base in inputs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append((s.apply(x, ids, base=base), torch.ops.harpq_b200.lora(x, a, b, ids, ranks, scales, base)))
+            places.append(s.workspace(len(x), side.cuda_stream).ptr())
+        graphs.append(graph)
+    with torch.cuda.stream(side):
+        places.append(s.workspace(3000, side.cuda_stream).ptr())
+        assert s.workspace(3000, side.cuda_stream).error_flags() == 0  # though no graph has run yet
+    assert len(set(places)) == 3
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(side):
+            eager = s.apply(*inputs[2][:2], base=inputs[2][2])
+    torch.cuda.synchronize()
+    assert torch.equal(eager, want[2])
+    for (own, op), w in zip(outs, want):
+        assert torch.equal(own, w) and torch.equal(op, w)
+
+
+def test_captured_operators_of_attention_have_workspaces_of_their_own():
+    import harpq_b200_ops
+
+    graphs, outs, want, keep, places = [], [], [], [], []
+    side = torch.cuda.Stream()
+    for seed in (1, 2):
+        s = make_attention(seed, [3000, 2000], [9, 7], 16, 2, 64, 16, F16)
+        keep.append((s["q"], s["k"], s["v"], s["kc"], s["vc"], s["tables"], ints(s["ctx"]), ints(s["starts"]), s["mask"], s["most"], 3000))
+        want.append(torch.ops.harpq_b200.tree_attention(*keep[-1]))
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(torch.ops.harpq_b200.tree_attention(*keep[-1]))
+            place = harpq_b200_ops._serving_workspace("attention", keep[-1][0].device, side.cuda_stream, 1).ptr()
+        assert place not in places
+        places.append(place)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_a_grown_workspace_keeps_its_error_word():
+    x, a, b, ranks, scales, ids, base = make_lora(3, 3000, 256, 64, 2, 16, F16, F16, full=True)
+    s = hqb.LoraSet(a, b, ranks, scales, max_tokens=0)
+    bad = ids[:300].clone()
+    bad[7] = 9
+    s.apply(x[:300], bad, base=base[:300])
+    s.apply(x, ids, base=base)
+    assert s.workspace(1, torch.cuda.current_stream().cuda_stream).error_flags() == hqb.DEVERR_INDEX

@@ -164,3 +164,9 @@ def test_host_memory_is_refused():
                       torch.empty(1, dtype=torch.int32, device="cuda:1")):
             with pytest.raises(ValueError):
                 hqb.PagedCache(k, k, flags)
+
+
+def test_the_default_stream_is_never_captured():
+    number = ctypes.c_uint64(7)
+    assert hqb.lib().hqb_stream_capture(None, ctypes.byref(number)) == 0 and number.value == 0
+    assert hqb.lib().hqb_stream_capture(None, None) == INVALID
