@@ -50,7 +50,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarp
   Walk w;
   const bool work = w.begin(p, blockIdx.x, bad);
   if (threadIdx.x == 0 && !p.whole) note_split(p, w, blockIdx.x, work, bad);
-  if (!work) return;
+  if (!work) {
+    if (bad != 0 && blockIdx.x == 0) atomicOr(p.error, static_cast<int>(bad));  // there may be no work at all
+    return;
+  }
   const uint32_t dim = p.c.head_dim;
   const T* const kc = static_cast<const T*>(p.c.k);
   const T* const vc = static_cast<const T*>(p.c.v);

@@ -119,3 +119,16 @@ def test_a_grown_workspace_keeps_its_error_word():
     s.apply(x[:300], bad, base=base[:300])
     s.apply(x, ids, base=base)
     assert s.workspace(1, torch.cuda.current_stream().cuda_stream).error_flags() == hqb.DEVERR_INDEX
+
+
+# ---- tree attention -------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("hq", [1, 16])
+@pytest.mark.parametrize("max_context", [40, 4000])
+@pytest.mark.parametrize("ctx,starts", [([40], [2, 0]), ([40], [-1, -1]), ([-5], [0, 0]), ([3, 40], [4, 1, 0]), ([40], [9, 9])])
+def test_attention_reports_bad_lengths_where_nothing_is_left_to_do(hq, max_context, ctx, starts):
+    s = make_attention(12, [40, 40], [2, 2], hq, 1, 64, 16, F16)
+    attend = hqb.TreeAttention(hqb.PagedCache(s["kc"], s["vc"]), hq, 2, 4, 2, max_context)
+    attend(s["q"], s["k"], s["v"], s["tables"][:len(ctx)].contiguous(), ints(ctx), ints(starts), s["mask"])
+    assert attend.ws.error_flags() == hqb.DEVERR_INDEX
