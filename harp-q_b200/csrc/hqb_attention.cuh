@@ -64,8 +64,8 @@ struct Request {
 
 __device__ __forceinline__ Request load_request(const AttnParams& p, uint32_t r, uint32_t& bad) {
   Request q;
-  const int32_t s0 = __ldg(p.a.starts + r), s1 = __ldg(p.a.starts + r + 1);
-  const int32_t c = __ldg(p.a.context_lens + r);
+  const int32_t s0 = p.a.starts[r], s1 = p.a.starts[r + 1];
+  const int32_t c = p.a.context_lens[r];
   const uint32_t cap = p.a.tokens;
   q.start = s0 < 0 ? 0u : min(static_cast<uint32_t>(s0), cap);
   const uint32_t end = s1 < 0 ? 0u : min(static_cast<uint32_t>(s1), cap);
@@ -232,7 +232,7 @@ __device__ __forceinline__ float2* part_stats(const AttnParams& p, uint32_t cta,
 __device__ __forceinline__ uint64_t key_offset(const AttnParams& p, const int32_t* table, uint32_t key, uint32_t head,
                                                uint32_t& bad) {
   const uint32_t column = p.by_page.quotient(key), inside = key - column * p.c.page_size;
-  uint32_t page = static_cast<uint32_t>(__ldg(table + column));
+  uint32_t page = static_cast<uint32_t>(table[column]);
   if (page >= p.c.num_pages) {
     bad |= HQB_DEVERR_PAGES;
     page = 0;
@@ -244,7 +244,7 @@ __device__ __forceinline__ uint64_t key_offset(const AttnParams& p, const int32_
 __device__ __forceinline__ uint32_t node_mask(const AttnParams& p, const Request& q, uint32_t node, uint32_t word) {
   uint32_t bits;
   if (p.a.mask != nullptr) {
-    bits = __ldg(p.a.mask + static_cast<uint64_t>(q.start + node) * p.a.mask_words + word);
+    bits = p.a.mask[static_cast<uint64_t>(q.start + node) * p.a.mask_words + word];
   } else {
     const int32_t n = static_cast<int32_t>(node) + 1 - static_cast<int32_t>(word * 32);  // nodes 0 .. node
     bits = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;

@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
           auto locate = [&](uint32_t b) {
             const uint32_t key = b * kKeys + (box << box_shift), column = p.by_page.quotient(key);
             const bool real = b < w.q.cached_blocks && key < w.q.ctx && h < DP / 64;
-            page = real ? static_cast<uint32_t>(__ldg(table + column)) : 0u;
+            page = real ? static_cast<uint32_t>(table[column]) : 0u;
             inside = key - column * p.c.page_size;
           };
           if (mapped) locate(w.b0);

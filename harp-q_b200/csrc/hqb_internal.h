@@ -43,7 +43,10 @@ inline cudaError_t allow_dynamic_smem(DeviceOnce& done, const void* kernel, uint
 
 // Launches a kernel as a programmatic dependent of the one before it in the stream: its CTAs may
 // start while that one ends.  Only for kernels that run griddepcontrol.wait before their first
-// access to global memory (in at least one thread of a grid that would otherwise end early).
+// access to global memory (in at least one thread of a grid that would otherwise end early), and that
+// read by plain loads: the read-only path (__ldg) is for data that nobody writes while the kernel
+// runs, and its loads may move above the wait; the kernel before may still be writing when this one
+// starts.
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t smem, uint32_t cluster,
                              cudaStream_t st, const A&... args) {

@@ -88,7 +88,7 @@ __device__ __forceinline__ void peer_store(uint32_t a, float v) {
 }
 
 __device__ __forceinline__ uint32_t group_of(const LoraParams& p, uint32_t token, uint32_t& bad) {
-  const int32_t id = __ldg(p.ids + token);
+  const int32_t id = p.ids[token];
   if (id < 0) return p.s.adapters;
   if (static_cast<uint32_t>(id) >= p.s.adapters) {
     bad |= HQB_DEVERR_INDEX;
@@ -97,10 +97,11 @@ __device__ __forceinline__ uint32_t group_of(const LoraParams& p, uint32_t token
   return static_cast<uint32_t>(id);
 }
 
-// Eight consecutive 16-bit elements at `src`, of which `real` exist (zeros after them).
+// Eight consecutive 16-bit elements at `src`, of which `real` exist (zeros after them).  From L2: every
+// element is read once (777 tokens of rank 24 16.7 us through L1, 15.5 us so).
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const void* src, int64_t real) {
-  if (VEC) return real > 0 ? __ldg(static_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+  if (VEC) return real > 0 ? __ldcg(static_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
   const uint16_t* s = static_cast<const uint16_t*>(src);
   uint32_t w[4];
 #pragma unroll
@@ -518,9 +519,9 @@ __device__ __forceinline__ bool find_tile(const LoraParams& p, uint32_t tile, in
 __device__ __forceinline__ uint32_t adapter(const LoraParams& p, uint32_t group, float& scale, uint32_t& bad) {
   scale = 0.0f;
   if (group >= p.s.adapters) return 0;
-  const int32_t v = p.s.ranks != nullptr ? __ldg(p.s.ranks + group) : static_cast<int32_t>(p.s.max_rank);
+  const int32_t v = p.s.ranks != nullptr ? p.s.ranks[group] : static_cast<int32_t>(p.s.max_rank);
   if (v < 0 || v > static_cast<int32_t>(p.s.max_rank)) bad |= HQB_DEVERR_INDEX;
-  scale = p.s.scales != nullptr ? __ldg(p.s.scales + group) : 1.0f;
+  scale = p.s.scales != nullptr ? p.s.scales[group] : 1.0f;
   return v < 0 ? 0u : min(static_cast<uint32_t>(v), p.s.max_rank);
 }
 
@@ -943,7 +944,7 @@ __global__ void __launch_bounds__(256) lora_lay_kernel(const __grid_constant__ L
     const uint16_t* src = static_cast<const uint16_t*>(p.s.b) + row * p.s.max_rank;
     uint16_t v[8];
 #pragma unroll
-    for (uint32_t k = 0; k < 8; ++k) v[k] = r + k < p.s.max_rank ? __ldg(src + r + k) : 0;
+    for (uint32_t k = 0; k < 8; ++k) v[k] = r + k < p.s.max_rank ? src[r + k] : 0;
     static_cast<uint4*>(p.laid)[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
   }
 }

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
             bad |= HQB_DEVERR_INDEX;
             break;
           }
-          const int32_t up = __ldg(parent + at);
+          const int32_t up = parent[at];
           if (up < -1 || up >= static_cast<int32_t>(at)) bad |= HQB_DEVERR_INDEX;
           if (up < 0 || up >= static_cast<int32_t>(at)) break;  // a root; parents come strictly earlier
           at = static_cast<uint32_t>(up);

@@ -170,3 +170,12 @@ def test_the_default_stream_is_never_captured():
     number = ctypes.c_uint64(7)
     assert hqb.lib().hqb_stream_capture(None, ctypes.byref(number)) == 0 and number.value == 0
     assert hqb.lib().hqb_stream_capture(None, None) == INVALID
+
+
+@pytest.mark.parametrize("name", ["hqb_page.cu", "hqb_attention.cuh", "hqb_attention.cu", "hqb_attention_tmem.cu", "hqb_lora.cu",
+                                  "hqb_serve.cuh"])
+def test_programmatic_dependents_read_by_plain_loads(name):
+    """These kernels start while the one before them may still write their inputs: the read-only path is
+    for data that does not change while a kernel runs, and its loads may move above the wait."""
+    source = (hqb.PKG / "csrc" / name).read_text()
+    assert "__ldg" not in source and "ld.global.nc" not in source
