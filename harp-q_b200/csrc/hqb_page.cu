@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
       if (a.token_request != nullptr) a.token_request[t] = static_cast<int32_t>(rr);
       uint32_t depth = node;
       if (a.parents != nullptr) {
-        const uint32_t given = a.parent_count > s_start[lo] ? a.parent_count - s_start[lo] : 0u;  // of this request
+        const bool given = t < a.parent_count;  // then its ancestors are too
+        if (!given) bad |= HQB_DEVERR_INDEX;
         const int32_t* parent = a.parents + s_start[lo];
         uint32_t words[kPlanWords];
 #pragma unroll
@@ -135,10 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
           if (a.mask != nullptr && (at >> 5) >= a.mask_words) bad |= HQB_DEVERR_INDEX;
 #pragma unroll
           for (uint32_t w = 0; w < kPlanWords; ++w) words[w] |= w == (at >> 5) ? 1u << (at & 31) : 0u;
-          if (at >= given) {
-            bad |= HQB_DEVERR_INDEX;
-            break;
-          }
+          if (!given) break;
           const int32_t up = parent[at];
           if (up < -1 || up >= static_cast<int32_t>(at)) bad |= HQB_DEVERR_INDEX;
           if (up < 0 || up >= static_cast<int32_t>(at)) break;  // a root; parents come strictly earlier
