@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   volatile uint32_t* abort = &bars.abort;
   const uint32_t tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   uint32_t bad = 0;
-  griddep_launch_dependents();
   if ((smem_u32(sm) & 1023u) != 0) {  // the swizzle goes by address bits
+    griddep_wait();
     if (tid == 0) atomicOr(p.error, HQB_DEVERR_LAUNCH);
     return;
   }
@@ -130,6 +130,9 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(bars.tmem);
+  // only now: a dependent that shared the SM and took tensor memory first would wait for this grid,
+  // and this CTA for it
+  griddep_launch_dependents();
   griddep_wait();
   // a wait that runs out ends every role's loop; nothing is left in flight but this CTA's copies
   // (for a whole warp, whose lanes must go on or stop together)

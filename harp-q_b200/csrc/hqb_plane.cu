@@ -1848,7 +1848,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) gemv_tc_kernel(const __grid_con
   volatile uint32_t* abort = misc + 1;
   const uint64_t total = p.total;
   const uint32_t ctas = static_cast<uint32_t>(total < gridDim.x ? total : gridDim.x), cta = blockIdx.x;
-  griddep_launch_dependents();
   if (cta >= ctas) return;
   const uint64_t u0 = unit_start(cta, total, ctas), u1 = unit_start(cta + 1, total, ctas);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1883,6 +1882,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) gemv_tc_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = misc[0];
+  griddep_launch_dependents();  // only now: a dependent must not take this CTA's tensor memory and then wait for it
   SplitRows split{0u, 0u, 0u};
 
   if (warp == 8) {

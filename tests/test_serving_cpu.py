@@ -179,3 +179,15 @@ def test_programmatic_dependents_read_by_plain_loads(name):
     for data that does not change while a kernel runs, and its loads may move above the wait."""
     source = (hqb.PKG / "csrc" / name).read_text()
     assert "__ldg" not in source and "ld.global.nc" not in source
+
+
+def test_dependents_start_after_tensor_memory_is_taken():
+    """A programmatic dependent that shares an SM and takes tensor memory before its predecessor's CTA has
+    would wait for that CTA, which waits for the memory."""
+    found = 0
+    for path in sorted((hqb.PKG / "csrc").glob("*.cu")):
+        for kernel in path.read_text().split("__global__")[1:]:
+            if "tmem_alloc(" in kernel:
+                found += 1
+                assert kernel.index("tmem_alloc(") < kernel.index("griddep_launch_dependents("), path.name
+    assert found == 2
