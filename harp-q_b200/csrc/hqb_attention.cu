@@ -19,9 +19,9 @@ constexpr uint32_t kChunk = 16;  // keys a warp takes at once
 template <int DP, int kRowsWarps, int kStages>
 constexpr uint32_t kRowsSmem = kRowsWarps * kStages * 2 * kChunk * DP * 2;
 
-// Mathematics: the softmax over the keys in one pass.  A warp keeps, per row, the running
-// maximum m of t = scale*log2(e) * q.k, the sum l of 2^(t - m) and the sums O of 2^(t - m) v;
-// a larger maximum m' rescales l and O by 2^(m - m').  Warps, and CTAs, that saw different keys
+// Mathematics: the softmax over the keys in one pass.  A warp keeps, per row, a reference m (the
+// running maximum of t = scale*log2(e) * q.k, less kWeightShift), the sum l of 2^(t - m) and the sums O
+// of 2^(t - m) v; a larger reference m' rescales l and O by 2^(m - m').  Warps, and CTAs, that saw different keys
 // are joined the same way.
 // Split: the warps of a CTA take the segment's 16-key chunks in turn, each with its own
 // ring of asynchronous copies, so the loop has no CTA barrier and keeps 2 chunks (16 KB at 128
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarp
       for (int e = 0; e < 2; ++e) {
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-        const float next = fmaxf(m[e], top[e]);
+        const float next = fmaxf(m[e], top[e] - kWeightShift<T>);
         grew |= next != m[e];
         use[e] = next == -INFINITY ? 0.0f : next;
         factor[e] = fast_exp2(m[e] - use[e]);

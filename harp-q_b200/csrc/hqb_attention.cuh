@@ -30,6 +30,19 @@ struct Divisor {
 
 struct Split;
 
+// The softmax's reference for the exponent lies kWeightShift below the maximum, so that the weights reach
+// up to 2^15 in FP16.  They are rounded to the type for the product with the values, and FP16 ends at
+// 2^-24: weights up to 1 would lose what is below 2^-25 of the largest, from the product alone, and keys of
+// that size that are many would be missing from the result.  So they keep all their bits down to 2^-27
+// of the largest, and end at 2^-38.  BF16 has FP32's range.
+template <typename T>
+constexpr bool kNarrow = Elem<T>::kExpMask == 0x7C00u;
+// log2 of how far the tensor-memory kernel lets the maximum outgrow its reference before it rescales sums
+template <typename T>
+constexpr float kSlack = kNarrow<T> ? 2.0f : 8.0f;
+template <typename T>
+constexpr float kWeightShift = kNarrow<T> ? 13.0f : 0.0f;
+
 struct AttnParams {
   hqb_attention_args a;
   hqb_paged_cache c;

@@ -17,7 +17,6 @@ constexpr uint32_t kCopyWarp = 9;    // plain copies, and the values' last rows
 constexpr uint32_t kMmaWarp = 10;
 constexpr uint32_t kValuesWarp = 11; // tensor-map copies of values
 constexpr uint32_t kTmemThreads = 384;  // warps 0-7 softmax
-constexpr float kSlack = 8.0f;       // log2 of how far the maximum may grow before sums are rescaled
 
 // One segment as the MMA and softmax warps see it, written by the loading warp.
 struct Segment {
@@ -58,9 +57,9 @@ struct Maps {
 };
 
 // Mathematics: the one-pass softmax of attention_rows_kernel.  A running reference m stands in
-// for the maximum: it follows the maximum only when that has grown by more than 8 in the
-// exponent, so weights stay below 2^8 and the sums in tensor memory are rarely rescaled; the
-// result is the same sum up to rounding.
+// for the maximum: it follows the maximum (less kWeightShift) only when that has grown by more than
+// kSlack in the exponent, so weights stay within the type and the sums in tensor memory are rarely
+// rescaled; the result is the same sum up to rounding.
 // Roles: 4 + 4 warps take the scores of two streams out of tensor memory (a thread a row: no
 // shuffles), turn them into weights and put those back, packed in 16 bits over the scores, as
 // the A operand of weights x values; a warp brings keys and queries, another one values, into
@@ -592,8 +591,8 @@ __global__ void __launch_bounds__(kTmemThreads, 1) attention_tmem_kernel(const _
               for (int k = 0; k < 4; ++k) t4[k] = fmaxf(t4[k], fmaxf(__uint_as_float(va[e + k]), __uint_as_float(vb[e + k])));
             top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
           }
-          const float tops = top * c;
-          const bool grow = tops > m + kSlack || (m == -INFINITY && tops > m);
+          const float tops = fmaf(top, c, -kWeightShift<T>);
+          const bool grow = tops > m + kSlack<T> || (m == -INFINITY && tops > m);
           if (ballot(grow) != 0) {
             const float next = grow ? tops : m;
             const float f = grow ? fast_exp2(m - next) : 1.0f;

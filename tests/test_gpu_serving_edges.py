@@ -3,13 +3,15 @@ test_gpu_serving.py (whose tolerances hold here too)."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import harpq_b200 as hqb  # noqa: E402
-from test_gpu_serving import BF16, F16, ints, make_attention, make_lora, plan_reference  # noqa: E402
+from test_gpu_serving import BF16, F16, U, ints, make_attention, make_lora, plan_reference  # noqa: E402
 
 
 # ---- page plan ----------------------------------------------------------------------------
@@ -132,3 +134,33 @@ def test_attention_reports_bad_lengths_where_nothing_is_left_to_do(hq, max_conte
     attend = hqb.TreeAttention(hqb.PagedCache(s["kc"], s["vc"]), hq, 2, 4, 2, max_context)
     attend(s["q"], s["k"], s["v"], s["tables"][:len(ctx)].contiguous(), ints(ctx), ints(starts), s["mask"])
     assert attend.ws.error_flags() == hqb.DEVERR_INDEX
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("group,heads,keys,gap", [
+    (1, 1, 60000, 18.25), (32, 1, 60000, 18.25), (1, 1, 400, 14.0), (24, 1, 400, 14.0), (32, 1, 3000, 12.5),
+    # more heads than CTAs: one of them sees nearly all keys of a head
+    (1, 296, 8000, 18.25), (24, 148, 8000, 18.25)])
+def test_attention_many_small_weights(kind, group, heads, keys, gap):
+    """One key far above very many others, whose values make up the result: weights w of 2^-18 to 2^-26.3
+    of the largest.  A weight is rounded by at most u w, or by 2^-25 of FP16's weights up to 2^13 for the
+    largest key (2^-38 of that one); scores here are exact, the exponential within 2^-20."""
+    hq = group * heads
+    q = torch.zeros(1, hq, 64, dtype=kind, device="cuda")
+    q[..., 0] = 1
+    k, v = (torch.zeros(-(-keys // 16), 16, heads, 64, dtype=kind, device="cuda") for _ in range(2))
+    k[keys // 16 // 2, 3, :, 0] = gap
+    v[:] = 1000
+    v[keys // 16 // 2, 3] = 0
+    own = torch.zeros(1, heads, 64, dtype=kind, device="cuda")
+    own[..., 0] = -60000.0  # the step's own key counts for nothing
+    attend = hqb.TreeAttention(hqb.PagedCache(k, v), hq, 1, 1, 1, keys)
+    lse = torch.empty(1, hq, device="cuda")
+    out = attend(q, own, own, ints([list(range(len(k)))]), ints([keys]), ints([0, 1]), scale=1.0, lse=lse)
+    small = (keys - 1) * math.exp(-gap)
+    want = 1000 * small / (1 + small)
+    tol = (2 * U[kind] + 2.0 ** -19) * want + 2.0 ** -38 * (keys - 1) * 1000 / (1 + small)
+    err = (out.double() - want).abs().max().item()
+    assert err <= tol, f"{err:.3e} over {tol:.3e} at {want:.3e}"
+    assert (lse.double() - gap - math.log1p(small)).abs().max().item() <= 2.0 ** -20 * gap + 2.0 ** -20
+    assert attend.ws.error_flags() == 0
