@@ -675,6 +675,18 @@ class StreamWorkspaces:
             ws = self.eager[stream] = self._make(size, stream, ws)
         return ws
 
+    def error_flags(self, reset: bool = False) -> int:
+        """The HQB_DEVERR_* bits of the calls so far, all streams', and of the newest captures' last
+        replays; waits for the device."""
+        bits = 0
+        with torch.cuda.device(self.device):
+            torch.cuda.synchronize()
+            for stream, ws in [*self.eager.items(), *((s, ws) for s, (_, ws) in self.captured.items())]:
+                bits |= ws.error_flags(stream)
+                if reset:
+                    check(lib().hqb_workspace_init(ws.ptr(), 256, stream), "hqb_workspace_init")
+        return bits
+
     def _make(self, size: int, stream: int, smaller: Workspace | None) -> Workspace:
         size = 1 << (size - 1).bit_length()
         # on the stream that uses it: the allocator then reuses it in that order
@@ -911,6 +923,10 @@ class LoraSet:
 
     def workspace_bytes(self, tokens: int) -> int:
         return lib().hqb_lora_workspace_bytes(self._at, tokens, self._index)
+
+    def error_flags(self, reset: bool = False) -> int:
+        """HQB_DEVERR_* bits of the set's calls that brought no workspace (see StreamWorkspaces)."""
+        return self._workspaces.error_flags(reset)
 
     def workspace(self, tokens: int, stream: int) -> Workspace:
         """The stream's workspace, or under capture the capture's, grown to what `tokens` tokens need."""

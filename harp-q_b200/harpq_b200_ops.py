@@ -99,7 +99,7 @@ def _gemv_fake(x, planes, rows, cols, prefix, bias=None, out_dtype=torch.float16
 #
 # The same calls and the same bits as PagedCache.append, TreeAttention and LoraSet.apply, whose
 # arguments they share, without a handle to keep.  Workspaces are kept per stream and capture
-# (harpq_b200.StreamWorkspaces).
+# (harpq_b200.StreamWorkspaces); serving_errors() reads what their calls reported.
 
 _SERVING_WORKSPACES: dict = {}
 
@@ -109,6 +109,15 @@ def _serving_workspace(kind: str, device: torch.device, stream: int, need: int) 
     if key not in _SERVING_WORKSPACES:
         _SERVING_WORKSPACES[key] = hqb.StreamWorkspaces(device, lambda size: size)
     return _SERVING_WORKSPACES[key].take(need, stream)
+
+
+def serving_errors(device: Optional[torch.device] = None, reset: bool = False) -> dict:
+    """HQB_DEVERR_* bits of the serving operators' calls on a device (None: the current one), by operator;
+    waits for the device."""
+    index = torch.cuda.current_device() if device is None else hqb._device_index(torch.device(device))
+    kinds = {"cache": "cache_append", "attention": "tree_attention", "lora": "lora"}
+    return {name: ws.error_flags(reset) if (ws := _SERVING_WORKSPACES.get((kind, index))) is not None else 0
+            for kind, name in kinds.items()}
 
 
 def _serving_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, stream: int) -> "hqb.PagedCache":

@@ -164,3 +164,44 @@ def test_attention_many_small_weights(kind, group, heads, keys, gap):
     assert err <= tol, f"{err:.3e} over {tol:.3e} at {want:.3e}"
     assert (lse.double() - gap - math.log1p(small)).abs().max().item() <= 2.0 ** -20 * gap + 2.0 ** -20
     assert attend.ws.error_flags() == 0
+
+
+# ---- errors that calls without a workspace report -------------------------------------------------
+
+
+def test_errors_of_implicit_workspaces_can_be_read():
+    import harpq_b200_ops
+
+    ops, clear = torch.ops.harpq_b200, {"cache_append": 0, "tree_attention": 0, "lora": 0}
+    harpq_b200_ops.serving_errors(reset=True)
+    x, a, b, ranks, scales, ids, base = make_lora(7, 400, 256, 64, 2, 16, F16, F16, full=True)
+    s = hqb.LoraSet(a, b, ranks, scales)
+    s.apply(x, ids, base=base)
+    ops.lora(x, a, b, ids, ranks, scales, base)
+    assert s.error_flags() == 0 and harpq_b200_ops.serving_errors() == clear
+    ids[4] = 9
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        s.apply(x, ids, base=base)
+        ops.lora(x, a, b, ids, ranks, scales, base)
+    assert s.error_flags(reset=True) == hqb.DEVERR_INDEX and s.error_flags() == 0
+    assert harpq_b200_ops.serving_errors("cuda:0", reset=True) == {**clear, "lora": hqb.DEVERR_INDEX}
+    t = make_attention(12, [40, 40], [2, 2], 4, 1, 64, 16, F16)
+    ops.cache_append(t["kc"], t["vc"], t["k"], t["v"], ints([3, 10 ** 6, 4, 5]))
+    ops.tree_attention(t["q"], t["k"], t["v"], t["kc"], t["vc"], t["tables"], ints([-1, 40]), ints([0, 2, 4]), t["mask"], 2, 40)
+    assert harpq_b200_ops.serving_errors(reset=True) == {"cache_append": hqb.DEVERR_PAGES, "tree_attention": hqb.DEVERR_INDEX, "lora": 0}
+    assert harpq_b200_ops.serving_errors() == clear
+
+
+def test_errors_of_a_replay_can_be_read():
+    x, a, b, ranks, scales, ids, base = make_lora(7, 40, 256, 64, 2, 16, F16, F16, full=True)
+    s = hqb.LoraSet(a, b, ranks, scales)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.apply(x, ids, base=base)
+    ids[4] = 9
+    graph.replay()
+    assert s.error_flags() == hqb.DEVERR_INDEX
+    ids[4] = 0
+    graph.replay()  # clears the word first
+    assert s.error_flags() == 0
