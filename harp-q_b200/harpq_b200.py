@@ -700,9 +700,11 @@ class StreamWorkspaces:
 
 class PagePlan:
     """One decode step's lengths as addresses (hqb_page_plan), in buffers that are kept between
-    steps: starts [requests + 1], requests, positions and slots [tokens] (entries past the
-    step's last token are -1), held [requests], free_head [1], mask [tokens, words] (with
-    max_new > 0: trees of up to that many nodes) and flags [1] (HQB_DEVERR_* bits, OR-ed)."""
+    steps: starts [requests + 1], requests and positions [tokens] (entries past the step's last
+    token are -1) and flags [1] (HQB_DEVERR_* bits, OR-ed); of a build with tables also slots
+    [tokens], held [requests] and free_head [1], of a build with parents mask [tokens, words] (with
+    max_new > 0: trees of up to that many nodes).  These four are None after a build that left them
+    out; before the first one they are the buffers."""
 
     def __init__(self, requests: int, tokens: int, page_size: int, num_pages: int, max_new: int = 0, device=None):
         if requests < 1 or tokens < 1 or page_size < 1 or num_pages < 1:
@@ -714,8 +716,9 @@ class PagePlan:
         # one buffer, so that a step's metadata is one copy where it is wanted on the host
         sizes = [requests + 1, tokens, tokens, tokens, requests, 1, 1, tokens * self.words]
         parts = torch.zeros(sum(sizes), dtype=torch.int32, device=device or "cuda").split(sizes)
-        self.starts, self.requests, self.positions, self.slots, self.held, self.free_head, self.flags, mask = parts
-        self.mask = mask.view(tokens, self.words) if self.words else None
+        self.starts, self.requests, self.positions, self._slots, self._held, self._free_head, self.flags, mask = parts
+        self._mask = mask.view(tokens, self.words) if self.words else None
+        self._paged = self._tree = True
         _on_gpu("a plan's buffers", self.starts)
         self.device = self.starts.device
         self._index = _device_index(self.device)
@@ -740,7 +743,24 @@ class PagePlan:
             if status == _UNFIT:
                 self._refuse(context_lens, new_lens, held, tables, free_pages, free_head, parents)
             check(status, "hqb_page_plan")
+        self._paged, self._tree = tables is not None, parents is not None
         return self
+
+    @property
+    def slots(self) -> torch.Tensor | None:
+        return self._slots if self._paged else None
+
+    @property
+    def held(self) -> torch.Tensor | None:
+        return self._held if self._paged else None
+
+    @property
+    def free_head(self) -> torch.Tensor | None:
+        return self._free_head if self._paged else None
+
+    @property
+    def mask(self) -> torch.Tensor | None:
+        return self._mask if self._tree else None
 
     def _refuse(self, context_lens, new_lens, held, tables, free_pages, free_head, parents) -> None:
         n, device = self.batch, self._index

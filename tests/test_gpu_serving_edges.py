@@ -39,6 +39,20 @@ def test_plan_of_no_tokens_takes_no_parents():
     assert plan.starts.tolist() == [0, 0, 0] and plan.positions.tolist() == [-1] * 3 and plan.flags.item() == 0
 
 
+def test_plan_gives_no_outputs_of_an_earlier_build():
+    """A tree's mask would hide a later chain's nodes; slots of an earlier step would be written again."""
+    plan = hqb.PagePlan(1, 4, 16, 8, max_new=4)
+    assert plan.slots is not None and plan.mask is not None
+    paged = dict(held=ints([1]), tables=ints([[3, -1]]), free_pages=ints([5, 6]), free_head=ints([0]))
+    plan.build(ints([14]), ints([4]), parents=ints([-1, 0, 0, 1]), **paged)
+    assert plan.slots.tolist() == [62, 63, 80, 81] and plan.held.tolist() == [2] and plan.free_head.tolist() == [1]
+    assert plan.mask.flatten().tolist() == [1, 3, 5, 11]
+    plan.build(ints([14]), ints([4]), parents=ints([-1, 0, 0, 1]))
+    assert plan.slots is None and plan.held is None and plan.free_head is None and plan.mask is not None
+    plan.build(ints([14]), ints([4]), **paged)
+    assert plan.slots is not None and plan.mask is None
+
+
 # ---- memory that callers bring --------------------------------------------------------------
 
 
