@@ -143,7 +143,10 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
                    tables: torch.Tensor, context_lens: torch.Tensor, starts: torch.Tensor,
                    mask: Optional[torch.Tensor], max_new: int, max_context: int,
                    scale: Optional[float] = None) -> torch.Tensor:
-    """Attention of each request's drafted nodes over its cached context and the nodes its mask shows."""
+    """Attention of each request's drafted nodes over its cached context and the nodes its mask shows
+    (rows of no request are not written)."""
+    if q.shape[0] == 0:
+        return q.new_empty(q.shape)
     stream = torch.cuda.current_stream(q.device).cuda_stream
     attend = hqb.TreeAttention(_serving_cache(k_cache, v_cache, stream), q.shape[1], context_lens.numel(), q.shape[0], max_new,
                                max_context, workspace=lambda need: _serving_workspace("attention", q.device, stream, need))

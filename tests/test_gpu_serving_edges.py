@@ -180,6 +180,20 @@ def test_attention_many_small_weights(kind, group, heads, keys, gap):
     assert attend.ws.error_flags() == 0
 
 
+def test_operators_take_steps_without_tokens():
+    ops = torch.ops.harpq_b200
+    import harpq_b200_ops  # noqa: F401
+
+    s = make_attention(12, [40], [2], 4, 2, 64, 16, F16)
+    x, a, b, ranks, scales, ids, base = make_lora(7, 4, 64, 32, 2, 8, F16, F16)
+    before = s["kc"].clone()
+    ops.cache_append(s["kc"], s["vc"], s["k"][:0], s["v"][:0], ints([]))
+    assert torch.equal(s["kc"], before)
+    out = ops.tree_attention(s["q"][:0], s["k"][:0], s["v"][:0], s["kc"], s["vc"], s["tables"], ints([40]), ints([0, 0]), None, 2, 40)
+    assert out.shape == (0, 4, 64) and out.dtype == F16
+    assert ops.lora(x[:0], a, b, ids[:0], ranks, scales, base[:0]).shape == (0, 32)
+
+
 # ---- errors that calls without a workspace report -------------------------------------------------
 
 
