@@ -7,6 +7,7 @@
 // method then says which.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -42,6 +43,9 @@ bool heads(PyObject* o, int64_t rows, int64_t heads, int64_t dim, int type, int 
          (*t)->size(2) == dim && (type < 0 || code((*t)->scalar_type()) == type) && (*t)->is_cuda() &&
          (*t)->get_device() == device && (dim == 1 || (*t)->stride(2) == 1);
 }
+
+// Whether each element of a result has a place of its own.
+bool distinct(const Tensor& t) { return at::has_internal_overlap(t) != at::MemOverlap::Yes; }
 
 // The current stream of the device, or the one given as a number.
 void* stream_of(PyObject* o, int device) {
@@ -145,7 +149,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t tokens = q->size(0), requests = ctx->numel();
   if (tokens > p.tokens || requests > p.requests || !heads(a[7], tokens, c->kv_heads, c->head_dim, c->dtype, device, &k) ||
       !heads(a[8], tokens, c->kv_heads, c->head_dim, c->dtype, device, &v) || k->strides() != v->strides() ||
-      !heads(a[14], tokens, p.q_heads, c->head_dim, c->dtype, device, &out) || table->dim() != 2 || table->size(0) != requests ||
+      !heads(a[14], tokens, p.q_heads, c->head_dim, c->dtype, device, &out) || !distinct(*out) || table->dim() != 2 || table->size(0) != requests ||
       !ints(a[9], table->numel(), device, false, &p.tables) || !ints(a[10], requests, device, false, &p.context_lens) ||
       !ints(a[11], requests + 1, device, false, &p.starts))
     return status(kUnfit);
@@ -213,6 +217,9 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t tokens = x->size(0);
   if (!ints(a[6], tokens, device, false, &ids) || !rows_of(a[8], tokens, static_cast<int64_t>(s->rows), kind, device, &out, &out_stride) ||
       (a[7] != Py_None && !rows_of(a[7], tokens, static_cast<int64_t>(s->rows), kind, device, &base, &base_stride)))
+    return status(kUnfit);
+  // base is read ahead of the stores: it is out itself, or elsewhere
+  if (base != nullptr && base->data_ptr() != out->data_ptr() && at::get_overlap_status(*base, *out) == at::MemOverlapStatus::Partial)
     return status(kUnfit);
   return status(hqb_lora(s, x->const_data_ptr(), x_stride, ids, static_cast<uint32_t>(tokens),
                          base == nullptr ? nullptr : base->const_data_ptr(), base_stride, out->data_ptr(), kind, out_stride,

@@ -891,6 +891,8 @@ class TreeAttention:
                 raise ValueError(f"{name}: a head's elements must be adjacent")
         if k.stride() != v.stride():
             raise ValueError("k and v must share strides")
+        if any(n > 1 and step == 0 for n, step in zip(out.shape, out.stride())):
+            raise ValueError("out: elements must not share their place (an expanded tensor)")
         if requests > self.requests or tokens > self.tokens:
             raise ValueError(f"built for {self.requests} requests and {self.tokens} tokens, got {requests} and {tokens}")
         _table("tables", tables, requests, c._index)
@@ -983,6 +985,7 @@ class LoraSet:
             if (t.stride(1) != 1 and cols > 1) or (t.stride(0) < cols and tokens > 1):
                 raise ValueError(f"{name}: a row's elements must be adjacent, and rows must not overlap")
         _ints("ids", ids, tokens, self._index)
+        raise ValueError("base must be out itself or not overlap it")
 
 
 # ---- output-row sharding across ranks --------------------------------------------------

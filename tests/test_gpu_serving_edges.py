@@ -233,3 +233,24 @@ def test_errors_of_a_replay_can_be_read():
     ids[4] = 0
     graph.replay()  # clears the word first
     assert s.error_flags() == 0
+
+
+# ---- refusals ------------------------------------------------------------------------------------
+
+
+def test_results_that_overlap_are_refused():
+    s = make_attention(12, [40], [3], 4, 2, 64, 16, F16)
+    attend = hqb.TreeAttention(hqb.PagedCache(s["kc"], s["vc"]), 4, 1, 3, 3, 40)
+    args = (s["q"], s["k"], s["v"], s["tables"], ints([40]), ints([0, 3]), s["mask"])
+    for out in (torch.empty(1, 4, 64, dtype=F16, device="cuda").expand(3, 4, 64),
+                torch.empty(3, 1, 64, dtype=F16, device="cuda").expand(3, 4, 64)):
+        with pytest.raises(ValueError, match="share their place"):
+            attend(*args, out=out)
+    attend(*args, out=torch.empty(4, 3, 64, dtype=F16, device="cuda").transpose(0, 1))
+    x, a, b, ranks, scales, ids, base = make_lora(7, 4, 64, 32, 2, 8, F16, F16)
+    store = torch.zeros(6, 32, dtype=F16, device="cuda")
+    lora = hqb.LoraSet(a, b, ranks, scales)
+    with pytest.raises(ValueError, match="overlap"):
+        lora.apply(x, ids, base=store[:4], out=store[1:5])
+    lora.apply(x, ids, base=store[:4], out=store[:4])
+    lora.apply(x[:2], ids[:2], base=store[:2], out=store[2:4])
