@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import harpq_b200 as hqb  # noqa: E402
-from test_gpu_serving import BF16, F16, U, ints, make_attention, make_lora, plan_reference  # noqa: E402
+from test_gpu_serving import BF16, F16, F32, U, check_attention, ints, lora_reference, make_attention, make_lora, plan_reference  # noqa: E402
 
 
 # ---- page plan ----------------------------------------------------------------------------
@@ -178,6 +178,103 @@ def test_attention_many_small_weights(kind, group, heads, keys, gap):
     assert err <= tol, f"{err:.3e} over {tol:.3e} at {want:.3e}"
     assert (lse.double() - gap - math.log1p(small)).abs().max().item() <= 2.0 ** -20 * gap + 2.0 ** -20
     assert attend.ws.error_flags() == 0
+
+
+@pytest.mark.parametrize("requests", [33, 64, 100])
+@pytest.mark.parametrize("hq,hk,dim", [(2, 2, 64), (8, 2, 128), (40, 2, 64)])
+@pytest.mark.parametrize("most", [60, 700])
+def test_attention_of_many_requests(requests, hq, hk, dim, most):
+    """More requests than one round of 32 lengths, some without tokens where two rounds meet."""
+    ctx = [(r * 97 + 13) % most for r in range(requests)]
+    new = [1 + r % 3 for r in range(requests)]
+    for r in (0, 31, 32, 63, 64, 65, requests - 1):
+        if r < requests:
+            new[r] = 0
+    ctx[5], ctx[31] = most, most * 2
+    check_attention(make_attention(requests, ctx, new, hq, hk, dim, 16, F16))
+
+
+def test_attention_of_many_requests_without_tokens():
+    """Whole rounds of requests without tokens before and behind the one that has some."""
+    new = [0] * 70 + [5] + [0] * 60
+    for hq in (2, 16):
+        check_attention(make_attention(1, [3 * r for r in range(131)], new, hq, 1, 64, 16, BF16))
+
+
+@pytest.mark.parametrize("page", [64, 4])
+@pytest.mark.parametrize("group", [1, 32])
+def test_attention_past_32_bits(group, page):
+    """Pages beyond 2^32 elements, and rows of q, k, v and out beyond 2^31, by each kernel and kind of copy."""
+    heads, dim = 4, 128
+    pages = 2 ** 32 // (page * heads * dim) + 40
+    store = torch.empty(pages, page, heads, dim, dtype=BF16, device="cuda")
+    last = torch.arange(pages - 40, pages, dtype=torch.int32, device="cuda")
+    store[-40:] = torch.randn(40, page, heads, dim, device="cuda").to(BF16)
+    keys, far = 40 * page - 3, 2 ** 31 + 64
+    q, k, v = (torch.randn(2, n, dim, device="cuda").to(BF16) for n in (heads * group, heads, heads))
+    near = store[-40:].clone()
+    args = ints([keys, keys - 2]), ints([0, 1, 2])
+    want = hqb.TreeAttention(hqb.PagedCache(near, near), heads * group, 2, 2, 1, 4000)(
+        q, k, v, (last - (pages - 40)).expand(2, -1).contiguous(), *args)
+    wide = []
+    for t in (q, k, v, want):
+        wide.append(torch.empty(far + t[0].numel(), dtype=BF16, device="cuda").as_strided(t.shape, (far, dim, 1)))
+        wide[-1].copy_(t)
+    wide[3].zero_()
+    attend = hqb.TreeAttention(hqb.PagedCache(store, store), heads * group, 2, 2, 1, 4000)
+    attend(*wide[:3], last.expand(2, -1).contiguous(), *args, out=wide[3])
+    assert torch.equal(wide[3], want) and attend.ws.error_flags() == 0
+
+
+@pytest.mark.parametrize("tokens,far", [(2, 2 ** 31 + 64), (600, 2 ** 23 + 64)])
+def test_lora_rows_past_32_bits(tokens, far):
+    x, a, b, ranks, scales, ids, base = make_lora(tokens, tokens, 256, 128, 3, 64, F16, F32)
+    ids[-1] = 0
+    want, tol = lora_reference(x, a, b, ranks, scales, ids, base, F32)
+    xs = torch.empty(far * (tokens - 1) + 256, dtype=F16, device="cuda").as_strided(x.shape, (far, 1))
+    ys = torch.empty(far * (tokens - 1) + 128, dtype=F32, device="cuda").as_strided(base.shape, (far, 1))
+    xs.copy_(x), ys.copy_(base)
+    s = hqb.LoraSet(a, b, ranks, scales)
+    s.apply(xs, ids, base=ys, out=ys)
+    assert bool(((ys.double() - want).abs() <= tol).all()) and s.error_flags() == 0
+
+
+@pytest.mark.parametrize("tokens,rank,cols,rows", [
+    (3, 64, 64, 2 ** 18), (600, 64, 64, 2 ** 18), (600, 63, 64, 2 ** 18), (3, 63, 64, 2 ** 18), (3, 64, 2 ** 18, 64), (600, 64, 2 ** 18, 64)])
+def test_lora_sets_past_32_bits(tokens, rank, cols, rows):
+    """The last adapter's a or b begins beyond 2^32 elements."""
+    adapters = 2 ** 32 // (rank * max(cols, rows)) + 2
+    a = torch.empty(adapters, rank, cols, dtype=BF16, device="cuda")
+    b = torch.empty(adapters, rows, rank, dtype=BF16, device="cuda")
+    a[-1] = torch.randn(rank, cols, device="cuda") * cols ** -0.5
+    b[-1] = torch.randn(rows, rank, device="cuda") * 0.2
+    x = torch.randn(tokens, cols, device="cuda").to(BF16)
+    ids = torch.full((tokens,), adapters - 1, dtype=torch.int32, device="cuda")
+    y = hqb.LoraSet(a, b, max_tokens=0).apply(x, ids)
+    want = hqb.LoraSet(a[-1:].clone(), b[-1:].clone(), max_tokens=0).apply(x, torch.zeros_like(ids))
+    t, u = x.float() @ a[-1].float().T, U[BF16]
+    size = t.abs() @ b[-1].float().abs().T
+    # the same product, by kernels that may sum it in another order (the sizes choose them)
+    assert bool(((y.float() - want.float()).abs() <= 2 * u * want.float().abs() + 4 * u * size).all())
+    assert y.count_nonzero() > y.numel() // 2
+
+
+def test_one_workspace_serves_a_stream():
+    """Sets and attentions of several layers, one after the other on a stream, in one workspace."""
+    layers = [make_lora(n, n, 256, 128, 4, rank, F16, F32) for n, rank in ((7, 16), (900, 64), (300, 27), (40, 8))]
+    sets = [hqb.LoraSet(*t[1:5], max_tokens=0) for t in layers]
+    ws = hqb.Workspace(max(s.workspace_bytes(len(t[0])) for s, t in zip(sets, layers)))
+    want = [s.apply(t[0], t[5], base=t[6]) for s, t in zip(sets, layers)]
+    got = [s.apply(t[0], t[5], base=t[6], workspace=ws) for s, t in zip(sets, layers)]
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and ws.error_flags() == 0
+    steps = [make_attention(i, [900, 2000], [n, 3], hq, 2, 64, 16, F16) for i, (n, hq) in enumerate(((1, 2), (30, 16), (2, 4)))]
+    shared = hqb.Workspace(64 << 20)
+    outs = []
+    for own in (True, False):
+        attends = [hqb.TreeAttention(hqb.PagedCache(s["kc"], s["vc"]), s["q"].shape[1], 2, len(s["q"]), s["most"], 2000,
+                                     workspace=None if own else lambda need: shared) for s in steps]
+        outs.append([f(s["q"], s["k"], s["v"], s["tables"], ints(s["ctx"]), ints(s["starts"]), s["mask"]) for f, s in zip(attends, steps)])
+    assert all(torch.equal(x, y) for x, y in zip(*outs)) and shared.error_flags() == 0
 
 
 def test_operators_take_steps_without_tokens():

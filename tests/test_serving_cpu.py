@@ -191,3 +191,14 @@ def test_dependents_start_after_tensor_memory_is_taken():
                 found += 1
                 assert kernel.index("tmem_alloc(") < kernel.index("griddep_launch_dependents("), path.name
     assert found == 2
+
+
+@pytest.mark.parametrize("rank", [1, 5, 27, 63, 121])
+def test_lora_workspace_of_odd_ranks_never_shrinks_with_tokens(rank):
+    """The laid-out rows of b join it with the token count."""
+    for adapters in (1, 9, 40, 200, 700):
+        s = changed(a_set(), adapters=adapters, max_rank=rank, cols=8192)
+        sizes = [hqb.lib().hqb_lora_workspace_bytes(AT(s), t, 0) for t in [*range(1, 600), *range(600, 3000, 7)]]
+        assert sizes == sorted(sizes) and sizes[0] >= 256
+        pitch = -(-rank // 8) * 8
+        assert sizes[-1] >= adapters * 128 * pitch * 2  # laid out by then
