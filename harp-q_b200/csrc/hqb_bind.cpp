@@ -59,10 +59,13 @@ PyObject* status(long s) { return PyLong_FromLong(s); }
 // a launch takes the current one's.
 class OnDevice {
  public:
-  explicit OnDevice(int device) : guard_(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))) {}
+  explicit OnDevice(int device) {
+    const c10::Device d(c10::kCUDA, static_cast<c10::DeviceIndex>(device));
+    if (c10::impl::getDeviceGuardImpl(c10::kCUDA)->getDevice() != d) guard_.reset_device(d);
+  }
 
  private:
-  c10::DeviceGuard guard_;
+  c10::OptionalDeviceGuard guard_;
 };
 
 // page_plan(args address, device, stream, context_lens, new_lens, held, tables, free_pages, free_head,

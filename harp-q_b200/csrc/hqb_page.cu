@@ -132,15 +132,15 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const __grid_co
         for (uint32_t w = 0; w < kPlanWords; ++w) words[w] = 0;
         depth = 0;
         uint32_t at = node;
+        int32_t up = given ? parent[at] : -1;
         for (;;) {
           if (a.mask != nullptr && (at >> 5) >= a.mask_words) bad |= HQB_DEVERR_INDEX;
 #pragma unroll
           for (uint32_t w = 0; w < kPlanWords; ++w) words[w] |= w == (at >> 5) ? 1u << (at & 31) : 0u;
-          if (!given) break;
-          const int32_t up = parent[at];
           if (up < -1 || up >= static_cast<int32_t>(at)) bad |= HQB_DEVERR_INDEX;
           if (up < 0 || up >= static_cast<int32_t>(at)) break;  // a root; parents come strictly earlier
           at = static_cast<uint32_t>(up);
+          up = parent[at];
           ++depth;
         }
         if (a.mask != nullptr) {
