@@ -628,6 +628,15 @@ def _ints(name: str, t: torch.Tensor, n: int, device: int) -> None:
                          f"got {list(t.shape)} {t.dtype} on {t.device}")
 
 
+def _result(shape: tuple, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """A call's new result, from the memory of the stream that writes it: another stream's could still
+    be in use there."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(_raw_stream(stream), device)):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _on_gpu(name: str, t: torch.Tensor) -> None:
     """Refuses host memory: its address means nothing to a kernel."""
     if t.device.type != "cuda":
@@ -834,8 +843,9 @@ class PagedCache:
 class TreeAttention:
     """Attention of drafted trees over a paged cache (hqb_tree_attention) for steps of up to
     `requests` requests, `tokens` tokens in all, max_new nodes and about max_context cached
-    tokens a request; holds the call's workspace (or takes one: workspace(bytes) gives it), so
-    calls that overlap need one each."""
+    tokens a request; holds the call's workspace, cleared on the stream that is current here (or
+    takes one: workspace(bytes) gives it, and attentions that follow one another on a stream may
+    share it), so calls that overlap need one each."""
 
     def __init__(self, cache: PagedCache, q_heads: int, requests: int, tokens: int, max_new: int, max_context: int,
                  workspace=None):
@@ -868,10 +878,10 @@ class TreeAttention:
         first context_lens[r] cached tokens of its row of tables [requests, columns].  mask
         [tokens, words]: bit j of a node's row shows it node j of its request (None: the nodes
         up to itself).  scale None: dim ** -0.5.  lse [tokens, q_heads] FP32 gets the logarithm of
-        the sum of weights."""
+        the sum of weights.  Rows of no request are not written."""
         c = self.cache
         if out is None:
-            out = torch.empty(q.shape[0], self.q_heads, c.dim, dtype=c.dtype, device=c.device)
+            out = _result((q.shape[0], self.q_heads, c.dim), c.dtype, c.device, stream)
         status = self._call(c._at, self._at, self._ws, self._ws_bytes, c._index, _raw_stream(stream), q, k, v, tables,
                             context_lens, starts, mask, self._scale if scale is None else scale, out, lse)
         if status:
@@ -962,7 +972,7 @@ class LoraSet:
         set's or FP32.  out=base adds in place, e.g. to the output of a projection's gemv()."""
         if out is None:
             kind = y_dtype or (base.dtype if base is not None else x.dtype)
-            out = torch.empty(x.shape[0], self.rows, dtype=kind, device=self.device)
+            out = _result((x.shape[0], self.rows), kind, self.device, stream)
         s = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else _raw_stream(stream)
         ws = self._workspaces.take(x.shape[0], s) if workspace is None else _own_workspace(workspace, self._index)
         status = self._call(self._at, ws.ptr(), ws.nbytes, self._index, s, x, ids, base, out)

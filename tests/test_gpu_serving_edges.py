@@ -291,6 +291,27 @@ def test_operators_take_steps_without_tokens():
     assert ops.lora(x[:0], a, b, ids[:0], ranks, scales, base[:0]).shape == (0, 32)
 
 
+def test_new_results_come_from_the_memory_of_their_stream():
+    """A block that the current stream has just given up may still be in use there."""
+    side = torch.cuda.Stream()
+    x, a, b, ranks, scales, ids, base = make_lora(7, 9, 64, 4104, 2, 8, F16, F32)
+    t = make_attention(12, [40], [9], 36, 4, 64, 16, F16)
+    lora, attend = hqb.LoraSet(a, b, ranks, scales), hqb.TreeAttention(hqb.PagedCache(t["kc"], t["vc"]), 36, 1, 9, 9, 40)
+    args = (t["q"], t["k"], t["v"], t["tables"], ints([40]), ints([0, 9]), t["mask"])
+    torch.cuda.synchronize()
+    for call in (lambda s: lora.apply(x, ids, base=base, stream=s), lambda s: attend(*args, stream=s)):
+        want = call(None)
+        for stream in (side, side.cuda_stream):
+            out = call(stream)
+            side.synchronize()
+            assert torch.equal(out, want)
+            place, size, kind = out.data_ptr(), out.shape, out.dtype
+            del out
+            with torch.cuda.stream(side):
+                again = torch.empty(size, dtype=kind, device="cuda")
+            assert again.data_ptr() == place
+
+
 # ---- errors that calls without a workspace report -------------------------------------------------
 
 
