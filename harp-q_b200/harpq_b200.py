@@ -12,6 +12,7 @@ this module without the built library, or calling it without a CUDA device, rais
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 from pathlib import Path
@@ -628,12 +629,20 @@ def _ints(name: str, t: torch.Tensor, n: int, device: int) -> None:
                          f"got {list(t.shape)} {t.dtype} on {t.device}")
 
 
+def _on_stream(stream: int, device: torch.device):
+    """Makes a stream, by its handle, the device's current one for a while."""
+    if stream == torch.cuda.current_stream(device).cuda_stream:
+        return contextlib.nullcontext()
+    # (an ExternalStream of handle 0 would be a new stream, not the default one)
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device))
+
+
 def _result(shape: tuple, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
     """A call's new result, from the memory of the stream that writes it: another stream's could still
     be in use there."""
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(_raw_stream(stream), device)):
+    with _on_stream(_raw_stream(stream), device):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
@@ -699,7 +708,7 @@ class StreamWorkspaces:
     def _make(self, size: int, stream: int, smaller: Workspace | None) -> Workspace:
         size = 1 << (size - 1).bit_length()
         # on the stream that uses it: the allocator then reuses it in that order
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, self.device)):
+        with _on_stream(stream, self.device):
             ws = Workspace(self.bytes_of(size), self.device, clear=256)
             if smaller is not None:
                 ws.buf[:256].copy_(smaller.buf[:256])  # the error word

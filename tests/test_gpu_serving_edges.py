@@ -312,6 +312,22 @@ def test_new_results_come_from_the_memory_of_their_stream():
             assert again.data_ptr() == place
 
 
+@pytest.mark.parametrize("aside", [False, True])
+def test_default_stream_has_its_own_memory(aside):
+    """Its handle is 0, which PyTorch's wrapper of a handle takes for none."""
+    default, device = torch.cuda.default_stream(), torch.device("cuda", torch.cuda.current_device())
+    x, a, b, ranks, scales, ids, base = make_lora(7, 9, 64, 4104, 2, 8, F16, F32)
+    lora = hqb.LoraSet(a, b, ranks, scales, max_tokens=0)
+    with torch.cuda.stream(torch.cuda.Stream() if aside else default):
+        spaces = hqb.StreamWorkspaces(device, lambda size: size)
+        ws = spaces.take(1 << 24, 0)
+        out = lora.apply(x, ids, base=base, stream=default)
+    places = [(ws.ptr(), (1 << 24,), torch.uint8), (out.data_ptr(), out.shape, F32)]
+    del spaces, ws, out
+    for place, shape, kind in places:
+        assert torch.empty(shape, dtype=kind, device="cuda").data_ptr() == place
+
+
 # ---- errors that calls without a workspace report -------------------------------------------------
 
 
