@@ -957,7 +957,8 @@ class LoraSet:
                           self.max_rank, _SERVING_DTYPES[a.dtype], 0)
         self._at, self._index = ctypes.addressof(self.c), _device_index(a.device)
         self._call = bind().lora
-        self._workspaces = StreamWorkspaces(self.device, self.workspace_bytes)
+        c, index = self.c, self._index  # (not self: a cycle would keep the set's memory)
+        self._workspaces = StreamWorkspaces(self.device, lambda tokens: lib().hqb_lora_workspace_bytes(ctypes.byref(c), tokens, index))
         self._ws = self._workspaces.eager
         if max_tokens > 0:
             self.workspace(max_tokens, torch.cuda.current_stream(a.device).cuda_stream)

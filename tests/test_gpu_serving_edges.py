@@ -312,6 +312,26 @@ def test_new_results_come_from_the_memory_of_their_stream():
             assert again.data_ptr() == place
 
 
+def test_handles_are_freed_with_their_last_reference():
+    """Not by the garbage collector: they hold large workspaces."""
+    import gc
+    import weakref
+
+    x, a, b, ranks, scales, ids, base = make_lora(7, 9, 64, 32, 2, 8, F16, F32)
+    t = make_attention(12, [40], [9], 4, 2, 64, 16, F16)
+    gc.disable()
+    try:
+        cache = hqb.PagedCache(t["kc"], t["vc"])
+        for make in (lambda: hqb.LoraSet(a, b, ranks, scales), lambda: hqb.TreeAttention(cache, 4, 1, 9, 9, 40),
+                     lambda: hqb.PagePlan(1, 9, 16, 8, max_new=9)):
+            handle = make()
+            seen = weakref.ref(handle)
+            del handle
+            assert seen() is None
+    finally:
+        gc.enable()
+
+
 @pytest.mark.parametrize("aside", [False, True])
 def test_default_stream_has_its_own_memory(aside):
     """Its handle is 0, which PyTorch's wrapper of a handle takes for none."""
