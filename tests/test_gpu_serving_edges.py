@@ -53,6 +53,20 @@ def test_plan_gives_no_outputs_of_an_earlier_build():
     assert plan.slots is not None and plan.mask is None
 
 
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("hq", [1, 24])
+@pytest.mark.parametrize("above", [1.3, 2.0, 2.009, 2.02, 5.5, 5.6, 40.0])
+def test_attention_maximum_grows(kind, hq, above):
+    """A later key above all earlier ones by less and by more than what the kernels' reference may lag behind
+    (2.9 and 8 in the exponent to base 2): no weight leaves its type."""
+    s = make_attention(31, [1500, 700], [1, 1], hq, 1, 64, 16, kind)
+    s["q"].zero_(), s["kc"].zero_()
+    s["q"][..., 0] = 1
+    for r, key in ((0, 1200), (1, 600)):
+        s["kc"][s["tables"][r, key // 16], key % 16, 0, 0] = above
+    check_attention(s, scale=1.0)
+
+
 # ---- memory that callers bring --------------------------------------------------------------
 
 
