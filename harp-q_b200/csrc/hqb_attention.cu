@@ -28,7 +28,8 @@ constexpr uint32_t kRowsSmem = kRowsWarps * kStages * 2 * kChunk * DP * 2;
 // dimensions) a warp in flight; the warps are joined once per segment.  Rows: the group's heads
 // of all nodes share the keys, so a key is read once per 16 rows.
 // Warps: four, two CTAs an SM, so that one CTA's ends of segments lie under the other's copies.  Where
-// items are not cut (up to 512 keys): eight for few items, every copy then in flight at once; four
+// items are not cut (up to 512 keys): eight for few items, whose rings then hold two chunks each in flight
+// (256 keys a CTA; a third starts behind the first wait); four
 // or two for more items than SMs, with twelve warps an SM in CTAs of their own.
 // Bound by HBM at 16 rows: 32 MMAs a chunk are about 310 cycles of one of the four tensor pipes
 // a chunk against 1400 cycles an SM needs to fetch four chunks; by latency at short contexts (launch, lengths,
@@ -258,7 +259,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, kStages == 2 ? 12 / kRowsWarp
           s[n][e] = fast_exp2(s[n][e] - use[e >> 1]);
           l[e >> 1] += s[n][e];
         }
-      // weights as the A operand of weights x values: the sums above keep the unrounded weights
+      // Weights as the A operand of weights x values: the tensor cores multiply 16-bit types at full rate, and the
+      // rounding (half a unit of the type a weight, either way) is of the output's own size.  The sum of weights
+      // keeps the unrounded ones, since the log of it is an output in FP32.
       const uint32_t a0 = Elem<T>::pack(s[0][0], s[0][1]), a1 = Elem<T>::pack(s[0][2], s[0][3]);
       const uint32_t a2 = Elem<T>::pack(s[1][0], s[1][1]), a3 = Elem<T>::pack(s[1][2], s[1][3]);
       {

@@ -72,11 +72,13 @@ struct Maps {
 // while the other's weights are.
 // Tensor memory: scores 2 x 128 columns, sums 2 x DP columns.  Shared memory at DP 128: queries
 // 64 KB, rings of two blocks of keys and three of values, 32 KB each (three and two: 3 % slower).
-// Measured, B200, BF16, 64 heads over 8 of 128, 32 trees of up to 64 nodes over up to 8192 tokens: 318 us in a
-// short burst (766 TFLOP/s), 390 us in a long loop, where the card's power limit holds the clock at 1.5 GHz.
-// A block of two score tiles takes 2.6 us: per stream 2250 cycles of softmax (490 to read the scores and find
-// the maximum, 880 for each half of the exponentials), then 1100 for 4 + 8 MMAs to the next scores; the
-// tensor pipe works in 58 % of them.  A block of one score tile takes 1.8 us, of which HBM needs 1.5.
+// Measured, B200, BF16, 64 heads over 8 of 128, 32 trees of up to 64 nodes over up to 8192 tokens: 315 us in a
+// short burst (773 TFLOP/s), 380 us in a long loop (641), where the card's power limit holds the clock at 1.5 GHz.
+// The profiled launch: 317 us, 126 blocks a CTA, 4040 cycles a block at its 1.6 GHz, the tensor pipe active in 52 %.
+// Of these a block of two score tiles takes 3500 between two others: per stream 2250 of softmax (490 to read
+// the scores and find the maximum, 880 for each half of the exponentials), then 1100 for 4 + 8 MMAs to the next
+// scores, and barriers; the rest are the ends of segments and the first scores of the next.
+// Weights are rounded to 16 bits as in attention_rows_kernel, for the same reasons.
 // 7 trees of up to 33 nodes over up to 3001 tokens, 12 heads over 4 of 64, FP16: 17.4 us with the join, bound by
 // latency (lengths and work division 1.8 us, first scores 2.3, blocks 5, sums and join 6).
 template <typename T, int DP>

@@ -522,7 +522,8 @@ HQB_API int hqb_cache_append(const hqb_paged_cache* cache, const void* k, const 
  * and lse = -inf.  Keys and values that a
  * node does not see change nothing for it, NaN and infinities among them.  q, k, v and out have
  * the cache's type; products are summed in FP32, softmax statistics kept in FP32, and the
- * weights w_j rounded to the cache's type for the product with v.
+ * weights w_j rounded to the cache's type for the product with v (in FP16 scaled first, so that
+ * they keep all their bits down to 2^-27 of the largest).  Rows of no request are not written.
  * max_new and max_context bound the requests' lengths on the host: they size the launch.  A
  * longer context is still computed in full; nodes past max_new are left out
  * (HQB_DEVERR_INDEX).  A context longer than its table row is cut (HQB_DEVERR_PAGES), and a
@@ -579,7 +580,7 @@ typedef struct hqb_lora_set {
  * an id >= adapters counts as none (HQB_DEVERR_INDEX), and so does a rank of 0; a rank past
  * max_rank is taken as max_rank (HQB_DEVERR_INDEX).  base NULL: zeros; base may be y (with the
  * same stride), otherwise they must not overlap.  x has the set's type; y and base have y_dtype (the set's type or
- * HQB_F32).  Strides are elements between tokens.  Both products are summed in FP32.  The
+ * HQB_F32).  x and y must not overlap.  Strides are elements between tokens.  Both products are summed in FP32.  The
  * inner vector a_a x[t] is kept in FP32 and enters the second product as terms of the set's
  * type: one term (HQB_F16, HQB_BF16 y) or enough of them for 22 bits (HQB_F32 y). */
 HQB_API uint64_t hqb_lora_workspace_bytes(const hqb_lora_set* set, uint32_t tokens, int device);
