@@ -53,14 +53,23 @@ class Decoder:
         self.head = progressive(VOCAB, HIDDEN, g)
         rows, rank = (HEADS + 2 * KV_HEADS) * DIM, 8
         self.lora = [hqb.LoraSet(torch.randn(requests, rank, HIDDEN, generator=g, device="cuda").mul(HIDDEN ** -0.5).half(),
-                                 torch.randn(requests, rows, rank, generator=g, device="cuda").mul(0.1).half())
+                                 torch.randn(requests, rows, rank, generator=g, device="cuda").mul(0.1).half(), max_tokens=0)
                      for _ in range(LAYERS)]
         pages = requests * -(-capacity // PAGE)
         self.caches = [hqb.PagedCache(*(torch.zeros(pages, PAGE, KV_HEADS, DIM, dtype=torch.float16, device="cuda")
                                         for _ in range(2))) for _ in range(LAYERS)]
         self.nodes = sum(BRANCH ** level for level in range(DEPTH))
         tokens = requests * self.nodes
-        self.attend = [hqb.TreeAttention(c, HEADS, requests, tokens, self.nodes, capacity) for c in self.caches]
+        # the layers follow one another, so one workspace of each kind serves them all
+        scratch: list = []
+
+        def shared(need: int) -> "hqb.Workspace":
+            if not scratch or scratch[-1].nbytes < need:
+                scratch.append(hqb.Workspace(need, clear=256))
+            return scratch[-1]
+
+        self.attend = [hqb.TreeAttention(c, HEADS, requests, tokens, self.nodes, capacity, workspace=shared) for c in self.caches]
+        self.lora_scratch = hqb.Workspace(max(s.workspace_bytes(tokens) for s in self.lora), clear=256)
         self.tree = hqb.PagePlan(requests, tokens, PAGE, pages, max_new=self.nodes)
         self.keep = hqb.PagePlan(requests, tokens, PAGE, pages)
         self.tables = torch.full((requests, -(-capacity // PAGE)), -1, dtype=torch.int32, device="cuda")
@@ -82,7 +91,7 @@ class Decoder:
         ids, kept = plan.requests[:n].contiguous(), []
         for layer in range(LAYERS):
             y = self.project(self.qkv[layer], hidden, prefix)
-            self.lora[layer].apply(hidden, ids, base=y, out=y)
+            self.lora[layer].apply(hidden, ids, base=y, out=y, workspace=self.lora_scratch)
             q, k, v = (t.view(n, -1, DIM) for t in y.split([HEADS * DIM, KV_HEADS * DIM, KV_HEADS * DIM], 1))
             mixed = self.attend[layer](q, k, v, self.tables, self.lengths, plan.starts, plan.mask)
             mixed = self.project(self.out[layer], mixed.view(n, HIDDEN), prefix)
