@@ -679,6 +679,13 @@ class StreamWorkspaces:
         self._index, self._capture = _device_index(device), bind().capture
         self.eager: dict = {}
         self.captured: dict = {}
+        self.kept: dict = {}
+
+    def given(self, ws: Workspace, stream: int) -> Workspace:
+        """A workspace that a caller brings: one that a capture uses is kept, whatever replaces it here."""
+        if self._capture(self._index, stream):
+            self.kept[ws.ptr()] = ws
+        return ws
 
     def take(self, size: int, stream: int) -> Workspace:
         """A workspace for a call of `size` on a stream."""
@@ -984,7 +991,10 @@ class LoraSet:
             kind = y_dtype or (base.dtype if base is not None else x.dtype)
             out = _result((x.shape[0], self.rows), kind, self.device, stream)
         s = torch._C._cuda_getCurrentRawStream(self._index) if stream is None else _raw_stream(stream)
-        ws = self._workspaces.take(x.shape[0], s) if workspace is None else _own_workspace(workspace, self._index)
+        if workspace is None:
+            ws = self._workspaces.take(x.shape[0], s)
+        else:
+            ws = self._workspaces.given(_own_workspace(workspace, self._index), s)
         status = self._call(self._at, ws.ptr(), ws.nbytes, self._index, s, x, ids, base, out)
         if status:
             if status == _UNFIT:

@@ -141,6 +141,24 @@ def test_captured_operators_of_attention_have_workspaces_of_their_own():
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
 
 
+def test_a_workspace_given_to_a_capture_is_kept():
+    """Also where it is the stream's own, and a later call replaces that one."""
+    x, a, b, ranks, scales, ids, base = make_lora(2, 3000, 256, 128, 5, 32, BF16, BF16)
+    s, stream = hqb.LoraSet(a, b, ranks, scales, max_tokens=0), torch.cuda.current_stream().cuda_stream
+    few = (x[:1100], ids[:1100])
+    want = s.apply(*few, base=base[:1100])
+    graph, place = torch.cuda.CUDAGraph(), s.workspace(1100, stream).ptr()
+    with torch.cuda.graph(graph):
+        out = s.apply(*few, base=base[:1100], workspace=s._ws[stream])
+    size = s.workspace(1100, stream).nbytes
+    s.apply(x, ids, base=base)
+    filler = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]  # takes what was freed
+    assert s.workspace(1, stream).ptr() != place and all(f.data_ptr() != place for f in filler)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want) and all(bool((f == 255).all()) for f in filler)
+
+
 def test_a_grown_workspace_keeps_its_error_word():
     x, a, b, ranks, scales, ids, base = make_lora(3, 3000, 256, 64, 2, 16, F16, F16, full=True)
     s = hqb.LoraSet(a, b, ranks, scales, max_tokens=0)
